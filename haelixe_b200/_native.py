@@ -41,6 +41,18 @@ class AttnShape(ctypes.Structure):
     ]
 
 
+class PagedCache(ctypes.Structure):
+    """hx_paged_cache."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("block_table", ctypes.c_void_p)] + \
+        [(n, ctypes.c_int64) for n in ("stride_page", "stride_slot", "stride_head", "table_stride")] + \
+        [(n, ctypes.c_int32) for n in ("num_pages", "page_size", "H", "D", "num_seqs", "max_pages")]
+
+
+class Rows(ctypes.Structure):
+    """hx_rows."""
+    _fields_ = [("data", ctypes.c_void_p), ("stride_row", ctypes.c_int64), ("stride_head", ctypes.c_int64)]
+
+
 class ArenaStats(ctypes.Structure):
     _fields_ = [(n, ctypes.c_uint64) for n in
                 ("live_bytes", "cached_bytes", "cached_slabs", "cached_bins", "hits", "misses")]
@@ -111,6 +123,9 @@ SIGNATURES = {
     "hx_rope_fwd": (_I, [_P, _I, _SHP, _P, _P, _F]),
     "hx_rope_bwd": (_I, [_P, _I, _SHP, _P, _P, _F]),
     "hx_rope_fwd_qk": (_I, [_P, _I, _SHP, _P, _P, _P, _P, _F]),
+    "hx_paged_append": (_I, [_P, _I, _P, _I, _P, _P, _P, _P, _I, _P, _P, _F]),
+    "hx_paged_attention_workspace_size": (_I, [_I, _P, _I, ctypes.POINTER(_U64)]),
+    "hx_paged_attention": (_I, [_P, _I, _P, _I, _P, _P, _P, _P, _F, _P, _U64]),
     "hx_reassemble_heads": (_I, [_P, _I, _P, _P, _I, _I, _I, _I, _I, _I]),
     "hx_torch_malloc": (_P, [ctypes.c_size_t, _I, _P]),
     "hx_torch_free": (None, [_P, ctypes.c_size_t, _I, _P]),

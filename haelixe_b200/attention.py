@@ -58,6 +58,7 @@ class CudaContext:
         N.check(st)
         self.handle = h.value
         self._stream = None  # raw stream last handed to hx_ctx_set_stream
+        self.lock = threading.Lock()  # held from use_stream to the call that follows it
 
     def close(self) -> None:
         if self.handle:

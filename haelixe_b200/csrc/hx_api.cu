@@ -689,6 +689,145 @@ int hx_reassemble_heads(hx_ctx* c, hx_dtype dt, const void* shards, void* out, i
                       "hx_reassemble_heads");
 }
 
+// ---- the paged key/value cache ----------------------------------------------------
+
+static int validate_cache(const hx_ctx* ctx, hx_dtype dt, const hx_paged_cache* c, const char* who) {
+    int st;
+    if ((st = validate_dtype(ctx, dt, who))) return st;
+    if (c == nullptr) return set_error(ctx, HX_ERR_INVALID, "%s: cache is NULL", who);
+    if (c->num_pages <= 0 || c->page_size <= 0 || c->H <= 0 || c->D <= 0 || c->num_seqs < 0 || c->max_pages <= 0)
+        return set_error(ctx, HX_ERR_INVALID, "%s: num_pages, page_size, H, D and max_pages must be positive", who);
+    if (c->D % 8 || c->D > 256)
+        return set_error(ctx, HX_ERR_UNSUPPORTED, "%s: head_dim %d is not a multiple of 8 up to 256", who, c->D);
+    if (c->H > 65535) return set_error(ctx, HX_ERR_UNSUPPORTED, "%s: H must be <= 65535", who);
+    const int64_t eb = dt == HX_F32 ? 4 : 2;
+    if (c->stride_slot < c->D || c->stride_head < 0 || c->stride_page < 0 || c->table_stride < 0 ||
+        (c->num_seqs > 1 && c->table_stride < c->max_pages))
+        return set_error(ctx, HX_ERR_INVALID, "%s: cache or table strides overlap their rows", who);
+    if (!c->k || !c->v || (c->num_seqs > 0 && !c->block_table))
+        return set_error(ctx, HX_ERR_INVALID, "%s: NULL cache operand", who);
+    if (!aligned16(c->k) || !aligned16(c->v) || (c->stride_page * eb) % 16 || (c->stride_slot * eb) % 16 ||
+        (c->stride_head * eb) % 16)
+        return set_error(ctx, HX_ERR_INVALID, "%s: the cache and its strides must be 16-byte aligned", who);
+    return HX_OK;
+}
+
+static hx::PagedView view_of(const hx_paged_cache& c) {
+    hx::PagedView v;
+    v.k = c.k;
+    v.v = c.v;
+    v.num_pages = c.num_pages;
+    v.page_size = c.page_size;
+    v.page_shift = (c.page_size & (c.page_size - 1)) == 0 ? __builtin_ctz((unsigned)c.page_size) : -1;
+    v.H = c.H;
+    v.D = c.D;
+    v.sp = c.stride_page;
+    v.ss = c.stride_slot;
+    v.sh = c.stride_head;
+    v.table = c.block_table;
+    v.table_stride = c.table_stride;
+    v.num_seqs = c.num_seqs;
+    v.max_pages = c.max_pages;
+    return v;
+}
+
+int hx_paged_append(hx_ctx* c, hx_dtype dt, const hx_paged_cache* cache, int tokens, const hx_rows* k,
+                    const hx_rows* v, const int32_t* seq_ids, const int32_t* positions, int Hq, const hx_rows* q,
+                    const hx_rows* q_out, float rope_base) {
+    if (c == nullptr) return HX_ERR_INVALID;
+    const char* who = "hx_paged_append";
+    int st;
+    if ((st = validate_cache(c, dt, cache, who))) return st;
+    if (tokens < 0 || Hq < 0 || Hq > 65535)
+        return set_error(c, HX_ERR_INVALID, "%s: tokens or Hq out of range", who);
+    if (!isfinite(rope_base) || rope_base < 0.f)
+        return set_error(c, HX_ERR_INVALID, "%s: rope_base must be finite and >= 0", who);
+    if (tokens == 0) return HX_OK;
+    if (!k || !v || !k->data || !v->data || !seq_ids || !positions ||
+        (Hq > 0 && (!q || !q_out || !q->data || !q_out->data)))
+        return set_error(c, HX_ERR_INVALID, "%s: NULL operand", who);
+    DeviceGuard g(c->device);
+    NvtxRange nv(who);
+    LaunchCount lc(c);
+    hx::PagedAppend a{};
+    a.cache = view_of(*cache);
+    a.k = k->data, a.k_st = k->stride_row, a.k_sh = k->stride_head;
+    a.v = v->data, a.v_st = v->stride_row, a.v_sh = v->stride_head;
+    if (Hq > 0) {
+        a.q = q->data, a.q_st = q->stride_row, a.q_sh = q->stride_head;
+        a.q_out = q_out->data, a.qo_st = q_out->stride_row, a.qo_sh = q_out->stride_head;
+    }
+    a.Hq = Hq;
+    a.rotate = rope_base > 0.f;
+    a.log2_base = a.rotate ? log2((double)rope_base) : 0.0;
+    a.seq_ids = seq_ids;
+    a.positions = positions;
+    return check_cuda(c, hx::paged_append(c->stream, c->sm_count, dt, a, tokens), who);
+}
+
+static int paged_heads(const hx_ctx* c, const hx_paged_cache* cache, int Hq, const char* who) {
+    if (Hq <= 0 || Hq % cache->H)
+        return set_error(c, HX_ERR_INVALID, "%s: Hq %d is not a multiple of the cache's %d heads", who, Hq, cache->H);
+    if ((int64_t)cache->num_seqs * Hq > INT32_MAX)
+        return set_error(c, HX_ERR_UNSUPPORTED, "%s: num_seqs * Hq must fit 31 bits", who);
+    return HX_OK;
+}
+
+int hx_paged_attention_workspace_size(hx_dtype dt, const hx_paged_cache* cache, int Hq, uint64_t* bytes) {
+    if (bytes == nullptr) return HX_ERR_INVALID;
+    int st;
+    if ((st = validate_cache(nullptr, dt, cache, "")) || (st = paged_heads(nullptr, cache, Hq, ""))) return st;
+    *bytes = hx::paged_attn_workspace_bytes(dt, Hq, cache->H, cache->D);
+    return HX_OK;
+}
+
+int hx_paged_attention(hx_ctx* c, hx_dtype dt, const hx_paged_cache* cache, int Hq, const hx_rows* q,
+                       const hx_rows* o, float* lse, const int32_t* seq_lens, float scale, void* workspace,
+                       uint64_t workspace_bytes) {
+    if (c == nullptr) return HX_ERR_INVALID;
+    const char* who = "hx_paged_attention";
+    int st;
+    if ((st = validate_cache(c, dt, cache, who)) || (st = paged_heads(c, cache, Hq, who))) return st;
+    if (!isfinite(scale)) return set_error(c, HX_ERR_INVALID, "%s: scale is not finite", who);
+    if (cache->num_seqs == 0) return HX_OK;
+    if (!q || !o || !q->data || !o->data || !seq_lens)
+        return set_error(c, HX_ERR_INVALID, "%s: NULL operand", who);
+    const int64_t eb = dt == HX_F32 ? 4 : 2;
+    if (!aligned16(q->data) || (q->stride_row * eb) % 16 || (q->stride_head * eb) % 16)
+        return set_error(c, HX_ERR_INVALID, "%s: q and its strides must be 16-byte aligned", who);
+    DeviceGuard g(c->device);
+    NvtxRange nv(who);
+    LaunchCount lc(c);
+    const uint64_t need = hx::paged_attn_workspace_bytes(dt, Hq, cache->H, cache->D);
+    void* ws = workspace;
+    if (ws == nullptr) {
+        cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+        if ((st = check_cuda(c, cudaStreamIsCapturing(c->stream, &cap), who))) return st;
+        // An arena slab goes back after the call, but a graph would keep writing to it at each replay.
+        if (cap != cudaStreamCaptureStatusNone)
+            return set_error(c, HX_ERR_INVALID, "%s: pass a workspace while the stream is captured", who);
+        if ((st = hx_alloc(c, need, &ws))) return st;
+    } else if (workspace_bytes < need) {
+        return set_error(c, HX_ERR_INVALID, "%s: workspace of %llu bytes < %llu needed", who,
+                         (unsigned long long)workspace_bytes, (unsigned long long)need);
+    } else if (((uintptr_t)ws & 255u) != 0) {
+        return set_error(c, HX_ERR_INVALID, "%s: workspace must be 256-byte aligned", who);
+    }
+    hx::PagedAttn a{};
+    a.cache = view_of(*cache);
+    a.q = q->data, a.q_sn = q->stride_row, a.q_sh = q->stride_head;
+    a.o = o->data, a.o_sn = o->stride_row, a.o_sh = o->stride_head;
+    a.lse = lse;
+    a.lens = seq_lens;
+    a.Hq = Hq;
+    a.G = Hq / cache->H;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.part = (float*)ws;
+    st = check_cuda(c, hx::paged_attn(c->stream, c->sm_count, dt, a), who);
+    if (workspace == nullptr) hx_free(c, ws);  // stream-ordered: the next user of the slab queues behind us
+    return st;
+}
+
 uint64_t hx_kernel_launches(const hx_ctx* c) { return c ? c->kernel_launches : 0; }
 
 // ---- the attention block around the kernel: Linear and RMSNorm ------------

@@ -134,6 +134,41 @@ cudaError_t col_sum(cudaStream_t st, hx_dtype dt, const void* dy, void* db, floa
 int64_t col_scratch_floats(int64_t rows, int cols);
 int64_t rmsnorm_bwd_scratch_floats(int64_t rows, int hidden);
 
+// ---- the paged key/value cache (paged_append.cu, paged_attn.cu) ----
+struct PagedView {
+    void* k;
+    void* v;
+    int num_pages, page_size, page_shift;  // page_shift: log2(page_size), -1 when not a power of two
+    int H, D;                              // key heads, head_dim
+    int64_t sp, ss, sh;                    // element strides of a page, a slot and a head
+    const int32_t* table;                  // [num_seqs, max_pages] page numbers
+    int64_t table_stride;
+    int num_seqs, max_pages;
+};
+struct PagedAppend {
+    PagedView cache;
+    const void *k, *v, *q;  // [tokens, heads, D]; q NULL when Hq is 0
+    void* q_out;
+    int64_t k_st, k_sh, v_st, v_sh, q_st, q_sh, qo_st, qo_sh;  // element strides of a token and a head
+    int Hq, rotate;
+    double log2_base;
+    const int32_t *seq_ids, *positions;
+};
+cudaError_t paged_append(cudaStream_t st, int sm_count, hx_dtype dt, const PagedAppend& a, int tokens);
+struct PagedAttn {
+    PagedView cache;
+    const void* q;  // [num_seqs, Hq, D]
+    void* o;
+    float* lse;  // [num_seqs, Hq] or NULL
+    const int32_t* lens;
+    int64_t q_sn, q_sh, o_sn, o_sh;
+    int Hq, G;  // query heads, query heads of one key head
+    float scale_log2;
+    float* part;
+};
+uint64_t paged_attn_workspace_bytes(hx_dtype dt, int Hq, int Hkv, int D);
+cudaError_t paged_attn(cudaStream_t st, int sm_count, hx_dtype dt, const PagedAttn& a);
+
 // ---- failure-path self-test (selftest.cu) ----
 cudaError_t selftest_wait_timeout(cudaStream_t st, DeviceStatus* status);
 

@@ -1,0 +1,697 @@
+// Attention of one new token per sequence over a paged key/value cache:
+// o = sum_j p_j v_j, p = softmax_j(scale q . k_j) over the first len positions
+// of the sequence, for G query heads to a key head (G = 1: every head has its own keys).
+//
+// Every key and value is read once, so the bytes of the cache bound it, and
+// the work has to be even over the SMs although lengths differ and are known
+// on the device alone. The (sequence, key head, up to HB of its query heads)
+// items are cut into tiles of 64 keys, the tiles of all items are numbered in a row,
+// and every worker (a 4-warp CTA, as many as are resident at once) takes an
+// equal run of them. A run that holds all of an item writes its result; the
+// others write (max, sum, unnormalised o) to the workspace, at most two a
+// worker, and paged_join_kernel joins an item's parts in the order of its keys
+// (no atomics: the same call gives the same bits).
+//
+// Softmax statistics and all sums are f32. A warp keeps a running maximum that
+// only moves when a score passes it by 2^8, so the accumulator is rarely rescaled.
+// Positions at or past len are never read: their pages may hold anything.
+#include <atomic>
+
+#include "hx_internal.h"
+#include "mma_bf16.cuh"
+
+namespace hx {
+namespace {
+
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kWarpKeys = 16, kTile = kWarps * kWarpKeys;
+constexpr int kMaxWorkers = 1024;
+constexpr int kMinTiles = 2;  // a run shorter than this costs more to join than it saves
+constexpr float kLazy = 8.f;  // log2 growth of the maximum that triggers a rescale
+constexpr float kLn2 = 0.69314718055994530942f;
+
+struct Item {
+    int n, h, c;  // sequence, key head, chunk of its query heads
+};
+
+// Sequences with nothing to read (len <= 0) or longer than their table row have no tiles;
+// paged_join_kernel writes their rows.
+__device__ __forceinline__ int tiles_of(const PagedAttn& a, int n) {
+    const int64_t len = a.lens[n];
+    return len <= 0 || len > (int64_t)a.cache.max_pages * a.cache.page_size ? 0 : (int)((len + kTile - 1) / kTile);
+}
+
+__device__ __forceinline__ int64_t run_of(int64_t total, int workers) {
+    const int64_t r = (total + workers - 1) / workers;
+    return r < kMinTiles ? kMinTiles : r;
+}
+
+// Sum of the tiles of the sequences [0, n) and of all; every thread of the block gets both.
+template <int THREADS>
+__device__ __forceinline__ void tile_sums(const PagedAttn& a, int n, int64_t& before, int64_t& all) {
+    __shared__ int64_t sums[2][THREADS / 32];
+    int64_t b = 0, t = 0;
+    for (int i = threadIdx.x; i < a.cache.num_seqs; i += THREADS) {
+        const int v = tiles_of(a, i);
+        t += v;
+        if (i < n) b += v;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        b += __shfl_xor_sync(0xffffffffu, b, o);
+        t += __shfl_xor_sync(0xffffffffu, t, o);
+    }
+    if (threadIdx.x % 32 == 0) sums[0][threadIdx.x / 32] = b, sums[1][threadIdx.x / 32] = t;
+    __syncthreads();
+    before = all = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) before += sums[0][w], all += sums[1][w];
+}
+
+// The sequence that holds tile `start` of the row (times `per` for each of its
+// tiles), and the number of tiles before it. start < total.
+__device__ __forceinline__ void find_sequence(const PagedAttn& a, int64_t start, int per, int& n, int64_t& before) {
+    __shared__ int64_t warp_sum[kWarps];
+    __shared__ int found_n;
+    __shared__ int64_t found_before;
+    int64_t carry = 0;
+    for (int base = 0;; base += kThreads) {
+        const int i = base + threadIdx.x;
+        const int64_t v = i < a.cache.num_seqs ? (int64_t)tiles_of(a, i) * per : 0;
+        int64_t incl = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t u = __shfl_up_sync(0xffffffffu, incl, o);
+            if ((int)(threadIdx.x % 32) >= o) incl += u;
+        }
+        if (threadIdx.x % 32 == 31) warp_sum[threadIdx.x / 32] = incl;
+        __syncthreads();
+        int64_t block = 0, prev = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < (int)(threadIdx.x / 32)) prev += warp_sum[w];
+            block += warp_sum[w];
+        }
+        incl += prev + carry;
+        if (incl - v <= start && start < incl) found_n = i, found_before = incl - v;
+        carry += block;
+        __syncthreads();
+        if (start < carry || base + kThreads >= a.cache.num_seqs) break;
+    }
+    n = found_n;
+    before = found_before;
+}
+
+// Element offset of key `key` of sequence n in the cache; kNone at or past len, kBad when
+// its table entry is no page (such a row comes out as NaN, nothing is read for it).
+constexpr int64_t kNone = -1, kBad = -2;
+__device__ __forceinline__ int entry_of(const PagedView& c, const int32_t* row, int key, int len) {
+    if (key >= len) return 0;
+    return row[c.page_shift >= 0 ? key >> c.page_shift : key / c.page_size];
+}
+__device__ __forceinline__ int64_t offset_of(const PagedView& c, int page, int key, int len) {
+    if (key >= len) return kNone;
+    if (page < 0 || page >= c.num_pages) return kBad;
+    const int slot = c.page_shift >= 0 ? key & (c.page_size - 1) : key % c.page_size;
+    return (int64_t)page * c.sp + (int64_t)slot * c.ss;
+}
+
+__device__ __forceinline__ uint4 ld_stream(const void* p) {
+    uint4 u;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                 : "l"(p));
+    return u;
+}
+
+// What a warp leaves of its keys of an item, in shared memory: o (unnormalised) in
+// [HB][D + pad], (max in log2 units, sum) of each head.
+template <int HB, int DP>
+struct Parts {
+    static constexpr int kRow = DP + 2;
+    float o[kWarps][HB * kRow];
+    float2 ml[kWarps][HB];
+};
+
+__device__ __forceinline__ float safe_max(float m) { return m == -INFINITY ? 0.f : m; }
+
+// Joins the four warps' parts: the item's output, or the worker's part of it.
+template <typename T, int HB, int DP>
+__device__ __forceinline__ void finish_item(const PagedAttn& a, const Parts<HB, DP>& sp, const Item& it, bool whole,
+                                            int slot) {
+    const int D = a.cache.D;
+    const int h0 = it.h * a.G + it.c * HB;
+    const int heads = min(HB, a.G - it.c * HB);
+    for (int i = threadIdx.x; i < heads * D; i += kThreads) {
+        const int h = i / D, d = i - h * D;
+        float m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sp.ml[w][h].x);
+        float l = 0.f, o = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float f = exp2f(sp.ml[w][h].x - safe_max(m));
+            l += f * sp.ml[w][h].y;
+            o += f * sp.o[w][h * Parts<HB, DP>::kRow + d];
+        }
+        if (whole) {
+            ((T*)a.o)[(int64_t)it.n * a.o_sn + (int64_t)(h0 + h) * a.o_sh + d] = T(o / l);
+            if (d == 0 && a.lse) a.lse[(int64_t)it.n * a.Hq + h0 + h] = (m + log2f(l)) * kLn2;
+        } else {
+            float* part = a.part + (int64_t)slot * HB * (D + 2);
+            part[h * D + d] = o;
+            if (d == 0) reinterpret_cast<float2*>(part + HB * D)[h] = make_float2(m, l);
+        }
+    }
+}
+
+// ---- bf16: the warp's 16 keys as one mma operand --------------------------------
+// S^T[16 keys, 8 heads] = K Q^T and O^T[D, 8 heads] += V^T P^T put the keys (or D)
+// on the 16-row side and the few query heads on the 8-column side of mma_bf16.
+// Both K and V^T fragments come straight from 16-byte global loads, with no
+// shared memory: the order of the summed index is free as long as both operands
+// use the same one, so lane t's 16 bytes of a key row are its columns of two products,
+// and V^T pairs the keys 2t, 2t+1 by two byte permutes. P goes from the first product's
+// layout to the second's by an 8x8 transpose, as bf16 hi + lo, so that the
+// result carries only its own rounding.
+// K of the next step is loaded as soon as the scores are taken, V as soon as P V is,
+// so one of the two is always in flight.
+template <int DC, int NT>
+struct AttnBf16 {
+    static constexpr int kD = 64 * DC;       // D rounded up; the rest reads as zero
+    static constexpr int HB = 8 * NT;
+    static constexpr int VC = DC > 2 ? 2 : DC;  // 64-wide chunks of V held at once
+
+    uint4 q[NT][2 * DC], k[2][2 * DC], v[4][VC];
+    float acc[NT][DC][4][4];
+    float m[NT][2], l[NT][2];
+    const PagedAttn& a;
+    const int32_t* row;
+    const __nv_bfloat16 *kh, *vh;
+    int len, g, t;
+
+    __device__ __forceinline__ AttnBf16(const PagedAttn& args) : a(args) {
+        g = (threadIdx.x % 32) / 4;
+        t = threadIdx.x % 4;
+    }
+
+    __device__ __forceinline__ void load_k(int64_t off) {
+        const int64_t o0 = __shfl_sync(0xffffffffu, off, g), o1 = __shfl_sync(0xffffffffu, off, g + 8);
+#pragma unroll
+        for (int b = 0; b < 2 * DC; ++b) {
+            const int d = 32 * b + 8 * t;
+            const bool in = d < a.cache.D;
+            k[0][b] = in && o0 >= 0 ? ld_stream(kh + o0 + d) : make_uint4(0, 0, 0, 0);
+            k[1][b] = in && o1 >= 0 ? ld_stream(kh + o1 + d) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    __device__ __forceinline__ void load_v(int64_t off, int c0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t o = __shfl_sync(0xffffffffu, off, 2 * t + (j & 1) + 8 * (j >> 1));
+#pragma unroll
+            for (int c = 0; c < VC; ++c) {
+                const int d = 64 * (c0 + c) + 8 * g;
+                v[j][c] = o >= 0 && d < a.cache.D ? ld_stream(vh + o + d) : make_uint4(0, 0, 0, 0);
+            }
+        }
+    }
+
+    __device__ __forceinline__ void run(const Item& it, int tile, int tiles, Parts<HB, kD>& sp) {
+        const PagedView& c = a.cache;
+        const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+        len = a.lens[it.n];
+        row = c.table + (int64_t)it.n * c.table_stride;
+        kh = (const __nv_bfloat16*)c.k + (int64_t)it.h * c.sh;
+        vh = (const __nv_bfloat16*)c.v + (int64_t)it.h * c.sh;
+        const int h0 = it.h * a.G + it.c * HB, heads = min(HB, a.G - it.c * HB);
+        // Key of this lane (16 of them) at step i: tile * 64 + 64 i + 16 warp + lane % 16.
+        int key = tile * kTile + warp * kWarpKeys + lane % 16;
+        int page = entry_of(c, row, key, len);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int b = 0; b < 2 * DC; ++b) {
+                const int d = 32 * b + 8 * t;
+                q[n][b] = 8 * n + g < heads && d < c.D
+                              ? *reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.q + (int64_t)it.n * a.q_sn +
+                                                                (int64_t)(h0 + 8 * n + g) * a.q_sh + d)
+                              : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+            for (int x = 0; x < DC; ++x)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[n][x][e][r] = 0.f;
+        }
+        int64_t off = offset_of(c, page, key, len);
+        load_k(off);
+        load_v(off, 0);
+        page = entry_of(c, row, key + kTile, len);
+        for (int i = 0; i < tiles; ++i) {
+            const uint32_t bad = __ballot_sync(0xffffffffu, off == kBad);
+            const uint32_t none = __ballot_sync(0xffffffffu, off == kNone);
+            // scores, in log2 units: s[n][0..1] key g, heads 2t, 2t+1; s[n][2..3] key g + 8
+            float s[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[n][r] = 0.f;
+#pragma unroll
+                for (int b = 0; b < 2 * DC; ++b) {
+                    mma_bf16(s[n], k[0][b].x, k[1][b].x, k[0][b].y, k[1][b].y, q[n][b].x, q[n][b].y);
+                    mma_bf16(s[n], k[0][b].z, k[1][b].z, k[0][b].w, k[1][b].w, q[n][b].z, q[n][b].w);
+                }
+            }
+            const int64_t off_now = off;
+            const bool more = i + 1 < tiles;
+            if (more) {
+                key += kTile;
+                off = offset_of(c, page, key, len);
+                load_k(off);
+                if (i + 2 < tiles) page = entry_of(c, row, key + kTile, len);
+            }
+            uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int kk = g + 8 * (r >> 1);
+                    s[n][r] *= a.scale_log2;
+                    if (bad >> kk & 1) s[n][r] = __int_as_float(0x7fffffff);
+                    if (none >> kk & 1) s[n][r] = -INFINITY;
+                }
+                float mx[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    mx[r] = fmaxf(s[n][r], s[n][r + 2]);
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], o));
+                }
+                if (__any_sync(0xffffffffu, mx[0] > m[n][0] + kLazy || mx[1] > m[n][1] + kLazy)) {
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const float mn = fmaxf(m[n][r], mx[r]);
+                        const float f = exp2f(m[n][r] - safe_max(mn));
+                        m[n][r] = mn;
+                        l[n][r] *= f;
+#pragma unroll
+                        for (int x = 0; x < DC; ++x)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                acc[n][x][e][r] *= f;
+                                acc[n][x][e][r + 2] *= f;
+                            }
+                    }
+                }
+                const float m0 = safe_max(m[n][0]), m1 = safe_max(m[n][1]);
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float p0 = exp2f(s[n][2 * r] - m0), p1 = exp2f(s[n][2 * r + 1] - m1);
+                    l[n][0] += p0;
+                    l[n][1] += p1;
+                    const uint32_t hi = pack_bf16(p0, p1);
+                    const float2 back = unpack_bf16(hi);
+                    ph[n][r] = transpose8x8(hi);
+                    pl[n][r] = transpose8x8(pack_bf16(p0 - back.x, p1 - back.y));
+                }
+            }
+#pragma unroll
+            for (int c0 = 0; c0 < DC; c0 += VC) {
+                if (c0 > 0) load_v(off_now, c0);
+#pragma unroll
+                for (int x = 0; x < VC; ++x) {
+                    const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&v[0][x]);
+                    const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&v[1][x]);
+                    const uint32_t* w2 = reinterpret_cast<const uint32_t*>(&v[2][x]);
+                    const uint32_t* w3 = reinterpret_cast<const uint32_t*>(&v[3][x]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t a0 = pair_lo(w0[e], w1[e]), a1 = pair_hi(w0[e], w1[e]);
+                        const uint32_t a2 = pair_lo(w2[e], w3[e]), a3 = pair_hi(w2[e], w3[e]);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            mma_bf16(acc[n][c0 + x][e], a0, a1, a2, a3, ph[n][0], ph[n][1]);
+                            mma_bf16(acc[n][c0 + x][e], a0, a1, a2, a3, pl[n][0], pl[n][1]);
+                        }
+                    }
+                }
+            }
+            if (more) load_v(off, 0);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) l[n][r] += __shfl_xor_sync(0xffffffffu, l[n][r], o);
+                const int h = 8 * n + 2 * t + r;
+                if (g == 0) sp.ml[warp][h] = make_float2(m[n][r], l[n][r]);
+#pragma unroll
+                for (int x = 0; x < DC; ++x)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        *reinterpret_cast<float2*>(&sp.o[warp][h * Parts<HB, kD>::kRow + 64 * x + 8 * g + 2 * e]) =
+                            make_float2(acc[n][x][e][r], acc[n][x][e][r + 2]);
+            }
+        }
+    }
+};
+
+// ---- f32: scores and sums in f32 on the FMA pipes ---------------------------------
+// Lane 4 g + t takes keys g and g + 8 and every fourth 16-byte piece of their rows;
+// the scores pass through shared memory to a layout with four lanes a head, and the
+// probabilities back as one broadcast read a key. Lane l owns DV elements of o.
+template <int GH, int DV>
+struct AttnF32 {
+    static constexpr int kD = 32 * DV;
+    static constexpr int HB = GH;
+
+    struct alignas(16) Scratch {
+        float q[GH][kD];
+        float s[kWarps][GH][kWarpKeys];
+        float p[kWarps][kWarpKeys][GH];
+        float f[kWarps][GH];
+    };
+
+    const PagedAttn& a;
+    Scratch& sm;
+    __device__ __forceinline__ AttnF32(const PagedAttn& args, Scratch& scratch) : a(args), sm(scratch) {}
+
+    __device__ __forceinline__ void run(const Item& it, int tile, int tiles, Parts<HB, kD>& sp) {
+        const PagedView& c = a.cache;
+        const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
+        const int len = a.lens[it.n], D = c.D;
+        const int32_t* row = c.table + (int64_t)it.n * c.table_stride;
+        const float* kh = (const float*)c.k + (int64_t)it.h * c.sh;
+        const float* vh = (const float*)c.v + (int64_t)it.h * c.sh;
+        const int h0 = it.h * a.G + it.c * HB, heads = min(HB, a.G - it.c * HB);
+        for (int i = threadIdx.x; i < GH * kD; i += kThreads) {
+            const int h = i / kD, d = i % kD;
+            sm.q[h][d] = h < heads && d < D
+                             ? ((const float*)a.q)[(int64_t)it.n * a.q_sn + (int64_t)(h0 + h) * a.q_sh + d]
+                             : 0.f;
+        }
+        __syncthreads();
+        // max and sum of head lane / 4 (the same in its four lanes, the sum after the loop)
+        const int hs = lane / 4;
+        const bool has = hs < GH;
+        float m = -INFINITY, l = 0.f;
+        float acc[GH][DV];
+#pragma unroll
+        for (int h = 0; h < GH; ++h)
+#pragma unroll
+            for (int x = 0; x < DV; ++x) acc[h][x] = 0.f;
+        int key = tile * kTile + warp * kWarpKeys + lane % 16;
+        int page = entry_of(c, row, key, len);
+        for (int i = 0; i < tiles; ++i) {
+            const int64_t off = offset_of(c, page, key, len);
+            key += kTile;
+            if (i + 1 < tiles) page = entry_of(c, row, key, len);
+            const uint32_t bad = __ballot_sync(0xffffffffu, off == kBad);
+            const uint32_t none = __ballot_sync(0xffffffffu, off == kNone);
+            const int64_t o0 = __shfl_sync(0xffffffffu, off, g), o1 = __shfl_sync(0xffffffffu, off, g + 8);
+            float s0[GH], s1[GH];
+#pragma unroll
+            for (int h = 0; h < GH; ++h) s0[h] = s1[h] = 0.f;
+#pragma unroll
+            for (int j = 0; j < kD / 16; ++j) {
+                const int d = 16 * j + 4 * t;
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+                if (d < D) {
+                    if (o0 >= 0) x = *reinterpret_cast<const float4*>(kh + o0 + d);
+                    if (o1 >= 0) y = *reinterpret_cast<const float4*>(kh + o1 + d);
+                }
+#pragma unroll
+                for (int h = 0; h < GH; ++h) {
+                    const float4 w = *reinterpret_cast<const float4*>(&sm.q[h][d]);
+                    s0[h] = fmaf(x.x, w.x, fmaf(x.y, w.y, fmaf(x.z, w.z, fmaf(x.w, w.w, s0[h]))));
+                    s1[h] = fmaf(y.x, w.x, fmaf(y.y, w.y, fmaf(y.z, w.z, fmaf(y.w, w.w, s1[h]))));
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < GH; ++h) {
+#pragma unroll
+                for (int o = 1; o < 4; o <<= 1) {
+                    s0[h] += __shfl_xor_sync(0xffffffffu, s0[h], o);
+                    s1[h] += __shfl_xor_sync(0xffffffffu, s1[h], o);
+                }
+                if (t == 0) sm.s[warp][h][g] = s0[h], sm.s[warp][h][g + 8] = s1[h];
+            }
+            __syncwarp();
+            float f = 1.f;
+            if (has) {
+                float s[4], mx = -INFINITY;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int kk = 4 * t + r;
+                    s[r] = sm.s[warp][hs][kk] * a.scale_log2;
+                    if (bad >> kk & 1) s[r] = __int_as_float(0x7fffffff);
+                    if (none >> kk & 1) s[r] = -INFINITY;
+                    mx = fmaxf(mx, s[r]);
+                }
+                const uint32_t active = GH == 8 ? 0xffffffffu : (1u << (4 * GH)) - 1u;
+                mx = fmaxf(mx, __shfl_xor_sync(active, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(active, mx, 2));
+                const float mn = fmaxf(m, mx);
+                f = exp2f(m - safe_max(mn));
+                m = mn;
+                l *= f;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float p = exp2f(s[r] - safe_max(m));
+                    l += p;
+                    sm.p[warp][4 * t + r][hs] = p;
+                }
+                if (t == 0) sm.f[warp][hs] = f;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int h = 0; h < GH; ++h) {
+                const float fh = sm.f[warp][h];
+#pragma unroll
+                for (int x = 0; x < DV; ++x) acc[h][x] *= fh;
+            }
+#pragma unroll
+            for (int kk = 0; kk < kWarpKeys; ++kk) {
+                const int64_t o = __shfl_sync(0xffffffffu, off, kk);
+                float v[DV];
+#pragma unroll
+                for (int x = 0; x < DV; ++x) v[x] = 0.f;
+                if (o >= 0) {
+                    if constexpr (DV == 2) {
+                        if (2 * lane < D) {
+                            const float2 u = *reinterpret_cast<const float2*>(vh + o + 2 * lane);
+                            v[0] = u.x, v[1] = u.y;
+                        }
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < DV; x += 4) {
+                            const int d = 32 * x + 4 * lane;
+                            if (d < D) {
+                                const float4 u = *reinterpret_cast<const float4*>(vh + o + d);
+                                v[x] = u.x, v[x + 1] = u.y, v[x + 2] = u.z, v[x + 3] = u.w;
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < GH; ++h) {
+                    const float p = sm.p[warp][kk][h];
+#pragma unroll
+                    for (int x = 0; x < DV; ++x) acc[h][x] = fmaf(p, v[x], acc[h][x]);
+                }
+            }
+            __syncwarp();
+        }
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        if (has && t == 0) sp.ml[warp][hs] = make_float2(m, l);
+#pragma unroll
+        for (int h = 0; h < GH; ++h)
+#pragma unroll
+            for (int x = 0; x < DV; ++x) {
+                const int d = DV == 2 ? 2 * lane + x : 32 * (x & ~3) + 4 * lane + (x & 3);
+                sp.o[warp][h * Parts<HB, kD>::kRow + d] = acc[h][x];
+            }
+    }
+};
+
+template <typename T, typename W>
+__device__ __forceinline__ void paged_worker(const PagedAttn& a, W& w, Parts<W::HB, W::kD>& sp) {
+    const int chunks = (a.G + W::HB - 1) / W::HB;
+    const int per = a.cache.H * chunks;
+    int64_t before, total;
+    tile_sums<kThreads>(a, 0, before, total);
+    total *= per;
+    const int64_t run = run_of(total, gridDim.x);
+    const int64_t start = run * blockIdx.x, end = min(total, start + run);
+    if (start >= end) return;
+    int n;
+    find_sequence(a, start, per, n, before);
+    int T_n = tiles_of(a, n);
+    int item = (int)((start - before) / T_n), tile = (int)((start - before) % T_n);
+    for (int64_t at = start; at < end;) {
+        const int tiles = (int)min((int64_t)(T_n - tile), end - at);
+        const Item it{n, item / chunks, item % chunks};
+        w.run(it, tile, tiles, sp);
+        __syncthreads();
+        finish_item<T, W::HB, W::kD>(a, sp, it, tiles == T_n, 2 * blockIdx.x + (at != start));
+        __syncthreads();
+        at += tiles;
+        tile = 0;
+        if (++item == per && at < end) {
+            item = 0;
+            do {
+                if (++n == a.cache.num_seqs) return;
+                T_n = tiles_of(a, n);
+            } while (T_n == 0);
+        }
+    }
+}
+
+template <int DC, int NT>
+__global__ void __launch_bounds__(kThreads) paged_attn_bf16_kernel(PagedAttn a) {
+    __shared__ Parts<8 * NT, 64 * DC> sp;
+    AttnBf16<DC, NT> w(a);
+    paged_worker<__nv_bfloat16>(a, w, sp);
+}
+
+template <int GH, int DV>
+__global__ void __launch_bounds__(kThreads) paged_attn_f32_kernel(PagedAttn a) {
+    using W = AttnF32<GH, DV>;
+    __shared__ Parts<GH, 32 * DV> sp;
+    __shared__ typename W::Scratch scratch;
+    W w(a, scratch);
+    paged_worker<float>(a, w, sp);
+}
+
+// One CTA a query head of a sequence: the join of its item's parts, the zeros of an
+// empty sequence, or the NaN of one that is longer than its table row.
+constexpr int kJoinThreads = 256;
+template <typename T, int HB>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedAttn a, int workers) {
+    constexpr int kJoinWarps = kJoinThreads / 32;
+    __shared__ float so[kJoinWarps][256];
+    __shared__ float2 sml[kJoinWarps];
+    const int n = blockIdx.x / a.Hq, hq = blockIdx.x % a.Hq, D = a.cache.D;
+    const int chunks = (a.G + HB - 1) / HB, per = a.cache.H * chunks;
+    T* o = (T*)a.o + (int64_t)n * a.o_sn + (int64_t)hq * a.o_sh;
+    float* lse = a.lse ? a.lse + (int64_t)n * a.Hq + hq : nullptr;
+    const int T_n = tiles_of(a, n);
+    if (T_n == 0) {
+        const bool empty = a.lens[n] <= 0;
+        const float nan = __int_as_float(0x7fffffff);
+        for (int d = threadIdx.x; d < D; d += kJoinThreads) o[d] = T(empty ? 0.f : nan);
+        if (threadIdx.x == 0 && lse) *lse = empty ? -INFINITY : nan;
+        return;
+    }
+    int64_t before, total;
+    tile_sums<kJoinThreads>(a, n, before, total);
+    const int64_t run = run_of(total * per, workers);
+    const int in_group = hq % a.G;
+    const int64_t first = before * per + ((int64_t)(hq / a.G) * chunks + in_group / HB) * T_n, last = first + T_n - 1;
+    const int w0 = (int)(first / run), w1 = min((int)(last / run), workers - 1);
+    if (w0 == w1) return;  // one worker had it all
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, head = in_group % HB;
+    float m = -INFINITY, l = 0.f, acc[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) acc[x] = 0.f;
+    // Warp w takes the parts w0 + w, w0 + w + 8, ...; lane l the elements l, l + 32, ...
+    for (int w = w0 + warp; w <= w1; w += kJoinWarps) {
+        const int slot = 2 * w + (first > run * w);
+        const float* part = a.part + (int64_t)slot * HB * (D + 2);
+        const float2 ml = reinterpret_cast<const float2*>(part + HB * D)[head];
+        const float mn = fmaxf(m, ml.x);
+        const float f0 = exp2f(m - safe_max(mn)), f1 = exp2f(ml.x - safe_max(mn));
+        m = mn;
+        l = l * f0 + ml.y * f1;
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+            if (lane + 32 * x < D) acc[x] = acc[x] * f0 + part[head * D + lane + 32 * x] * f1;
+    }
+#pragma unroll
+    for (int x = 0; x < 8; ++x)
+        if (lane + 32 * x < D) so[warp][lane + 32 * x] = acc[x];
+    if (lane == 0) sml[warp] = make_float2(m, l);
+    __syncthreads();
+    m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, sml[w].x);
+    l = 0.f;
+    float f[kJoinWarps];
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+        f[w] = exp2f(sml[w].x - safe_max(m));
+        l += f[w] * sml[w].y;
+    }
+    for (int d = threadIdx.x; d < D; d += kJoinThreads) {
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) s += f[w] * so[w][d];
+        o[d] = T(s / l);
+    }
+    if (threadIdx.x == 0 && lse) *lse = (m + log2f(l)) * kLn2;
+}
+
+template <typename T, int HB, void (*KERNEL)(PagedAttn)>
+cudaError_t launch(cudaStream_t st, int sm_count, const PagedAttn& a) {
+    static std::atomic<int> known{0};  // CTAs resident on an SM, a property of the kernel alone
+    int resident = known.load(std::memory_order_relaxed);
+    cudaError_t e;
+    if (resident == 0) {
+        if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, KERNEL, kThreads, 0)) != cudaSuccess) return e;
+        known.store(resident, std::memory_order_relaxed);
+    }
+    int workers = sm_count * resident;
+    if (workers > kMaxWorkers) workers = kMaxWorkers;
+    KERNEL<<<workers, kThreads, 0, st>>>(a);
+    note_launch();
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    paged_join_kernel<T, HB><<<(unsigned)(a.cache.num_seqs * a.Hq), kJoinThreads, 0, st>>>(a, workers);
+    note_launch();
+    return cudaGetLastError();
+}
+
+// Query heads that one worker takes at once: a multiple of the mma's 8 columns in bf16
+// (16 where the registers allow it, so that the keys are still read once), up to 8 in f32.
+int heads_at_once(hx_dtype dt, int G, int D) {
+    if (dt == HX_BF16) return G > 8 && D <= 128 ? 16 : 8;
+    return G == 1 ? 1 : G <= 4 ? 4 : 8;
+}
+
+}  // namespace
+
+uint64_t paged_attn_workspace_bytes(hx_dtype dt, int Hq, int Hkv, int D) {
+    return (uint64_t)2 * kMaxWorkers * heads_at_once(dt, Hq / Hkv, D) * (D + 2) * sizeof(float);
+}
+
+cudaError_t paged_attn(cudaStream_t st, int sm_count, hx_dtype dt, const PagedAttn& a) {
+    const int D = a.cache.D, hb = heads_at_once(dt, a.G, D);
+    if (dt == HX_BF16) {
+        if (hb == 16)
+            return D <= 64 ? launch<__nv_bfloat16, 16, paged_attn_bf16_kernel<1, 2>>(st, sm_count, a)
+                           : launch<__nv_bfloat16, 16, paged_attn_bf16_kernel<2, 2>>(st, sm_count, a);
+        return D <= 64    ? launch<__nv_bfloat16, 8, paged_attn_bf16_kernel<1, 1>>(st, sm_count, a)
+               : D <= 128 ? launch<__nv_bfloat16, 8, paged_attn_bf16_kernel<2, 1>>(st, sm_count, a)
+                          : launch<__nv_bfloat16, 8, paged_attn_bf16_kernel<4, 1>>(st, sm_count, a);
+    }
+    if (hb == 1)
+        return D <= 64    ? launch<float, 1, paged_attn_f32_kernel<1, 2>>(st, sm_count, a)
+               : D <= 128 ? launch<float, 1, paged_attn_f32_kernel<1, 4>>(st, sm_count, a)
+                          : launch<float, 1, paged_attn_f32_kernel<1, 8>>(st, sm_count, a);
+    if (hb == 4)
+        return D <= 64    ? launch<float, 4, paged_attn_f32_kernel<4, 2>>(st, sm_count, a)
+               : D <= 128 ? launch<float, 4, paged_attn_f32_kernel<4, 4>>(st, sm_count, a)
+                          : launch<float, 4, paged_attn_f32_kernel<4, 8>>(st, sm_count, a);
+    return D <= 64    ? launch<float, 8, paged_attn_f32_kernel<8, 2>>(st, sm_count, a)
+           : D <= 128 ? launch<float, 8, paged_attn_f32_kernel<8, 4>>(st, sm_count, a)
+                      : launch<float, 8, paged_attn_f32_kernel<8, 8>>(st, sm_count, a);
+}
+
+}  // namespace hx

@@ -227,6 +227,64 @@ int hx_rope_bwd(hx_ctx* ctx, hx_dtype dtype, const hx_attn_shape* shape, const v
 int hx_rope_fwd_qk(hx_ctx* ctx, hx_dtype dtype, const hx_attn_shape* shape, const void* q, const void* k,
                    void* q_out, void* k_out, float base);
 
+/* ---- the paged key/value cache (attention one token at a time) ------------------ */
+/* Keys and values of many sequences in pages of page_size positions. Element
+ * (page, slot, head, d) is at page * stride_page + slot * stride_slot +
+ * head * stride_head + d of k and of v, so both [page, slot, head, d] and
+ * [page, head, slot, d] storage fit. block_table[s * table_stride + c] is the
+ * page that holds positions [c * page_size, (c + 1) * page_size) of sequence
+ * s, c < max_pages. Pages may be shared between sequences, and entries that no
+ * position of a call reaches may hold anything. k, v and the strides (in
+ * bytes) are multiples of 16, D is a multiple of 8, at most 256. The reference
+ * has no cache: it attends over the whole sequence each time (src/nn/attention.rs:46-98). */
+typedef struct hx_paged_cache {
+    void* k;
+    void* v;
+    const int32_t* block_table; /* device, [num_seqs, max_pages] */
+    int64_t stride_page, stride_slot, stride_head, table_stride; /* elements */
+    int32_t num_pages, page_size, H, D; /* H: key heads */
+    int32_t num_seqs, max_pages;
+} hx_paged_cache;
+
+/* Element strides of a [rows, heads, D] operand, D contiguous. */
+typedef struct hx_rows {
+    void* data;
+    int64_t stride_row, stride_head;
+} hx_rows;
+
+/* Writes k and v of `tokens` new tokens ([tokens, H, D]) to the slots of their
+ * positions: token t is position positions[t] of sequence seq_ids[t] (device,
+ * int32). With rope_base > 0, k is rotated by its position first (the pairs of
+ * hx_rope_fwd; the angle is formed in f64, so far positions keep their
+ * accuracy), and q ([tokens, Hq, D]; NULL with Hq 0) is rotated into q_out
+ * (which may be q itself). rope_base 0 writes k, and copies q, as they are.
+ * A token with a negative seq_id is padding: neither the cache nor its q_out
+ * row is touched. A token without a slot (sequence or position outside the
+ * table, an entry that is no page) writes nothing to the cache and NaN to its
+ * q_out row. Two tokens of a call with the same slot leave either's values. */
+int hx_paged_append(hx_ctx* ctx, hx_dtype dtype, const hx_paged_cache* cache, int tokens, const hx_rows* k,
+                    const hx_rows* v, const int32_t* seq_ids, const int32_t* positions, int Hq, const hx_rows* q,
+                    const hx_rows* q_out, float rope_base);
+
+/* Bytes of device workspace hx_paged_attention needs for Hq query heads. */
+int hx_paged_attention_workspace_size(hx_dtype dtype, const hx_paged_cache* cache, int Hq, uint64_t* bytes);
+
+/* o[s] = softmax(scale * q[s] k^T) v over the first seq_lens[s] positions of
+ * every sequence s < num_seqs (device, int32): the attention of
+ * hx_flash_attention_fwd for one query a sequence. Query head h reads key head
+ * h / (Hq / H); Hq is a multiple of H. lse (f32 [num_seqs, Hq], may be NULL)
+ * receives the log-sum-exp of the scaled scores. A sequence with seq_lens <= 0
+ * gives zeros and an lse of -inf; one that is longer than its table row, or
+ * that reads an entry that is no page, gives NaN. Positions at or past
+ * seq_lens are not read. The result does not depend on what else is in the
+ * batch beyond f32 rounding, and equal calls give equal bits. workspace
+ * (256-byte aligned) may be NULL, except during stream capture: the call then
+ * takes it from the context's arena. Calls that overlap on the GPU need
+ * workspaces of their own. */
+int hx_paged_attention(hx_ctx* ctx, hx_dtype dtype, const hx_paged_cache* cache, int Hq, const hx_rows* q,
+                       const hx_rows* o, float* lse, const int32_t* seq_lens, float scale, void* workspace,
+                       uint64_t workspace_bytes);
+
 /* ---- the attention block around the kernel (src/nn/attention.rs:46-98) ------------ */
 /* y[rows, out] = x[rows, in] w[in, out] + b[out] (Linear::forward,
  * src/nn/linear.rs:54-56, weight stored [in, out] as in linear.rs:41); b may be
