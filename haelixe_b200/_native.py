@@ -114,6 +114,10 @@ SIGNATURES = {
     "hx_rmsnorm_bwd": (_I, [_P, _I, _P, _P, _P, _P, _P, _I, _I, _F]),
     "hx_linear_residual_fwd": (_I, [_P, _I, _P, _P, _P, _P, _P, _I, _I, _I]),
     "hx_cross_entropy": (_I, [_P, _I, _P, _P, _P, _P, _I, _I]),
+    "hx_token_logprobs_fwd": (_I, [_P, _I, _P, ctypes.c_int64, _P, _P, _P, _P, _I, _P, _P, _I, _I]),
+    "hx_token_logprobs_bwd": (_I, [_P, _I, _P, ctypes.c_int64, _P, _P, _P, _P, _P, ctypes.c_int64, _I, _I]),
+    "hx_linear_w4_fwd": (_I, [_P, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I]),
+    "hx_quantize_w4": (_I, [_P, _I, _P, _P, _P, _I, _I, _I]),
     "hx_adamw_step": (_I, [_P, _P, _I, _F, _F, _F, _F, _F, _I]),
     "hx_embedding_fwd": (_I, [_P, _I, _P, _P, _P, _U64, _I, _I]),
     "hx_embedding_bwd": (_I, [_P, _I, _P, _P, _P, _U64, _I, _I]),

@@ -966,6 +966,40 @@ int hx_linear_bwd(hx_ctx* c, hx_dtype dt, const void* x, const void* w, const vo
     return st;
 }
 
+static int w4_args(hx_ctx* c, hx_dtype dt, int rows, int in, int out, int group, const char* who) {
+    int st;
+    if ((st = linear_args(c, dt, rows, in, out, who))) return st;
+    if (group <= 0 || group % 32)
+        return set_error(c, HX_ERR_INVALID, "%s: group %d is not a multiple of 32", who, group);
+    if (rows > 32 * 65535) return set_error(c, HX_ERR_UNSUPPORTED, "%s: more than %d rows", who, 32 * 65535);
+    return HX_OK;
+}
+
+int hx_linear_w4_fwd(hx_ctx* c, hx_dtype dt, const void* x, const uint32_t* packed, const void* scales, const void* b,
+                     const void* residual, void* y, int rows, int in_features, int out_features, int group) {
+    int st;
+    if ((st = w4_args(c, dt, rows, in_features, out_features, group, "hx_linear_w4_fwd"))) return st;
+    if (!x || !packed || !scales || !y) return set_error(c, HX_ERR_INVALID, "hx_linear_w4_fwd: NULL operand");
+    DeviceGuard g(c->device);
+    NvtxRange nv("hx_linear_w4_fwd");
+    LaunchCount lc(c);
+    return check_cuda(c, hx::linear_w4(c->stream, c->sm_count, dt, x, packed, scales, b, residual, y, rows,
+                                       in_features, out_features, group),
+                      "hx_linear_w4_fwd");
+}
+
+int hx_quantize_w4(hx_ctx* c, hx_dtype dt, const void* w, uint32_t* packed, void* scales, int in_features,
+                   int out_features, int group) {
+    int st;
+    if ((st = w4_args(c, dt, 1, in_features, out_features, group, "hx_quantize_w4"))) return st;
+    if (!w || !packed || !scales) return set_error(c, HX_ERR_INVALID, "hx_quantize_w4: NULL operand");
+    DeviceGuard g(c->device);
+    NvtxRange nv("hx_quantize_w4");
+    LaunchCount lc(c);
+    return check_cuda(c, hx::quantize_w4(c->stream, dt, w, packed, scales, in_features, out_features, group),
+                      "hx_quantize_w4");
+}
+
 int hx_rmsnorm_fwd(hx_ctx* c, hx_dtype dt, const void* x, const void* w, void* y, int rows, int hidden,
                    float eps) {
     if (c == nullptr) return HX_ERR_INVALID;
@@ -1083,6 +1117,54 @@ int hx_cross_entropy(hx_ctx* c, hx_dtype dt, const void* logits, const uint32_t*
                     "hx_cross_entropy");
     hx_free(c, row_loss);
     return st;
+}
+
+static int logprobs_args(hx_ctx* c, hx_dtype dt, int64_t stride, int rows, int classes, const char* who) {
+    if (c == nullptr) return HX_ERR_INVALID;
+    int st;
+    if ((st = validate_dtype(c, dt, who))) return st;
+    if (rows < 0 || classes <= 0)
+        return set_error(c, HX_ERR_INVALID, "%s: rows must be >= 0 and classes positive", who);
+    if (classes > (1 << 30)) return set_error(c, HX_ERR_UNSUPPORTED, "%s: more than 2^30 classes", who);
+    if (rows > 1 && stride < classes) return set_error(c, HX_ERR_INVALID, "%s: rows of logits overlap", who);
+    return HX_OK;
+}
+
+int hx_token_logprobs_fwd(hx_ctx* c, hx_dtype dt, const void* logits, int64_t row_stride, const uint32_t* targets,
+                          float* logprob, float* entropy, float* stats, int top_k, int32_t* top_ids,
+                          float* top_logprobs, int rows, int classes) {
+    const char* who = "hx_token_logprobs_fwd";
+    int st;
+    if ((st = logprobs_args(c, dt, row_stride, rows, classes, who))) return st;
+    if (top_k < 0 || top_k > 32 || top_k > classes)
+        return set_error(c, HX_ERR_INVALID, "%s: top_k must be 0 to 32 and at most classes", who);
+    if (rows == 0) return HX_OK;
+    if (!logits || !targets || !logprob || !entropy || (top_k > 0 && (!top_ids || !top_logprobs)))
+        return set_error(c, HX_ERR_INVALID, "%s: NULL operand", who);
+    DeviceGuard g(c->device);
+    NvtxRange nv(who);
+    LaunchCount lc(c);
+    return check_cuda(c, hx::token_logprobs_fwd(c->stream, dt, logits, row_stride, targets, logprob, entropy, stats,
+                                                top_k, top_ids, top_logprobs, rows, classes),
+                      who);
+}
+
+int hx_token_logprobs_bwd(hx_ctx* c, hx_dtype dt, const void* logits, int64_t row_stride, const uint32_t* targets,
+                          const float* stats, const float* g_logprob, const float* g_entropy, void* dlogits,
+                          int64_t drow_stride, int rows, int classes) {
+    const char* who = "hx_token_logprobs_bwd";
+    int st;
+    if ((st = logprobs_args(c, dt, row_stride, rows, classes, who)) ||
+        (st = logprobs_args(c, dt, drow_stride, rows, classes, who)))
+        return st;
+    if (rows == 0) return HX_OK;
+    if (!logits || !targets || !stats || !dlogits) return set_error(c, HX_ERR_INVALID, "%s: NULL operand", who);
+    DeviceGuard g(c->device);
+    NvtxRange nv(who);
+    LaunchCount lc(c);
+    return check_cuda(c, hx::token_logprobs_bwd(c->stream, c->sm_count, dt, logits, row_stride, targets, stats,
+                                                g_logprob, g_entropy, dlogits, drow_stride, rows, classes),
+                      who);
 }
 
 // f32 a^n by binary exponentiation with one rounding per product: the

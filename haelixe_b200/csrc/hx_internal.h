@@ -169,6 +169,22 @@ struct PagedAttn {
 uint64_t paged_attn_workspace_bytes(hx_dtype dt, int Hq, int Hkv, int D);
 cudaError_t paged_attn(cudaStream_t st, int sm_count, hx_dtype dt, const PagedAttn& a);
 
+// ---- log probabilities of given tokens (logprobs.cu) ----
+// stats: 3 floats a row (maximum, log of the sum relative to it, entropy), for the backward.
+cudaError_t token_logprobs_fwd(cudaStream_t st, hx_dtype dt, const void* logits, int64_t stride, const uint32_t* targets,
+                               float* logprob, float* entropy, float* stats, int top, int32_t* top_ids,
+                               float* top_logprobs, int rows, int classes);
+cudaError_t token_logprobs_bwd(cudaStream_t st, int sm_count, hx_dtype dt, const void* logits, int64_t stride,
+                               const uint32_t* targets, const float* stats, const float* g_logprob,
+                               const float* g_entropy, void* dlogits, int64_t dstride, int rows, int classes);
+
+// ---- Linear with 4-bit weights (linear_w4.cu) ----
+cudaError_t linear_w4(cudaStream_t st, int sm_count, hx_dtype dt, const void* x, const uint32_t* packed,
+                      const void* scales, const void* bias, const void* residual, void* y, int rows, int in, int out,
+                      int group);
+cudaError_t quantize_w4(cudaStream_t st, hx_dtype dt, const void* w, uint32_t* packed, void* scales, int in, int out,
+                        int group);
+
 // ---- failure-path self-test (selftest.cu) ----
 cudaError_t selftest_wait_timeout(cudaStream_t st, DeviceStatus* status);
 

@@ -18,7 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -38,6 +38,15 @@ def _ctx(t: torch.Tensor):
     c = context(t.device.index)
     c.use_stream()
     return c
+
+
+def _context_of(t: torch.Tensor):
+    """The context of t's device; the caller holds its lock from use_stream to the call."""
+    if not t.is_cuda:
+        raise RuntimeError("the attention block runs on CUDA tensors")
+    if t.dtype not in _DTYPES:
+        raise TypeError(f"unsupported dtype {t.dtype}; f32 and bf16 are supported")
+    return context(t.device.index)
 
 
 class _RMSNormFn(torch.autograd.Function):
@@ -176,6 +185,68 @@ class _CrossEntropyFn(torch.autograd.Function):
         return d, None
 
 
+class TokenLogprobs(NamedTuple):
+    """What token_logprobs returns; the top_ fields are None without alternatives."""
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    top_ids: Optional[torch.Tensor]
+    top_logprobs: Optional[torch.Tensor]
+
+
+def _token_logprobs(logits, flat, top_k, with_stats):
+    rows, classes = logits.shape
+    stride = logits.stride(0) if rows > 1 else classes
+    dev = logits.device
+    logprob, entropy = (torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(2))
+    stats = torch.empty(rows, 3, dtype=torch.float32, device=dev) if with_stats else None
+    ids = top = None
+    if top_k:
+        ids = torch.empty(rows, top_k, dtype=torch.int32, device=dev)
+        top = torch.empty(rows, top_k, dtype=torch.float32, device=dev)
+    c = _context_of(logits)
+    with c.lock:
+        c.use_stream()
+        N.check(N.lib().hx_token_logprobs_fwd(c.handle, _DTYPES[logits.dtype], logits.data_ptr(), stride,
+                                              flat.data_ptr(), logprob.data_ptr(), entropy.data_ptr(),
+                                              stats.data_ptr() if with_stats else None, top_k,
+                                              ids.data_ptr() if top_k else None, top.data_ptr() if top_k else None,
+                                              rows, classes), c.handle)
+    return logprob, entropy, ids, top, stats
+
+
+class _TokenLogprobsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(fctx, logits, flat, top_k):
+        logprob, entropy, ids, top, stats = _token_logprobs(logits, flat, top_k, True)
+        fctx.save_for_backward(logits, flat, stats)
+        fctx.set_materialize_grads(False)
+        if top_k:
+            fctx.mark_non_differentiable(ids, top)
+        return logprob, entropy, ids, top
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(fctx, g_logprob, g_entropy, _ids, _top):
+        logits, flat, stats = fctx.saved_tensors
+        rows, classes = logits.shape
+        if g_logprob is None and g_entropy is None:
+            return None, None, None
+        stride = logits.stride(0) if rows > 1 else classes
+        # Rows at the logits' stride, so that 16-byte pieces line up in both (unless that wastes memory).
+        dstride = stride if stride <= 2 * classes else classes
+        d = torch.empty_strided((rows, classes), (dstride, 1), dtype=logits.dtype, device=logits.device)
+        gl = None if g_logprob is None else g_logprob.contiguous()
+        gh = None if g_entropy is None else g_entropy.contiguous()
+        c = _context_of(logits)
+        with c.lock:
+            c.use_stream()
+            N.check(N.lib().hx_token_logprobs_bwd(c.handle, _DTYPES[logits.dtype], logits.data_ptr(), stride,
+                                                  flat.data_ptr(), stats.data_ptr(), None if gl is None else gl.data_ptr(),
+                                                  None if gh is None else gh.data_ptr(), d.data_ptr(), dstride, rows,
+                                                  classes), c.handle)
+        return d, None, None
+
+
 def gelu(x: torch.Tensor) -> torch.Tensor:
     """Tensor::gelu (kernels/activations.rs:192-237, tanh form) with its backward."""
     return _GeluFn.apply(x)
@@ -190,6 +261,93 @@ def cross_entropy(logits: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
     """Tensor::cross_entropy (src/tensor.rs:754-801): mean over rows of
     logsumexp(row) - row[target], a device scalar; logits [rows, classes]."""
     return _CrossEntropyFn.apply(logits, targets)
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0) -> TokenLogprobs:
+    """log softmax(logits)[r, targets[r]] and the entropy of each row, f32 [rows];
+    logits [rows, classes] with contiguous rows, targets an integer vector.
+    With top_k (at most 32) also the likeliest classes of each row, int32 and f32
+    [rows, top_k], the lower index first among equals. The row terms of
+    `cross_entropy`, differentiable in the log probability and the entropy; the
+    alternatives carry no gradient. A target (read as 32 bits) outside
+    [0, classes) gives NaN; so does a row with NaN, +inf or no finite logit."""
+    if logits.dim() != 2 or logits.stride(1) != 1 and logits.shape[1] > 1:
+        raise ValueError("logits must be [rows, classes] with contiguous rows")
+    if logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]:
+        logits = logits.contiguous()
+    flat = _ids(targets)
+    if flat.numel() != logits.shape[0]:
+        raise ValueError("targets length must match the number of logit rows")
+    if flat.device != logits.device:
+        raise ValueError("targets must be on the logits' device")
+    top_k = int(top_k)
+    if not 0 <= top_k <= min(32, logits.shape[1]):
+        raise ValueError("top_k must be 0 to 32 and at most the number of classes")
+    if logits.requires_grad and torch.is_grad_enabled():
+        return TokenLogprobs(*_TokenLogprobsFn.apply(logits, flat, top_k))
+    return TokenLogprobs(*_token_logprobs(logits, flat, top_k, False)[:4])
+
+
+def quantize_w4(weight: torch.Tensor, group: int = 128):
+    """(packed, scales) of a finite weight [in, out] for linear_w4: int32
+    [ceil(in / 8), out] with 8 consecutive inputs' q in a word, the first in the
+    lowest 4 bits, and [ceil(in / group), out] scales in the weight's dtype;
+    weight is about (q - 8) * scale."""
+    if weight.dim() != 2:
+        raise ValueError("weight must be [in, out]")
+    c = _context_of(weight)
+    w = weight.detach().contiguous()
+    in_f, out_f = w.shape
+    if group <= 0 or group % 32:
+        raise ValueError("group must be a multiple of 32")
+    packed = torch.empty(-(-in_f // 8), out_f, dtype=torch.int32, device=w.device)
+    scales = torch.empty(-(-in_f // group), out_f, dtype=w.dtype, device=w.device)
+    with c.lock:
+        c.use_stream()
+        N.check(N.lib().hx_quantize_w4(c.handle, _DTYPES[w.dtype], w.data_ptr(), packed.data_ptr(), scales.data_ptr(),
+                                       in_f, out_f, group), c.handle)
+    return packed, scales
+
+
+def linear_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, group: int,
+              bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """`linear` with 4-bit weights (quantize_w4's layout), for the few rows of a decode
+    step: x [..., in] -> [..., out], x, scales, bias and residual of one dtype.
+    For inference: it has no backward and refuses tensors that would need one."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, scales, bias, residual)):
+        raise RuntimeError("linear_w4 has no backward: call it under torch.no_grad()")
+    c = _context_of(x)
+    in_f, out_f = x.shape[-1], packed.shape[-1]
+    if group <= 0 or group % 32:
+        raise ValueError("group must be a multiple of 32")
+    if packed.dtype != torch.int32 or packed.shape != (-(-in_f // 8), out_f) or not packed.is_contiguous():
+        raise ValueError(f"packed must be contiguous int32 [{-(-in_f // 8)}, out] for {in_f} inputs")
+    if scales.shape != (-(-in_f // group), out_f) or not scales.is_contiguous():
+        raise ValueError(f"scales must be contiguous [{-(-in_f // group)}, {out_f}]")
+    shape = (*x.shape[:-1], out_f)
+    if bias is not None and (bias.shape != (out_f,) or not bias.is_contiguous()):
+        raise ValueError(f"bias must be a contiguous vector of {out_f}")
+    if residual is not None and residual.shape != shape:
+        raise ValueError(f"residual must be {shape}")
+    for t in (scales, bias, residual):
+        if t is not None and t.dtype != x.dtype:
+            raise ValueError("x, scales, bias and residual must share a dtype")
+    for t in (packed, scales, bias, residual):
+        if t is not None and t.device != x.device:
+            raise ValueError("all operands must be on x's device")
+    x = x.contiguous()
+    if residual is not None:
+        residual = residual.contiguous()
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    if y.numel() == 0:
+        return y
+    with c.lock:
+        c.use_stream()
+        N.check(N.lib().hx_linear_w4_fwd(c.handle, _DTYPES[x.dtype], x.data_ptr(), packed.data_ptr(), scales.data_ptr(),
+                                         None if bias is None else bias.data_ptr(),
+                                         None if residual is None else residual.data_ptr(), y.data_ptr(),
+                                         x.numel() // in_f, in_f, out_f, group), c.handle)
+    return y
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5) -> torch.Tensor:

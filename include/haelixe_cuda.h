@@ -299,6 +299,21 @@ int hx_linear_fwd(hx_ctx* ctx, hx_dtype dtype, const void* x, const void* w, con
  * dx, dw, db may be NULL to skip it. */
 int hx_linear_bwd(hx_ctx* ctx, hx_dtype dtype, const void* x, const void* w, const void* dy, void* dx,
                   void* dw, void* db, int rows, int in_features, int out_features);
+/* hx_linear_fwd with weights of 4 bits, for the few rows of a decode step:
+ * y[rows, out] = x[rows, in] w + b + residual, w[k, n] = (q[k, n] - 8) *
+ * scales[k / group, n]. packed[o, n] ([ceil(in / 8), out], row-major) holds q
+ * of k = 8 o ... 8 o + 7, the first in the lowest 4 bits; those at or past in
+ * are ignored. scales [ceil(in / group), out], b, residual and x are in
+ * `dtype`; b and residual may be NULL, residual may alias y; group is a
+ * multiple of 32. Sums in f32, one rounding. A weight is read once for each 32
+ * rows: for many rows a bf16 weight and hx_linear_fwd are faster. */
+int hx_linear_w4_fwd(hx_ctx* ctx, hx_dtype dtype, const void* x, const uint32_t* packed, const void* scales,
+                     const void* b, const void* residual, void* y, int rows, int in_features, int out_features,
+                     int group);
+/* packed and scales of a finite weight [in, out] for hx_linear_w4_fwd: the scale of
+ * a column's group is its largest magnitude / 7, q = round(w / scale) + 8. */
+int hx_quantize_w4(hx_ctx* ctx, hx_dtype dtype, const void* w, uint32_t* packed, void* scales, int in_features,
+                   int out_features, int group);
 /* RMSNorm over the last dimension (src/kernels/rms_norm.rs:20-55):
  * y = x / sqrt(mean(x^2) + eps) * w per row of `hidden` elements. */
 int hx_rmsnorm_fwd(hx_ctx* ctx, hx_dtype dtype, const void* x, const void* w, void* y, int rows,
@@ -336,6 +351,26 @@ int hx_linear_residual_fwd(hx_ctx* ctx, hx_dtype dtype, const void* x, const voi
  * panics on the out-of-range index). */
 int hx_cross_entropy(hx_ctx* ctx, hx_dtype dtype, const void* logits, const uint32_t* targets, float* loss,
                      void* dlogits, int rows, int classes);
+
+/* Log probabilities of given tokens under logits [rows, classes] (row r at
+ * logits + r * row_stride elements): logprob[r] = logits[r, targets[r]] -
+ * logsumexp(row), entropy[r] of softmax(row), both f32. The row terms of
+ * hx_cross_entropy, kept apart. top_k (0 to 32, at most classes) of the most
+ * likely classes go to top_ids and top_logprobs [rows, top_k], likeliest
+ * first, the lower index first among equals. A -inf logit has no weight; a
+ * row with NaN, +inf or no finite logit gives NaN (top_ids then rank NaN as
+ * -inf); a target >= classes gives a NaN logprob. stats (f32 [rows, 3], may be
+ * NULL) is what the backward needs. */
+int hx_token_logprobs_fwd(hx_ctx* ctx, hx_dtype dtype, const void* logits, int64_t row_stride,
+                          const uint32_t* targets, float* logprob, float* entropy, float* stats, int top_k,
+                          int32_t* top_ids, float* top_logprobs, int rows, int classes);
+/* dlogits for the upstream gradients of logprob and entropy (f32 [rows]; NULL
+ * for none): g_logprob (onehot - p) - g_entropy p (log p + entropy), in
+ * `dtype`, every element of [rows, classes] written. dlogits may be logits
+ * itself. A row whose target is >= classes gets NaN when g_logprob is given. */
+int hx_token_logprobs_bwd(hx_ctx* ctx, hx_dtype dtype, const void* logits, int64_t row_stride,
+                          const uint32_t* targets, const float* stats, const float* g_logprob,
+                          const float* g_entropy, void* dlogits, int64_t drow_stride, int rows, int classes);
 
 /* One tensor of an AdamW step: f32 master weights and moments, the gradient in
  * grad_dtype, and an optional bf16 copy of the updated weights (NULL for none)
