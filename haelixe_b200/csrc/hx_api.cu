@@ -971,7 +971,7 @@ static int w4_args(hx_ctx* c, hx_dtype dt, int rows, int in, int out, int group,
     if ((st = linear_args(c, dt, rows, in, out, who))) return st;
     if (group <= 0 || group % 32)
         return set_error(c, HX_ERR_INVALID, "%s: group %d is not a multiple of 32", who, group);
-    if (rows > 32 * 65535) return set_error(c, HX_ERR_UNSUPPORTED, "%s: more than %d rows", who, 32 * 65535);
+    if (rows > 16 * 65535) return set_error(c, HX_ERR_UNSUPPORTED, "%s: more than %d rows", who, 16 * 65535);
     return HX_OK;
 }
 
@@ -983,7 +983,7 @@ int hx_linear_w4_fwd(hx_ctx* c, hx_dtype dt, const void* x, const uint32_t* pack
     DeviceGuard g(c->device);
     NvtxRange nv("hx_linear_w4_fwd");
     LaunchCount lc(c);
-    return check_cuda(c, hx::linear_w4(c->stream, c->sm_count, dt, x, packed, scales, b, residual, y, rows,
+    return check_cuda(c, hx::linear_w4(c->stream, c->sm_count, c->status, dt, x, packed, scales, b, residual, y, rows,
                                        in_features, out_features, group),
                       "hx_linear_w4_fwd");
 }

@@ -179,7 +179,7 @@ cudaError_t token_logprobs_bwd(cudaStream_t st, int sm_count, hx_dtype dt, const
                                const float* g_entropy, void* dlogits, int64_t dstride, int rows, int classes);
 
 // ---- Linear with 4-bit weights (linear_w4.cu) ----
-cudaError_t linear_w4(cudaStream_t st, int sm_count, hx_dtype dt, const void* x, const uint32_t* packed,
+cudaError_t linear_w4(cudaStream_t st, int sm_count, DeviceStatus* status, hx_dtype dt, const void* x, const uint32_t* packed,
                       const void* scales, const void* bias, const void* residual, void* y, int rows, int in, int out,
                       int group);
 cudaError_t quantize_w4(cudaStream_t st, hx_dtype dt, const void* w, uint32_t* packed, void* scales, int in, int out,

@@ -12,13 +12,22 @@
 // with no shared memory. q - 8 and bf16 x are exact operands; f32 x is cut into
 // three bf16 that sum to it exactly, three products for one.
 //
-// A CTA's 8 warps take every 8th step of the same 32 columns; a cluster of up to 8
-// CTAs splits k further where there are few columns, and joins its sums through
-// distributed shared memory in a fixed order.
+// A CTA's 8 warps form k groups of wn warps: a group takes every so many units of 128 k of
+// 64 wn columns (32 wn for over 16 rows), each warp its own columns. A unit's weights and x come
+// by TMA into one of the group's two stages while the other is computed on, so the bytes in
+// flight cost neither registers nor issue slots (16-byte loads and row-wise bulk copies took longer
+// to issue than the products) and x is read once a group. The groups' sums are
+// joined in shared memory; a cluster of up to 8 CTAs splits k further where there
+// are few columns, and joins its sums through distributed shared memory. Every
+// join has a fixed order.
 #include <cooperative_groups.h>
+
+#include <atomic>
 
 #include "hx_internal.h"
 #include "mma_bf16.cuh"
+#include "sm100_ptx.cuh"
+#include "tma_host.h"
 
 namespace hx {
 namespace {
@@ -26,24 +35,37 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
-constexpr int kCols = 32, kStep = 32;  // columns of a CTA, k of a warp's step
-constexpr int kAhead = 4;              // steps whose loads are in flight together
+constexpr int kStep = 32;  // k of a warp's tensor products, one 16-byte load of weights a lane and 32 columns
 
 struct Args {
+    CUtensorMap w_map, x_map;
     const void* x;
     const uint32_t* packed;
     const void *scales, *bias, *residual;
     void* y;
-    int rows, in, out, group;
-    bool vec_x, vec_w;  // 16-byte loads fit the rows of x; of packed, scales
+    DeviceStatus* status;
+    int rows, in, out, group, group_shift;  // group_shift: log2(group), -1 when not a power of two
+    int wn_log, ks_log;  // log2 of the warps that share a unit, side by side, and of the cluster's size
 };
 
-// q - 8 of nibbles p and p + 4 of w, as bf16.
-__device__ __forceinline__ uint32_t weights_of(uint32_t w, int p) {
-    const uint32_t u = ((w >> (4 * p)) & 0x000f000fu) | 0x43004300u;
-    const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), __float2bfloat162_rn(136.f));
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
+// q - 8 of nibbles p and p + 4 of w, as bf16: one shift, one three-input logic operation
+// (w & nibbles | magic, both constants in registers) and one subtraction.
+struct Unpack {
+    uint32_t nibbles, magic, bias;
+    __device__ __forceinline__ Unpack() {
+        // Opaque to the compiler, which would split the operation to use immediates.
+        asm volatile("mov.b32 %0, 0x000f000f;" : "=r"(nibbles));
+        asm volatile("mov.b32 %0, 0x43004300;" : "=r"(magic));
+        asm volatile("mov.b32 %0, 0x43084308;" : "=r"(bias));  // 136
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t w, int p) const {
+        uint32_t u;
+        asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(u) : "r"(w >> (4 * p)), "r"(nibbles), "r"(magic));
+        const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u),
+                                         *reinterpret_cast<const __nv_bfloat162*>(&bias));
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+};
 
 // 8 consecutive x as PARTS sets of 4 words, whose sum they are, in the weights' order:
 // words (x0, x4), (x1, x5), (x2, x6), (x3, x7).
@@ -53,17 +75,9 @@ template <>
 struct X8<__nv_bfloat16> {
     static constexpr int PARTS = 1;
     uint4 raw;
-    __device__ __forceinline__ void load(const __nv_bfloat16* p, int valid, bool vec) {
-        if (vec && valid >= 8) {
-            raw = *reinterpret_cast<const uint4*>(p);
-        } else {
-            const uint16_t* s = reinterpret_cast<const uint16_t*>(p);
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                w[i] = (2 * i < valid ? s[2 * i] : 0u) | (2 * i + 1 < valid ? (uint32_t)s[2 * i + 1] << 16 : 0u);
-            raw = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+    // The 8 from 16-byte chunk `chunk` of a swizzled row whose number ends in g.
+    __device__ __forceinline__ void load(const unsigned char* row, int chunk, int g) {
+        raw = *reinterpret_cast<const uint4*>(row + 16 * (chunk ^ g));
     }
     __device__ __forceinline__ void words(uint32_t (&b)[1][4]) const {
         b[0][0] = pair_lo(raw.x, raw.z);
@@ -76,14 +90,10 @@ template <>
 struct X8<float> {
     static constexpr int PARTS = 3;
     float v[8];
-    __device__ __forceinline__ void load(const float* p, int valid, bool vec) {
-        if (vec && valid >= 8) {
-            const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = i < valid ? p[i] : 0.f;
-        }
+    __device__ __forceinline__ void load(const unsigned char* row, int chunk, int g) {
+        const float4 a = *reinterpret_cast<const float4*>(row + 16 * (chunk ^ g));
+        const float4 b = *reinterpret_cast<const float4*>(row + 16 * ((chunk + 1) ^ g));
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
     }
     // The upper 8 bits of the mantissa, the next 8 and the rest, each exact in bf16.
     // Infinities and NaN stay whole in the first part.
@@ -106,146 +116,283 @@ struct X8<float> {
     }
 };
 
-__device__ __forceinline__ uint4 ld_stream(const void* p) {
-    uint4 u;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
-                 : "l"(p));
-    return u;
-}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait;" ::: "memory"); }
 
+// Scales of 4 columns.
 template <typename T>
-__device__ __forceinline__ float4 load4(const T* p, bool vec, int valid) {
-    if (vec && valid >= 4) {
-        if constexpr (sizeof(T) == 2) {
-            const uint2 u = *reinterpret_cast<const uint2*>(p);
-            const float2 a = unpack_bf16(u.x), b = unpack_bf16(u.y);
-            return make_float4(a.x, a.y, b.x, b.y);
-        } else {
-            return *reinterpret_cast<const float4*>(p);
-        }
+struct alignas(4 * sizeof(T)) S4 {
+    T s[4];
+};
+
+constexpr int kUnit = 4;                    // steps whose weights and x are copied together
+constexpr int kUnitK = kUnit * kStep;       // 128
+constexpr int kUnitRows = kUnitK / 8;       // rows of packed words
+constexpr int kStages = 2;
+
+// Shared memory of a CTA. A stage holds the group's words as boxes of kUnitRows rows of 32
+// (a warp's CH boxes after another's), then x as boxes of R rows of 128 bytes, each 128-byte
+// row with its 16-byte chunks exchanged by the row number (the TMA's swizzle). With
+// column_of a quarter warp's 16-byte reads of the words fall on all banks. The stages become the
+// groups' sums, [8 / wn][R][C + 1].
+constexpr int kBox = kUnitRows * 128;
+struct Layout {
+    int w_bytes, stage, recv, bars, total;  // bytes, then byte offsets
+    __host__ __device__ Layout(int R, int CH, int wn, int eb) {
+        const int C = 32 * CH * wn, groups = kWarps / wn;
+        w_bytes = CH * wn * kBox;
+        stage = w_bytes + R * kUnitK * eb;
+        const int sums = groups * R * (C + 1) * 4;
+        recv = groups * kStages * stage;
+        if (recv < sums) recv = (sums + 15) / 16 * 16;
+        bars = recv + ((R * C + kThreads - 1) / kThreads + 7) * kThreads * 4;
+        total = bars + 2 * groups * kStages * 8 + 16;
     }
-    return make_float4(valid > 0 ? (float)p[0] : 0.f, valid > 1 ? (float)p[1] : 0.f, valid > 2 ? (float)p[2] : 0.f,
-                       valid > 3 ? (float)p[3] : 0.f);
-}
+};
 
-// NT: sets of 8 rows. grid: (column tiles x cluster, passes of 8 NT rows).
-template <typename T, int NT>
-__global__ void __launch_bounds__(kThreads) linear_w4_kernel(Args a) {
-    constexpr int R = 8 * NT, PARTS = X8<T>::PARTS;
-    __shared__ float part[kWarps][R][kCols + 1];
-    __shared__ float sums[R][kCols];
+// First of the 4 columns of lane group g within a set of 32.
+__device__ __forceinline__ int column_of(int g) { return 4 * ((g >> 1) | ((g & 1) << 2)); }
+
+// NT: sets of 8 rows; CH: sets of 32 columns of a warp; L: consecutive steps of a unit that
+// lie in one group of scales, so that their products are scaled once. grid: (column
+// tiles x cluster, passes of 8 NT rows).
+// VEC: the rows of x and of packed are multiples of 16 bytes and x, packed and scales are
+// aligned, as TMA needs. Otherwise wn is 1 and each warp fills its stage with plain loads.
+template <typename T, int NT, int CH, int L, bool VEC>
+__global__ void __launch_bounds__(kThreads, sizeof(T) * NT * CH <= 8 ? 2 : 1) linear_w4_kernel(const __grid_constant__ Args a) {
+    constexpr int R = 8 * NT, PARTS = X8<T>::PARTS, kBoxK = 128 / sizeof(T);  // k of a box of x
+    extern __shared__ __align__(1024) unsigned char smem[];
+    // Everything that is shared out is a power of two, so that no index costs a division.
+    const int wn_log = VEC ? a.wn_log : 0, wn = 1 << wn_log, c_log = (CH == 2 ? 6 : 5) + wn_log, C = 1 << c_log;
+    const int groups = kWarps >> wn_log, ks_log = a.ks_log, ks = 1 << ks_log, rank = blockIdx.x & (ks - 1);
+    const Layout lay(R, CH, wn, sizeof(T));
     cg::cluster_group cluster = cg::this_cluster();
-    const int ks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    if (ks > 1) cluster_arrive();  // waited for before the first write to another CTA: all have started
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-    const int n0 = (blockIdx.x / ks) * kCols, r0 = blockIdx.y * R;
-    const int n = n0 + 4 * g, cols = a.out - n;  // this lane's 4 columns, those that exist
-    const int octets = (a.in + 7) / 8, steps = (a.in + kStep - 1) / kStep;
-    const T* x = (const T*)a.x;
-    const T* scales = (const T*)a.scales;
+    const int group = warp >> wn_log, sub = warp & (wn - 1);
+    const int n0 = (blockIdx.x >> ks_log) << c_log, r0 = blockIdx.y * R;
+    const int rows = min(R, a.rows - r0);
+    const int octets = (a.in + 7) / 8, units = (a.in + kUnitK - 1) / kUnitK, stride = groups * ks;
+    const int first = rank * groups + group;
 
-    float acc[2][NT][4];
+    unsigned char* stages = smem + group * kStages * lay.stage;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + lay.bars) + 2 * kStages * group;
+    volatile int* abort_flag = reinterpret_cast<int*>(smem + lay.bars + 2 * groups * kStages * 8);
+    const uint32_t bar = ptx::smem_addr(bars);
+    auto full = [&](int i) { return bar + 8 * i; };
+    auto empty = [&](int i) { return bar + 8 * (kStages + i); };
+    if constexpr (VEC) {
+        if (threadIdx.x == 0) *abort_flag = 0;
+        if (sub == 0 && lane == 0) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
-
-    const int stride = kWarps * ks;
-    for (int s0 = rank * kWarps + warp; s0 < steps; s0 += kAhead * stride) {
-        uint4 w[kAhead];
-        float4 sc[kAhead];
-        X8<T> xs[kAhead][NT];
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            const int s = s0 + u * stride, o = 4 * s + t;  // this lane's 8 k: 8 o ... 8 o + 7
-            w[u] = make_uint4(0, 0, 0, 0);
-            sc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (s < steps && cols > 0) {
-                if (o < octets) {
-                    const uint32_t* p = a.packed + (int64_t)o * a.out + n;
-                    if (a.vec_w)
-                        w[u] = ld_stream(p);
-                    else
-                        w[u] = make_uint4(p[0], cols > 1 ? p[1] : 0u, cols > 2 ? p[2] : 0u, cols > 3 ? p[3] : 0u);
-                }
-                sc[u] = load4<T>(scales + (int64_t)(s * kStep / a.group) * a.out + n, a.vec_w, cols);
+            for (int i = 0; i < kStages; ++i) {
+                ptx::mbar_init(full(i), wn);
+                ptx::mbar_init(empty(i), wn);
             }
+            ptx::fence_mbar_init();
+        }
+        __syncthreads();
+    }
+    // Unit u into stage i: each warp its own words, the group's first warp x as well. What is
+    // past the last row, column or k reads as zero.
+    auto copy_unit = [&](int u, int i) {
+        unsigned char* st = stages + i * lay.stage;
+        if constexpr (VEC) {
+            if (lane == 0) {
+                ptx::mbar_arrive_expect_tx(full(i), CH * kBox + (sub == 0 ? R * kUnitK * (int)sizeof(T) : 0));
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const int row = r0 + 8 * j + g;
-                const bool live = s < steps && row < a.rows;
-                xs[u][j].load(x + (live ? (int64_t)row * a.in + 8 * o : 0), live ? a.in - 8 * o : 0, a.vec_x);
+                for (int c = 0; c < CH; ++c)
+                    ptx::tma_load_2d(ptx::smem_addr(st + (CH * sub + c) * kBox), &a.w_map, full(i),
+                                     n0 + 32 * (CH * sub + c), kUnitRows * u);
+                if (sub == 0)
+#pragma unroll
+                    for (int c = 0; c < kUnitK / kBoxK; ++c)
+                        ptx::tma_load_2d(ptx::smem_addr(st + lay.w_bytes + c * R * 128), &a.x_map, full(i),
+                                         kUnitK * u + c * kBoxK, r0);
+            }
+        } else {
+            for (int k = 0; k < kUnitRows; ++k)
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    const int n = n0 + 32 * c + lane, o = kUnitRows * u + k;
+                    reinterpret_cast<uint32_t*>(st + c * kBox + k * 128)[lane ^ (4 * (k & 7))] =
+                        n < a.out && o < octets ? a.packed[(int64_t)o * a.out + n] : 0u;
+                }
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int k = lane; k < kUnitK; k += 32) {
+                    const int chunk = (k % kBoxK) * (int)sizeof(T) / 16 ^ (r & 7), at = kUnitK * u + k;
+                    reinterpret_cast<T*>(st + lay.w_bytes + (k / kBoxK) * R * 128 + r * 128 + chunk * 16)[k % (16 / sizeof(T))] =
+                        r < rows && at < a.in ? ((const T*)a.x)[(int64_t)(r0 + r) * a.in + at] : T(0.f);
+                }
+            __syncwarp();
+        }
+    };
+
+    int col[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        col[c] = n0 + 32 * (CH * sub + c) + column_of(g);
+        if (VEC) col[c] = min(col[c], a.out - 4);
+    }
+    S4<T> sc[kUnit / L][CH];
+    auto load_scales = [&](int u, int l) {
+        const int k = min(kUnitK * u + l * L * kStep, a.in - 1);
+        const T* p = (const T*)a.scales + (int64_t)(a.group_shift >= 0 ? k >> a.group_shift : k / a.group) * a.out;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            if constexpr (VEC) {
+                sc[l][c] = *reinterpret_cast<const S4<T>*>(p + col[c]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sc[l][c].s[i] = col[c] + i < a.out ? p[col[c] + i] : T(0.f);
             }
         }
+    };
+
+    float acc[CH][2][NT][4];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            float d[2][NT][4];
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[c][m][j][e] = 0.f;
+
+    const Unpack weight;
+    uint32_t issued = 0, done = 0;  // units of this group
+    if constexpr (VEC) {
+        for (int u = first; u < units && issued < kStages; u += stride) copy_unit(u, issued++);
+    }
+    if (first < units) {
+#pragma unroll
+        for (int l = 0; l < kUnit / L; ++l) load_scales(first, l);
+    }
+    for (int u = first; u < units; u += stride) {
+        const int i = VEC ? done % kStages : 0;
+        if constexpr (VEC) {
+            if (!ptx::mbar_wait(full(i), done / kStages & 1, abort_flag, a.status, 50)) break;
+        } else {
+            copy_unit(u, 0);
+        }
+        ++done;
+        const unsigned char* ws = stages + i * lay.stage + CH * sub * kBox + t * 128;
+        const unsigned char* xs = stages + i * lay.stage + lay.w_bytes + g * 128;
+        float d[CH][2][NT][4];
+#pragma unroll
+        for (int l = 0; l < kUnit; ++l) {
+            if (l % L == 0) {
+#pragma unroll
+                for (int c = 0; c < CH; ++c)
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) d[c][m][j][e] = 0.f;
+            }
             uint32_t b[NT][PARTS][4];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                xs[u][j].words(b[j]);
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) d[i][j][e] = 0.f;
+                X8<T> x;
+                x.load(xs + 8 * j * 128 + (l * kStep / kBoxK) * R * 128, (l * kStep % kBoxK + 8 * t) * sizeof(T) / 16, g);
+                x.words(b[j]);
             }
-            const uint32_t col[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+            uint32_t q[CH][4];
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int c = 0; c < CH; ++c) {
+                const uint4 w =
+                    *reinterpret_cast<const uint4*>(ws + c * kBox + 4 * l * 128 + 16 * (column_of(g) / 4 ^ (4 * (l & 1) + t)));
+                q[c][0] = w.x, q[c][1] = w.y, q[c][2] = w.z, q[c][3] = w.w;
+            }
+            // All tiles' products of two nibble pairs before the next two: they do not wait for each other.
 #pragma unroll
-                for (int p = 0; p < 4; p += 2) {
-                    const uint32_t a0 = weights_of(col[2 * i], p), a1 = weights_of(col[2 * i + 1], p);
-                    const uint32_t a2 = weights_of(col[2 * i], p + 1), a3 = weights_of(col[2 * i + 1], p + 1);
+            for (int p = 0; p < 4; p += 2)
 #pragma unroll
-                    for (int j = 0; j < NT; ++j)
+                for (int c = 0; c < CH; ++c)
 #pragma unroll
-                        for (int q = PARTS - 1; q >= 0; --q)
-                            mma_bf16(d[i][j], a0, a1, a2, a3, b[j][q][p], b[j][q][p + 1]);
+                    for (int m = 0; m < 2; ++m) {
+                        const uint32_t a0 = weight(q[c][2 * m], p), a1 = weight(q[c][2 * m + 1], p);
+                        const uint32_t a2 = weight(q[c][2 * m], p + 1), a3 = weight(q[c][2 * m + 1], p + 1);
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+#pragma unroll
+                            for (int k = PARTS - 1; k >= 0; --k)
+                                mma_bf16(d[c][m][j], a0, a1, a2, a3, b[j][k][p], b[j][k][p + 1]);
+                    }
+            if (l % L == L - 1) {
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    const S4<T> s = sc[l / L][c];
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                acc[c][m][j][e] = fmaf((float)s.s[2 * m + (e >> 1)], d[c][m][j][e], acc[c][m][j][e]);
                 }
-            const float s[4] = {sc[u].x, sc[u].y, sc[u].z, sc[u].w};
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(s[2 * i + (e >> 1)], d[i][j][e], acc[i][j][e]);
+                if (u + stride < units) load_scales(u + stride, l / L);
+            }
+        }
+        __syncwarp();  // all lanes have read the stage
+        if constexpr (VEC) {
+            if (lane == 0) ptx::mbar_arrive(empty(i));
+            const int next = u + kStages * stride;
+            if (next < units) {
+                // A warp's words are its own; x goes over what the group's other warps have to have read.
+                if (sub == 0 && !ptx::mbar_wait(empty(i), (issued / kStages - 1) & 1, abort_flag, a.status, 51)) break;
+                copy_unit(next, i);
+                ++issued;
+            }
         }
     }
-    // acc[i][j][e]: column 4 g + 2 i + e / 2, row 8 j + 2 t + e % 2
+    if constexpr (VEC)  // after an expired wait alone: no copy outlives the stages
+        for (; done < issued; ++done) ptx::mbar_wait_drain(full(done % kStages), done / kStages & 1);
+    __syncthreads();  // the stages are free: the groups' sums take their place
+    float* sums = reinterpret_cast<float*>(smem);
+    // acc[c][m][j][e]: column 32 c + column_of(g) + 2 m + e / 2 of the warp's, row 8 j + 2 t + e % 2
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int c = 0; c < CH; ++c)
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+        for (int m = 0; m < 2; ++m)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) part[warp][8 * j + 2 * t + (e & 1)][4 * g + 2 * i + (e >> 1)] = acc[i][j][e];
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    sums[(group * R + 8 * j + 2 * t + (e & 1)) * (C + 1) + 32 * (CH * sub + c) + column_of(g) + 2 * m + (e >> 1)] =
+                        acc[c][m][j][e];
+    if (ks > 1) cluster_wait();
     __syncthreads();
-    const int live = min(R, a.rows - r0);
-    for (int i = threadIdx.x; i < live * kCols; i += kThreads) {
+    // Result r * C + n of the tile is in block (r * C + n) / 256, which CTA block % ks finishes:
+    // it receives its blocks from all CTAs of the cluster.
+    float* recv = reinterpret_cast<float*>(smem + lay.recv);
+    const int blocks = (((rows << c_log) + kThreads - 1) / kThreads + ks - 1) >> ks_log;
+    for (int at = threadIdx.x, block = 0; at < rows << c_log; at += kThreads, ++block) {
+        const int r = at >> c_log, n = at & (C - 1);
         float v = 0.f;
-#pragma unroll
-        for (int k = 0; k < kWarps; ++k) v += part[k][i / kCols][i % kCols];
-        sums[i / kCols][i % kCols] = v;
+        for (int k = 0; k < groups; ++k) v += sums[(k * R + r) * (C + 1) + n];
+        float* to = &recv[(rank * blocks + (block >> ks_log)) * kThreads + threadIdx.x];
+        if (ks > 1)
+            *cluster.map_shared_rank(to, block & (ks - 1)) = v;
+        else
+            *to = v;
     }
-    if (ks > 1) cluster.sync();
-    // Each CTA of the cluster finishes its share of the rows.
-    for (int i = rank * kThreads + threadIdx.x; i < live * kCols; i += ks * kThreads) {
-        const int r = i / kCols, c = i % kCols;
+    if (ks > 1) {
+        cluster_arrive();
+        cluster_wait();
+    }
+    for (int k = 0; k < blocks; ++k) {
+        const int at = ((k << ks_log) + rank) * kThreads + threadIdx.x, r = at >> c_log, n = n0 + (at & (C - 1));
+        if (r >= rows || n >= a.out) continue;
         float v = 0.f;
-        if (ks > 1) {
-            for (int k = 0; k < ks; ++k) v += cluster.map_shared_rank(&sums[0][0], k)[i];
-        } else {
-            v = sums[r][c];
-        }
-        if (n0 + c < a.out) {
-            const int64_t at = (int64_t)(r0 + r) * a.out + n0 + c;
-            if (a.bias) v += (float)((const T*)a.bias)[n0 + c];
-            if (a.residual) v += (float)((const T*)a.residual)[at];
-            ((T*)a.y)[at] = T(v);
-        }
+        for (int i = 0; i < ks; ++i) v += recv[(i * blocks + k) * kThreads + threadIdx.x];
+        const int64_t to = (int64_t)(r0 + r) * a.out + n;
+        if (a.bias) v += (float)((const T*)a.bias)[n];
+        if (a.residual) v += (float)((const T*)a.residual)[to];
+        ((T*)a.y)[to] = T(v);
     }
-    if (ks > 1) cluster.sync();  // no CTA leaves while its sums are read
 }
 
 // One thread a column of a group: s = max |w| / 7, q = round(w / s) + 8.
@@ -276,43 +423,92 @@ __global__ void __launch_bounds__(256) quantize_w4_kernel(const T* w, uint32_t* 
     }
 }
 
-template <typename T, int NT>
-cudaError_t launch(cudaStream_t st, int sm_count, const Args& a) {
-    const int tiles = (a.out + kCols - 1) / kCols, steps = (a.in + kStep - 1) / kStep;
-    int ks = 1;
-    while (ks < 8 && tiles * ks < 3 * sm_count && steps >= 2 * kWarps * kAhead * ks) ks *= 2;
+// Row-major [rows][cols], boxes of box_rows rows of box_cols (128 bytes), 128-byte swizzle; outside reads as 0.
+bool row_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, int rows, int cols, int eb, int box_cols,
+             int box_rows) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (fn == nullptr) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)cols * eb};
+    const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    return fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int NT, int CH, int L, bool VEC>
+cudaError_t launch(cudaStream_t st, int sm_count, Args a) {
+    const int units = (a.in + kUnitK - 1) / kUnitK, R = 8 * NT;
+    auto tiles = [&] { return (a.out + (32 * CH << a.wn_log) - 1) / (32 * CH << a.wn_log); };
+    // Two warps share a unit, or none where the columns are too few to occupy the SMs (8192 x
+    // 2048 in f32, 5 rows: 8.6 us against 12.1 with two). k is split as long as all CTAs are
+    // resident at once, two an SM, and every group keeps two units (8192 x 8192, 16 rows: 25.0 us
+    // at 128 CTAs, 19.5 at 256, 23.6 at 512).
+    a.wn_log = VEC ? 1 : 0;
+    if (VEC && 4 * tiles() < sm_count) a.wn_log = 0;
+    const int groups = kWarps >> a.wn_log;
+    while (a.ks_log < 3 && tiles() << a.ks_log <= sm_count && units >= 4 * groups << a.ks_log) ++a.ks_log;
+    const int bytes = Layout(R, CH, 1 << a.wn_log, sizeof(T)).total;
+    static std::atomic<int> allowed[64];  // by device: the shared memory the kernel may have so far
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    auto kernel = linear_w4_kernel<T, NT, CH, L, VEC>;
+    if (dev >= 64 || allowed[dev].load(std::memory_order_acquire) < bytes) {
+        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) != cudaSuccess) return e;
+        if (dev < 64) allowed[dev].store(bytes, std::memory_order_release);
+    }
+    if (VEC && (!row_map(&a.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT32, a.packed, (a.in + 7) / 8, a.out, 4, 32, kUnitRows) ||
+                !row_map(&a.x_map, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.x,
+                         a.rows, a.in, sizeof(T), 128 / (int)sizeof(T), R)))
+        return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(tiles * ks), (unsigned)((a.rows + 8 * NT - 1) / (8 * NT)));
+    cfg.gridDim = dim3((unsigned)(tiles() << a.ks_log), (unsigned)((a.rows + R - 1) / R));
     cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = (size_t)bytes;
     cfg.stream = st;
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = (unsigned)ks;
+    at.val.clusterDim.x = 1u << a.ks_log;
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, linear_w4_kernel<T, NT>, a);
+    e = cudaLaunchKernelEx(&cfg, kernel, a);
     if (e == cudaSuccess) note_launch();
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
+// Unaligned operands and odd widths take one form of the kernel each, the rest one by the
+// steps of a unit that share a group.
+template <typename T, int NT, int CH>
+cudaError_t by_group(cudaStream_t st, int sm_count, const Args& a, bool vec) {
+    if (!vec) return launch<T, NT, CH, 1, false>(st, sm_count, a);
+    if (a.group % 128 == 0) return launch<T, NT, CH, 4, true>(st, sm_count, a);
+    if (a.group % 64 == 0) return launch<T, NT, CH, 2, true>(st, sm_count, a);
+    return launch<T, NT, CH, 1, true>(st, sm_count, a);
+}
+
+// Up to 16 rows a warp takes 64 columns, which halves the reads of x; 32 rows
+// fit the registers with 32 columns, and only in bf16.
 template <typename T>
-cudaError_t by_rows(cudaStream_t st, int sm_count, const Args& a) {
-    if (a.rows <= 8) return launch<T, 1>(st, sm_count, a);
-    if (a.rows <= 16) return launch<T, 2>(st, sm_count, a);
-    return launch<T, 4>(st, sm_count, a);
+cudaError_t by_rows(cudaStream_t st, int sm_count, const Args& a, bool vec) {
+    if (a.rows <= 8) return by_group<T, 1, 2>(st, sm_count, a, vec);
+    if constexpr (sizeof(T) == 4) {
+        return by_group<T, 2, 2>(st, sm_count, a, vec);
+    } else {
+        if (a.rows <= 16) return by_group<T, 2, 2>(st, sm_count, a, vec);
+        return by_group<T, 4, 1>(st, sm_count, a, vec);
+    }
 }
 
 }  // namespace
 
-cudaError_t linear_w4(cudaStream_t st, int sm_count, hx_dtype dt, const void* x, const uint32_t* packed,
+cudaError_t linear_w4(cudaStream_t st, int sm_count, DeviceStatus* status, hx_dtype dt, const void* x, const uint32_t* packed,
                       const void* scales, const void* bias, const void* residual, void* y, int rows, int in, int out,
                       int group) {
-    const int eb = dt == HX_F32 ? 4 : 2;
-    Args a{x, packed, scales, bias, residual, y, rows, in, out, group, false, false};
-    a.vec_x = (uintptr_t)x % 16 == 0 && ((int64_t)in * eb) % 16 == 0;
-    a.vec_w = (uintptr_t)packed % 16 == 0 && (uintptr_t)scales % 16 == 0 && out % 4 == 0;
-    return dt == HX_F32 ? by_rows<float>(st, sm_count, a) : by_rows<__nv_bfloat16>(st, sm_count, a);
+    Args a{CUtensorMap{}, CUtensorMap{}, x, packed, scales, bias, residual, y, status, rows, in, out, group,
+                 (group & (group - 1)) == 0 ? __builtin_ctz((unsigned)group) : -1, 0, 0};
+    const bool vec = (uintptr_t)x % 16 == 0 && (int64_t)in * (dt == HX_F32 ? 4 : 2) % 16 == 0 && (uintptr_t)packed % 16 == 0 && (uintptr_t)scales % 16 == 0 && out % 4 == 0;
+    return dt == HX_F32 ? by_rows<float>(st, sm_count, a, vec) : by_rows<__nv_bfloat16>(st, sm_count, a, vec);
 }
 
 cudaError_t quantize_w4(cudaStream_t st, hx_dtype dt, const void* w, uint32_t* packed, void* scales, int in, int out,

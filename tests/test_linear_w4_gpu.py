@@ -2,10 +2,11 @@
 
 Tolerance, from the arithmetic: the products are exact (4-bit integers times
 bf16, f32 as three bf16 that sum to it), so only sums and the scale round. A
-step of 32 k is up to 6 tensor products, each adding 16 terms with at most
-2^-22 of their magnitude; then a warp adds in / 256 scaled steps, 8 warps and 8
-CTAs are joined, bias and residual added, each at 2^-24. Altogether
-(6 * 4 + in / 256 + 20) 2^-23 of the sum of magnitudes, and half a step of the type.
+unit of 128 k is up to 24 tensor products in a chain, each off by at most 2^-23 of
+the partial sum it adds to; then a group of warps adds its scaled units (in / 128 at
+most), 8 groups and 8 CTAs are joined, bias and residual added, each at 2^-24.
+Altogether (24 + in / 256 + 20) 2^-23 of the sum of magnitudes, and half a
+step of the type.
 """
 import pytest
 import torch
@@ -196,7 +197,7 @@ def test_refusals_and_empty():
     L, c, p = N.lib(), hx.context(), x.data_ptr()
     for rows, in_f, out_f, group in ((0, 64, 32, 32), (2, 0, 32, 32), (2, 64, 0, 32), (2, 64, 32, 0), (2, 64, 32, 48)):
         assert L.hx_linear_w4_fwd(c.handle, 1, p, p, p, None, None, p, rows, in_f, out_f, group) == N.HX_ERR_INVALID
-    assert L.hx_linear_w4_fwd(c.handle, 1, p, p, p, None, None, p, 32 * 65535 + 1, 64, 32, 32) == N.HX_ERR_UNSUPPORTED
+    assert L.hx_linear_w4_fwd(c.handle, 1, p, p, p, None, None, p, 16 * 65535 + 1, 64, 32, 32) == N.HX_ERR_UNSUPPORTED
     assert L.hx_linear_w4_fwd(c.handle, 1, p, None, p, None, None, p, 2, 64, 32, 32) == N.HX_ERR_INVALID
     assert L.hx_quantize_w4(c.handle, 1, p, None, p, 64, 32, 32) == N.HX_ERR_INVALID
     assert L.hx_quantize_w4(None, 1, p, p, p, 64, 32, 32) == N.HX_ERR_INVALID
