@@ -1144,8 +1144,8 @@ int hx_token_logprobs_fwd(hx_ctx* c, hx_dtype dt, const void* logits, int64_t ro
     DeviceGuard g(c->device);
     NvtxRange nv(who);
     LaunchCount lc(c);
-    return check_cuda(c, hx::token_logprobs_fwd(c->stream, dt, logits, row_stride, targets, logprob, entropy, stats,
-                                                top_k, top_ids, top_logprobs, rows, classes),
+    return check_cuda(c, hx::token_logprobs_fwd(c->stream, c->sm_count, dt, logits, row_stride, targets, logprob, entropy,
+                                                stats, top_k, top_ids, top_logprobs, rows, classes),
                       who);
 }
 

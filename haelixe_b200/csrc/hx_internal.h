@@ -171,9 +171,9 @@ cudaError_t paged_attn(cudaStream_t st, int sm_count, hx_dtype dt, const PagedAt
 
 // ---- log probabilities of given tokens (logprobs.cu) ----
 // stats: 3 floats a row (maximum, log of the sum relative to it, entropy), for the backward.
-cudaError_t token_logprobs_fwd(cudaStream_t st, hx_dtype dt, const void* logits, int64_t stride, const uint32_t* targets,
-                               float* logprob, float* entropy, float* stats, int top, int32_t* top_ids,
-                               float* top_logprobs, int rows, int classes);
+cudaError_t token_logprobs_fwd(cudaStream_t st, int sm_count, hx_dtype dt, const void* logits, int64_t stride,
+                               const uint32_t* targets, float* logprob, float* entropy, float* stats, int top,
+                               int32_t* top_ids, float* top_logprobs, int rows, int classes);
 cudaError_t token_logprobs_bwd(cudaStream_t st, int sm_count, hx_dtype dt, const void* logits, int64_t stride,
                                const uint32_t* targets, const float* stats, const float* g_logprob,
                                const float* g_entropy, void* dlogits, int64_t dstride, int rows, int classes);

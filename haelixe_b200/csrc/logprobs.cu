@@ -4,27 +4,36 @@
 //   logp(t) = z_t - ln s,  H = ln s - w / s
 //   dx_i = g_t (1[i = t] - p_i) - g_H p_i (ln p_i + H)
 // One read of the logits forward, one read and one write backward: bytes bound
-// both, and next to them the exponentials (one a logit). The forward keeps
-// (m, s, w) running, so the row is read once; both terms of H are
-// positive, so nothing cancels. Sums are f32, per thread and then joined in a
-// tree, the same for every call.
+// both, if a logit costs no more than about nine instructions, one of them the
+// exponential (7 TB/s of bf16 are 13 logits a clock and SM). So the differences,
+// products and sums run two to an instruction (f32x2), and whole 16-byte
+// pieces are loaded four ahead. The forward keeps (m, s, w) running, so the row is
+// read once; both terms of H are positive, so nothing cancels. Sums are f32,
+// per thread and then joined in a tree, the same for every call. A few rows are
+// split over a cluster of CTAs each, which join through distributed shared memory.
 //
 // The alternatives need no second pass over the row either. Each thread knows the
 // best of its own logits; the k best threads' values bound the k-th best logit
 // from below, and every logit that reaches the bound belongs to one of those k
-// threads, so only their share of the row (k / 512 of it) is looked at again.
+// threads, so only their share of the row (k / 256 of it) is looked at again.
 // Ties go to the lower index.
+#include <cooperative_groups.h>
+
 #include "hx_internal.h"
 #include "mma_bf16.cuh"
+#include "sm100_ptx.cuh"
 
 namespace hx {
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+namespace cg = cooperative_groups;
+
+constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr float kLowest = -3.402823466e+38f;
 constexpr float kFloor = -1.0e4f;  // exp2 of it is 0; keeps 0 * (-inf) out of the sums
 constexpr unsigned kAll = 0xffffffffu;
+constexpr int kAhead = 4;  // pieces of a thread in flight
 
 // max that keeps a NaN (fmaxf drops it).
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -32,9 +41,17 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
+using ptx::f2_add;
+using ptx::f2_fma;
+using ptx::f2_pack;
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
 
@@ -43,6 +60,12 @@ __device__ __forceinline__ uint32_t order_of(float v) {
     if (!(v == v)) v = -INFINITY;
     const uint32_t b = __float_as_uint(v + 0.f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
 }
 
 // A row as 16-byte pieces from the last 16-byte boundary at or before its start: piece j
@@ -56,7 +79,11 @@ struct RowView {
         : x(row), classes(n), lead((int)(((uintptr_t)row & 15) / sizeof(T))), pieces((int)(((int64_t)lead + n + E - 1) / E)) {}
     __device__ __forceinline__ int first(int j) const { return E * j - lead; }
     __device__ __forceinline__ bool whole(int j) const { return first(j) >= 0 && first(j) + E <= classes; }
-    __device__ __forceinline__ void decode(const uint4& u, float (&v)[E]) const {
+    // The whole pieces are [begin(), end()); one before and one after may be partial (or the only one).
+    __device__ __forceinline__ int begin() const { return lead > 0; }
+    __device__ __forceinline__ int end() const { return (lead + classes) / E; }
+    __device__ __forceinline__ uint4 raw(int j) const { return *reinterpret_cast<const uint4*>(x + first(j)); }
+    static __device__ __forceinline__ void decode(const uint4& u, float (&v)[E]) {
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
@@ -69,10 +96,20 @@ struct RowView {
             for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[i]);
         }
     }
+    // The largest element; NaN does not count unless there is nothing else.
+    static __device__ __forceinline__ float top(const uint4& u) {
+        if constexpr (sizeof(T) == 2) {
+            const float2 f = unpack_bf16(max2(max2(u.x, u.y), max2(u.z, u.w)));
+            return fmaxf(f.x, f.y);
+        } else {
+            return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)),
+                         fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+        }
+    }
     // Elements outside the row read as `pad`.
     __device__ __forceinline__ void load(int j, float (&v)[E], float pad) const {
         if (whole(j)) {
-            decode(*reinterpret_cast<const uint4*>(x + first(j)), v);
+            decode(raw(j), v);
         } else {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
@@ -93,22 +130,59 @@ __device__ __forceinline__ Stats join(const Stats& a, const Stats& b) {
     const float ea = ex2(da), eb = ex2(db);
     return Stats{m, a.s * ea + b.s * eb, ea * (a.w + da * a.s) + eb * (b.w + db * b.s)};
 }
-
-template <int E>
-__device__ __forceinline__ void add_piece(Stats& st, const float (&v)[E], float top) {
-    if (top > st.m) {
-        const float d = weight_of(st.m, top), e = ex2(d);
-        st.w = e * (st.w + d * st.s);
-        st.s *= e;
-        st.m = top;
-    }
+// Of the LANES first lanes of a warp, to all of them: the maximum first, so that each part is
+// weighted once.
+template <int LANES>
+__device__ __forceinline__ Stats join_lanes(Stats a) {
+    float m = a.m;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        const float z = max_nan((v[i] - st.m) * kLog2e, kFloor), e = ex2(z);
-        st.s += e;
-        st.w = fmaf(z, e, st.w);
+    for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
+    const float d = weight_of(a.m, m), e = ex2(d);
+    a = Stats{m, e * a.s, e * fmaf(d, a.s, a.w)};
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+        a.s += __shfl_xor_sync(kAll, a.s, o);
+        a.w += __shfl_xor_sync(kAll, a.w, o);
     }
+    return a;
 }
+
+// A thread's running statistics, the sums in two halves.
+struct Running {
+    float m = kLowest;
+    uint64_t s = 0, w = 0, minus_m = f2_pack(-kLowest, -kLowest);
+
+    // Before logits of at most `top` are added.
+    __device__ __forceinline__ void raise(float top) {
+        if (top > m) {
+            const float d = weight_of(m, top), e = ex2(d);
+            const uint64_t e2 = f2_pack(e, e);
+            w = f2_mul(e2, f2_fma(f2_pack(d, d), s, w));
+            s = f2_mul(e2, s);
+            m = top;
+            minus_m = f2_pack(-m, -m);
+        }
+    }
+    template <int E>
+    __device__ __forceinline__ void add(const float (&v)[E]) {
+        const uint64_t l2 = f2_pack(kLog2e, kLog2e);
+#pragma unroll
+        for (int i = 0; i < E; i += 2) {
+            float z0, z1;
+            ptx::f2_unpack(f2_mul(f2_add(f2_pack(v[i], v[i + 1]), minus_m), l2), z0, z1);
+            z0 = max_nan(z0, kFloor), z1 = max_nan(z1, kFloor);
+            const uint64_t e = f2_pack(ex2(z0), ex2(z1));
+            s = f2_add(s, e);
+            w = f2_fma(f2_pack(z0, z1), e, w);
+        }
+    }
+    __device__ __forceinline__ Stats stats() const {
+        float s0, s1, w0, w1;
+        ptx::f2_unpack(s, s0, s1);
+        ptx::f2_unpack(w, w0, w1);
+        return Stats{m, s0 + s1, w0 + w1};
+    }
+};
 
 // ---- the 32 largest keys of a block -----------------------------------------------
 __device__ __forceinline__ uint64_t shfl_key(uint64_t k, int o) { return __shfl_xor_sync(kAll, k, o); }
@@ -151,51 +225,149 @@ struct Fwd {
     const uint32_t* targets;
     float *logprob, *entropy, *stats, *top_logprobs;
     int32_t* top_ids;
-    int classes, top;
+    int classes, top, splits;  // splits: CTAs of a row, one cluster
 };
 
+constexpr int kHits = 128;  // logits that reach the bound, before the slow way
+
+// grid: rows x splits.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(Fwd a) {
-    constexpr int E = RowView<T>::E, kAhead = 4;
+__global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(Fwd a) {
+    constexpr int E = RowView<T>::E;
     __shared__ Stats parts[kWarps];
+    __shared__ Stats of_cta[8];          // in the cluster's first CTA
+    __shared__ uint64_t of_top[TOP ? 8 : 1][32];
     __shared__ uint64_t lists[TOP ? kWarps : 1][32];
-    __shared__ uint64_t chosen[32];
-    const int64_t r = blockIdx.x;
+    __shared__ uint64_t chosen[32], hits[TOP ? kHits : 1];
+    __shared__ int n_hits;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int splits = a.splits, rank = splits > 1 ? (int)(blockIdx.x % splits) : 0;
+    const int64_t r = splits > 1 ? blockIdx.x / splits : blockIdx.x;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const T* x = (const T*)a.logits + r * a.stride;
     const RowView<T> row(x, a.classes);
+    if (splits > 1) asm volatile("barrier.cluster.arrive;" ::: "memory");
+    if (TOP && tid == 0) n_hits = 0;
 
-    Stats st{kLowest, 0.f, 0.f};
-    uint64_t best = 0;  // (order of the value, ~piece)
-    for (int j0 = tid; j0 < row.pieces; j0 += kAhead * kThreads) {
-        float v[kAhead][E];
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            const int j = j0 + u * kThreads;
-            if (j < row.pieces) row.load(j, v[u], -INFINITY);
+    // Thread tid of CTA rank owns the pieces mine, mine + step, ...
+    const int mine = rank * kThreads + tid, step = splits * kThreads;
+    Running run;
+    float best_v = -INFINITY;
+    int best_j = -1;
+    auto note = [&](float top, int j) {  // a piece's largest logit
+        if constexpr (TOP) {
+            if (top > best_v || best_j < 0) best_j = j, best_v = top;
         }
+    };
+    auto add_partial = [&](int j) {
+        float v[E];
+        row.load(j, v, -INFINITY);
+        float top = v[0];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            const int j = j0 + u * kThreads;
-            if (j >= row.pieces) break;
-            float top = v[u][0];
+        for (int e = 1; e < E; ++e) top = fmaxf(top, v[e]);
+        note(top, j);
+        run.raise(top);
+        run.add(v);
+    };
+    if (mine == 0 && !row.whole(0)) add_partial(0);
+    const int end = row.end();
+    for (int j0 = mine < row.begin() ? mine + step : mine; j0 < end; j0 += kAhead * step) {
+        uint4 u[kAhead];
+        float top = -INFINITY;
 #pragma unroll
-            for (int e = 1; e < E; ++e) top = fmaxf(top, v[u][e]);
-            if constexpr (TOP) {
-                const uint64_t key = (uint64_t)order_of(top) << 32 | (uint32_t)~j;
-                best = key > best ? key : best;
+        for (int k = 0; k < kAhead; ++k)
+            if (j0 + k * step < end) u[k] = row.raw(j0 + k * step);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+            if (j0 + k * step < end) {
+                const float t = RowView<T>::top(u[k]);
+                note(t, j0 + k * step);
+                top = fmaxf(top, t);
             }
-            add_piece(st, v[u], top);
-        }
-    }
+        run.raise(top);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        st = join(st, Stats{__shfl_xor_sync(kAll, st.m, o), __shfl_xor_sync(kAll, st.s, o), __shfl_xor_sync(kAll, st.w, o)});
+        for (int k = 0; k < kAhead; ++k)
+            if (j0 + k * step < end) {
+                float v[E];
+                RowView<T>::decode(u[k], v);
+                run.add(v);
+            }
+    }
+    const int last = row.pieces - 1;
+    if (last > 0 && last >= end && last % step == mine) add_partial(last);
+    Stats st = join_lanes<32>(run.stats());
     if (lane == 0) parts[warp] = st;
     __syncthreads();
-    st = parts[0];
+    st = join_lanes<kWarps>(parts[lane % kWarps]);
+
+    uint64_t found = 0;
+    if constexpr (TOP) {
+        const uint64_t key = best_j < 0 ? 0 : (uint64_t)order_of(best_v) << 32 | (uint32_t)~best_j;
+        const uint64_t k = block_largest(sort_keys(key, lane), lists, warp, lane);
+        if (warp == 0) chosen[lane] = k;
+        __syncthreads();
+        const uint64_t bound = chosen[a.top - 1];
+        // The chosen threads' pieces again, each by a warp; a piece's element counts when
+        // (its order, ~its piece) reaches the bound.
+        auto scan = [&](auto&& take) {
+            for (int c = warp; c < a.top; c += kWarps) {
+                if (chosen[c] == 0) break;
+                for (int j0 = (int)(~(uint32_t)chosen[c] % step); j0 < row.pieces; j0 += 32 * step) {
+                    const int j = j0 + lane * step;
+                    float v[E];
+                    if (j < row.pieces) row.load(j, v, -INFINITY);
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) st = join(st, parts[w]);
+                    for (int e = 0; e < E; ++e) {
+                        const int i = row.first(j) + e;
+                        uint64_t key = 0;
+                        if (j < row.pieces && i >= 0 && i < a.classes) {
+                            const uint64_t high = (uint64_t)order_of(v[e]) << 32;
+                            if ((high | (uint32_t)~j) >= bound) key = high | (uint32_t)~i;
+                        }
+                        take(key);
+                    }
+                }
+            }
+        };
+        scan([&](uint64_t key) {
+            if (key != 0) {
+                const int at = atomicAdd(&n_hits, 1);
+                if (at < kHits) hits[at] = key;
+            }
+        });
+        __syncthreads();
+        // There are at least as many hits as alternatives, and rarely many more: one warp puts
+        // them in order (their number alone depends on the row, not on the atomics' order).
+        const int n = n_hits;
+        if (n <= kHits) {
+            if (warp == 0)
+                for (int i = 0; i < n; i += 32) {
+                    const uint64_t sorted = sort_keys(i + lane < n ? hits[i + lane] : 0, lane);
+                    found = i == 0 ? sorted : merge_keys(found, __shfl_sync(kAll, sorted, 31 - lane), lane);
+                }
+        } else {  // a row made of ties, say: every warp keeps the best of what it sees
+            scan([&](uint64_t key) {
+                if (__any_sync(kAll, key != 0)) {
+                    const uint64_t sorted = sort_keys(key, lane);
+                    found = merge_keys(found, __shfl_sync(kAll, sorted, 31 - lane), lane);
+                }
+            });
+            found = block_largest(found, lists, warp, lane);
+        }
+    }
+    if (splits > 1) {  // to the first CTA, which joins them in order
+        asm volatile("barrier.cluster.wait;" ::: "memory");
+        if (tid == 0) *cluster.map_shared_rank(&of_cta[rank], 0) = st;
+        if (TOP && warp == 0) *cluster.map_shared_rank(&of_top[TOP ? rank : 0][lane], 0) = found;
+        asm volatile("barrier.cluster.arrive;\nbarrier.cluster.wait;" ::: "memory");
+        if (rank != 0) return;
+        st = of_cta[0];
+        for (int k = 1; k < splits; ++k) st = join(st, of_cta[k]);
+        if (TOP && warp == 0) {
+            found = of_top[0][lane];
+            for (int k = 1; k < splits; ++k) found = merge_keys(found, of_top[TOP ? k : 0][31 - lane], lane);
+        }
+    }
     const float log_s = logf(st.s);
     if (tid == 0) {
         const uint32_t t = a.targets[r];
@@ -204,42 +376,10 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(Fwd a) {
         a.entropy[r] = h;
         if (a.stats) a.stats[3 * r] = st.m, a.stats[3 * r + 1] = log_s, a.stats[3 * r + 2] = h;
     }
-    if constexpr (TOP) {
-        const uint64_t k = block_largest(sort_keys(best, lane), lists, warp, lane);
-        if (warp == 0) chosen[lane] = k;
-        __syncthreads();
-        const uint64_t bound = chosen[a.top - 1];
-        // The chosen threads' pieces again, each by a warp; a piece's element counts when
-        // (its order, ~its piece) reaches the bound.
-        uint64_t mine = 0;
-        for (int c = warp; c < a.top; c += kWarps) {
-            if (chosen[c] == 0) break;
-            const int owner = (int)(~(uint32_t)chosen[c] % kThreads);
-            for (int j0 = owner; j0 < row.pieces; j0 += 32 * kThreads) {
-                const int j = j0 + lane * kThreads;
-                float v[E];
-                if (j < row.pieces) row.load(j, v, -INFINITY);
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const int i = row.first(j) + e;
-                    uint64_t key = 0;
-                    if (j < row.pieces && i >= 0 && i < a.classes) {
-                        const uint64_t high = (uint64_t)order_of(v[e]) << 32;
-                        if ((high | (uint32_t)~j) >= bound) key = high | (uint32_t)~i;
-                    }
-                    if (__any_sync(kAll, key != 0)) {
-                        const uint64_t sorted = sort_keys(key, lane);
-                        mine = merge_keys(mine, __shfl_sync(kAll, sorted, 31 - lane), lane);
-                    }
-                }
-            }
-        }
-        const uint64_t found = block_largest(mine, lists, warp, lane);
-        if (warp == 0 && lane < a.top) {
-            const int i = (int)~(uint32_t)found;
-            a.top_ids[r * a.top + lane] = i;
-            a.top_logprobs[r * a.top + lane] = ((float)x[i] - st.m) - log_s;
-        }
+    if (TOP && warp == 0 && lane < a.top) {
+        const int i = (int)~(uint32_t)found;
+        a.top_ids[r * a.top + lane] = i;
+        a.top_logprobs[r * a.top + lane] = ((float)x[i] - st.m) - log_s;
     }
 }
 
@@ -263,7 +403,7 @@ __device__ __forceinline__ void store_piece(T* p, const float (&d)[16 / sizeof(T
 
 // grid: (rows, splits of a row).
 template <typename T>
-__global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(Bwd a) {
+__global__ void __launch_bounds__(kThreads, 4) token_logprobs_bwd_kernel(Bwd a) {
     constexpr int E = RowView<T>::E;
     const int64_t r = blockIdx.x;
     const RowView<T> row((const T*)a.logits + r * a.stride, a.classes);
@@ -275,44 +415,91 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(Bwd a) {
     if (a.g_logprob && t >= (uint32_t)a.classes) gt = __int_as_float(0x7fffffff);  // as its log probability
     const float gh = a.g_entropy ? a.g_entropy[r] : 0.f;
     const float c = gt + gh * h;
-    for (int j = blockIdx.y * kThreads + threadIdx.x; j < row.pieces; j += gridDim.y * kThreads) {
-        float v[E];
-        row.load(j, v, 0.f);
-        const int i0 = row.first(j);
+    const uint64_t minus_m = f2_pack(-m, -m), minus_ls = f2_pack(-log_s, -log_s), l2 = f2_pack(kLog2e, kLog2e);
+    const uint64_t minus_gh = f2_pack(-gh, -gh), minus_c = f2_pack(-c, -c);
+    // p (-g_H ln p - (g_t + g_H H)), and g_t more at the target
+    auto gradient = [&](float (&v)[E], int i0) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const float z = max_nan((v[e] - m) - log_s, kFloor);
-            const float p = ex2(z * kLog2e);
-            v[e] = -p * fmaf(gh, z, c) + (i0 + e == (int)t ? gt : 0.f);
+        for (int e = 0; e < E; e += 2) {
+            float z0, z1, p0, p1;
+            ptx::f2_unpack(f2_add(f2_add(f2_pack(v[e], v[e + 1]), minus_m), minus_ls), z0, z1);
+            const uint64_t z = f2_pack(max_nan(z0, kFloor), max_nan(z1, kFloor));
+            ptx::f2_unpack(f2_mul(z, l2), p0, p1);
+            ptx::f2_unpack(f2_mul(f2_pack(ex2(p0), ex2(p1)), f2_fma(minus_gh, z, minus_c)), v[e], v[e + 1]);
         }
-        if (together && row.whole(j)) {
-            store_piece(out + i0, v);
-        } else {
+        if ((int)t - i0 >= 0 && (int)t - i0 < E) {
 #pragma unroll
             for (int e = 0; e < E; ++e)
-                if (i0 + e >= 0 && i0 + e < a.classes) out[i0 + e] = T(v[e]);
+                if (i0 + e == (int)t) v[e] += gt;
         }
+    };
+    auto one = [&](int j) {
+        float v[E];
+        row.load(j, v, 0.f);
+        gradient(v, row.first(j));
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int i = row.first(j) + e;
+            if (i >= 0 && i < a.classes) out[i] = T(v[e]);
+        }
+    };
+    const int mine = blockIdx.y * kThreads + threadIdx.x, step = gridDim.y * kThreads, end = row.end();
+    if (!together) {
+        for (int j = mine; j < row.pieces; j += step) one(j);
+        return;
     }
+    if (mine == 0 && !row.whole(0)) one(0);
+    for (int j0 = mine < row.begin() ? mine + step : mine; j0 < end; j0 += kAhead * step) {
+        uint4 u[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+            if (j0 + k * step < end) u[k] = row.raw(j0 + k * step);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+            if (j0 + k * step < end) {
+                float v[E];
+                RowView<T>::decode(u[k], v);
+                gradient(v, row.first(j0 + k * step));
+                store_piece(out + row.first(j0 + k * step), v);
+            }
+    }
+    const int last = row.pieces - 1;
+    if (last > 0 && last >= end && last % step == mine) one(last);
+}
+
+template <typename T, bool TOP>
+cudaError_t launch_fwd(cudaStream_t st, int sm_count, Fwd a, int rows) {
+    // Rows that do not occupy the SMs are split over a cluster each, as long as every thread keeps
+    // a piece. More splits only repeat the joins (515 rows of 131071 f32 with 20
+    // alternatives: 70 us whole, 72 in two, 103 in eight).
+    const int pieces = (int)(((int64_t)a.classes * (int)sizeof(T) + 15) / 16) + 1;
+    a.splits = 1;
+    while (a.splits < 8 && rows * (int64_t)a.splits < sm_count && pieces > kThreads * a.splits) a.splits *= 2;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)rows * (unsigned)a.splits);
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = (unsigned)a.splits;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = a.splits > 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, TOP>, a);
+    if (e == cudaSuccess) note_launch();
+    return e != cudaSuccess ? e : cudaGetLastError();
 }
 
 }  // namespace
 
-cudaError_t token_logprobs_fwd(cudaStream_t st, hx_dtype dt, const void* logits, int64_t stride, const uint32_t* targets,
-                               float* logprob, float* entropy, float* stats, int top, int32_t* top_ids,
-                               float* top_logprobs, int rows, int classes) {
-    const Fwd a{logits, stride, targets, logprob, entropy, stats, top_logprobs, top_ids, classes, top};
-    if (dt == HX_F32) {
-        if (top > 0)
-            token_logprobs_kernel<float, true><<<(unsigned)rows, kThreads, 0, st>>>(a);
-        else
-            token_logprobs_kernel<float, false><<<(unsigned)rows, kThreads, 0, st>>>(a);
-    } else if (top > 0) {
-        token_logprobs_kernel<__nv_bfloat16, true><<<(unsigned)rows, kThreads, 0, st>>>(a);
-    } else {
-        token_logprobs_kernel<__nv_bfloat16, false><<<(unsigned)rows, kThreads, 0, st>>>(a);
-    }
-    note_launch();
-    return cudaGetLastError();
+cudaError_t token_logprobs_fwd(cudaStream_t st, int sm_count, hx_dtype dt, const void* logits, int64_t stride,
+                               const uint32_t* targets, float* logprob, float* entropy, float* stats, int top,
+                               int32_t* top_ids, float* top_logprobs, int rows, int classes) {
+    const Fwd a{logits, stride, targets, logprob, entropy, stats, top_logprobs, top_ids, classes, top, 1};
+    if (dt == HX_F32)
+        return top > 0 ? launch_fwd<float, true>(st, sm_count, a, rows) : launch_fwd<float, false>(st, sm_count, a, rows);
+    return top > 0 ? launch_fwd<__nv_bfloat16, true>(st, sm_count, a, rows)
+                   : launch_fwd<__nv_bfloat16, false>(st, sm_count, a, rows);
 }
 
 cudaError_t token_logprobs_bwd(cudaStream_t st, int sm_count, hx_dtype dt, const void* logits, int64_t stride,

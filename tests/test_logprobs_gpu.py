@@ -2,8 +2,9 @@
 
 Tolerances, from the arithmetic, for a row with z = x - max, s = sum e^z: an
 exponential is good to 2^-22 and its argument is rounded twice (2^-23 |z|), a
-thread adds V/512 of them and a tree of 9 + 16 joins them, each at 2^-24 and
-2^-22 for the weights of the joins. So ln s is off by less than
+thread adds V/512 of them (in each of two halves) and a tree of 1 + 5 + 3 levels,
+with up to 8 CTAs after it, joins them, each at 2^-24 and 2^-22 for the weights of the
+joins. So ln s is off by less than
 rel = 2^-21 + (V/512 + 64) 2^-23 + 2^-22 E|z|, a log probability by that and 2^-23
 (|z| + |ln s|), the entropy by rel (1 + H) and 2^-22 E(z^2 + |z|).
 """
