@@ -777,7 +777,7 @@ int hx_paged_attention_workspace_size(hx_dtype dt, const hx_paged_cache* cache, 
     if (bytes == nullptr) return HX_ERR_INVALID;
     int st;
     if ((st = validate_cache(nullptr, dt, cache, "")) || (st = paged_heads(nullptr, cache, Hq, ""))) return st;
-    *bytes = hx::paged_attn_workspace_bytes(dt, Hq, cache->H, cache->D);
+    *bytes = hx::paged_attn_workspace_bytes(dt, Hq, cache->H, cache->D, cache->num_seqs);
     return HX_OK;
 }
 
@@ -798,7 +798,7 @@ int hx_paged_attention(hx_ctx* c, hx_dtype dt, const hx_paged_cache* cache, int 
     DeviceGuard g(c->device);
     NvtxRange nv(who);
     LaunchCount lc(c);
-    const uint64_t need = hx::paged_attn_workspace_bytes(dt, Hq, cache->H, cache->D);
+    const uint64_t need = hx::paged_attn_workspace_bytes(dt, Hq, cache->H, cache->D, cache->num_seqs);
     void* ws = workspace;
     if (ws == nullptr) {
         cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
@@ -822,8 +822,7 @@ int hx_paged_attention(hx_ctx* c, hx_dtype dt, const hx_paged_cache* cache, int 
     a.Hq = Hq;
     a.G = Hq / cache->H;
     a.scale_log2 = scale * 1.4426950408889634f;
-    a.part = (float*)ws;
-    st = check_cuda(c, hx::paged_attn(c->stream, c->sm_count, dt, a), who);
+    st = check_cuda(c, hx::paged_attn(c->stream, c->sm_count, dt, a, ws), who);
     if (workspace == nullptr) hx_free(c, ws);  // stream-ordered: the next user of the slab queues behind us
     return st;
 }

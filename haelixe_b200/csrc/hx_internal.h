@@ -155,6 +155,9 @@ struct PagedAppend {
     const int32_t *seq_ids, *positions;
 };
 cudaError_t paged_append(cudaStream_t st, int sm_count, hx_dtype dt, const PagedAppend& a, int tokens);
+struct PagedPlan {
+    int64_t run, empty;
+};
 struct PagedAttn {
     PagedView cache;
     const void* q;  // [num_seqs, Hq, D]
@@ -164,10 +167,13 @@ struct PagedAttn {
     int64_t q_sn, q_sh, o_sn, o_sh;
     int Hq, G;  // query heads, query heads of one key head
     float scale_log2;
+    // in the workspace, set by paged_attn
+    PagedPlan* plan;
+    int64_t* starts;
     float* part;
 };
-uint64_t paged_attn_workspace_bytes(hx_dtype dt, int Hq, int Hkv, int D);
-cudaError_t paged_attn(cudaStream_t st, int sm_count, hx_dtype dt, const PagedAttn& a);
+uint64_t paged_attn_workspace_bytes(hx_dtype dt, int Hq, int Hkv, int D, int num_seqs);
+cudaError_t paged_attn(cudaStream_t st, int sm_count, hx_dtype dt, PagedAttn a, void* workspace);
 
 // ---- log probabilities of given tokens (logprobs.cu) ----
 // stats: 3 floats a row (maximum, log of the sum relative to it, entropy), for the backward.

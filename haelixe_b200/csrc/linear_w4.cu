@@ -25,6 +25,7 @@
 #include <atomic>
 
 #include "hx_internal.h"
+#include "launch.h"
 #include "mma_bf16.cuh"
 #include "sm100_ptx.cuh"
 #include "tma_host.h"
@@ -193,6 +194,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * NT * CH <= 8 ? 2 : 1) li
         }
         __syncthreads();
     }
+    after_prior_kernels();
+    may_start_next();
+
     // Unit u into stage i: each warp its own words, the group's first warp x as well. What is
     // past the last row, column or k reads as zero.
     auto copy_unit = [&](int u, int i) {
@@ -461,20 +465,8 @@ cudaError_t launch(cudaStream_t st, int sm_count, Args a) {
                 !row_map(&a.x_map, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.x,
                          a.rows, a.in, sizeof(T), 128 / (int)sizeof(T), R)))
         return cudaErrorInvalidValue;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(tiles() << a.ks_log), (unsigned)((a.rows + R - 1) / R));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = (size_t)bytes;
-    cfg.stream = st;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = 1u << a.ks_log;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, a);
-    if (e == cudaSuccess) note_launch();
-    return e != cudaSuccess ? e : cudaGetLastError();
+    return launch_overlapped(st, kernel, dim3((unsigned)(tiles() << a.ks_log), (unsigned)((a.rows + R - 1) / R)), kThreads,
+                             (size_t)bytes, 1 << a.ks_log, a);
 }
 
 // Unaligned operands and odd widths take one form of the kernel each, the rest one by the

@@ -20,6 +20,7 @@
 #include <cooperative_groups.h>
 
 #include "hx_internal.h"
+#include "launch.h"
 #include "mma_bf16.cuh"
 #include "sm100_ptx.cuh"
 
@@ -248,6 +249,8 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(Fwd a) {
     const RowView<T> row(x, a.classes);
     if (splits > 1) asm volatile("barrier.cluster.arrive;" ::: "memory");
     if (TOP && tid == 0) n_hits = 0;
+    after_prior_kernels();
+    may_start_next();
 
     // Thread tid of CTA rank owns the pieces mine, mine + step, ...
     const int mine = rank * kThreads + tid, step = splits * kThreads;
@@ -405,6 +408,8 @@ __device__ __forceinline__ void store_piece(T* p, const float (&d)[16 / sizeof(T
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) token_logprobs_bwd_kernel(Bwd a) {
     constexpr int E = RowView<T>::E;
+    after_prior_kernels();
+    may_start_next();
     const int64_t r = blockIdx.x;
     const RowView<T> row((const T*)a.logits + r * a.stride, a.classes);
     T* out = (T*)a.dlogits + r * a.dstride;
@@ -475,19 +480,8 @@ cudaError_t launch_fwd(cudaStream_t st, int sm_count, Fwd a, int rows) {
     const int pieces = (int)(((int64_t)a.classes * (int)sizeof(T) + 15) / 16) + 1;
     a.splits = 1;
     while (a.splits < 8 && rows * (int64_t)a.splits < sm_count && pieces > kThreads * a.splits) a.splits *= 2;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)rows * (unsigned)a.splits);
-    cfg.blockDim = dim3(kThreads);
-    cfg.stream = st;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = (unsigned)a.splits;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = a.splits > 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, TOP>, a);
-    if (e == cudaSuccess) note_launch();
-    return e != cudaSuccess ? e : cudaGetLastError();
+    return launch_overlapped(st, token_logprobs_kernel<T, TOP>, dim3((unsigned)rows * (unsigned)a.splits), kThreads, 0,
+                             a.splits > 1 ? a.splits : 0, a);
 }
 
 }  // namespace
@@ -511,12 +505,8 @@ cudaError_t token_logprobs_bwd(cudaStream_t st, int sm_count, hx_dtype dt, const
     const int most = (pieces + kThreads - 1) / kThreads;
     if (splits > most) splits = most;
     const dim3 grid((unsigned)rows, (unsigned)splits);
-    if (dt == HX_F32)
-        token_logprobs_bwd_kernel<float><<<grid, kThreads, 0, st>>>(a);
-    else
-        token_logprobs_bwd_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(a);
-    note_launch();
-    return cudaGetLastError();
+    return launch_overlapped(st, dt == HX_F32 ? token_logprobs_bwd_kernel<float> : token_logprobs_bwd_kernel<__nv_bfloat16>,
+                             grid, kThreads, 0, 0, a);
 }
 
 }  // namespace hx

@@ -9,6 +9,7 @@
 // p = 10^5 is more than a bf16 rounding of the result. One CTA computes the
 // D/2 (cos, sin) pairs of its token once, for all of its heads.
 #include "hx_internal.h"
+#include "launch.h"
 #include "mma_bf16.cuh"
 
 namespace hx {
@@ -56,6 +57,8 @@ __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) paged_append_kernel(PagedAppend a) {
     __shared__ float2 cs[128];  // (cos, sin) of each pair
+    after_prior_kernels();
+    may_start_next();
     const int t = blockIdx.x;
     const int seq = a.seq_ids[t];
     if (seq < 0) return;  // padding: nothing of this token is touched
@@ -128,12 +131,7 @@ cudaError_t launch(cudaStream_t st, int sm_count, const PagedAppend& a, int toke
     const int most = (total + kThreads - 1) / kThreads;
     if (splits > most) splits = most;
     const dim3 grid((unsigned)tokens, (unsigned)splits);
-    if (vec)
-        paged_append_kernel<T, true><<<grid, kThreads, 0, st>>>(a);
-    else
-        paged_append_kernel<T, false><<<grid, kThreads, 0, st>>>(a);
-    note_launch();
-    return cudaGetLastError();
+    return launch_overlapped(st, vec ? paged_append_kernel<T, true> : paged_append_kernel<T, false>, grid, kThreads, 0, 0, a);
 }
 
 }  // namespace

@@ -6,11 +6,12 @@
 // the work has to be even over the SMs although lengths differ and are known
 // on the device alone. The (sequence, key head, up to HB of its query heads)
 // items are cut into tiles of 64 keys, the tiles of all items are numbered in a row,
-// and every worker (a 4-warp CTA, as many as are resident at once) takes an
-// equal run of them. A run that holds all of an item writes its result; the
-// others write (max, sum, unnormalised o) to the workspace, at most two a
-// worker, and paged_join_kernel joins an item's parts in the order of its keys
-// (no atomics: the same call gives the same bits).
+// each item's after a few empty places that stand for the time an item takes
+// besides its keys, and every worker (a 4-warp CTA, as many as are resident at
+// once) takes an equal run of them. A run that holds all of an item writes its
+// result; the others write (max, sum, unnormalised o) to the workspace, at most
+// two a worker, and paged_join_kernel joins an item's parts in the order of its
+// keys (no atomics: the same call gives the same bits).
 //
 // Softmax statistics and all sums are f32. A warp keeps a running maximum that
 // only moves when a score passes it by 2^8, so the accumulator is rarely rescaled.
@@ -18,6 +19,7 @@
 #include <atomic>
 
 #include "hx_internal.h"
+#include "launch.h"
 #include "mma_bf16.cuh"
 
 namespace hx {
@@ -26,7 +28,10 @@ namespace {
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kWarpKeys = 16, kTile = kWarps * kWarpKeys;
 constexpr int kMaxWorkers = 1024;
-constexpr int kMinTiles = 2;  // a run shorter than this costs more to join than it saves
+// Empty places of an item, where workers have several tiles each: 64 sequences of 1 to 8192 keys
+// take 79 us without, 52 with 2, 56 with 4. With less to do than that none, so that it is
+// spread as far as it goes.
+constexpr int kItemPlaces = 2, kPlacesFrom = 4;
 constexpr float kLazy = 8.f;  // log2 growth of the maximum that triggers a rescale
 constexpr float kLn2 = 0.69314718055994530942f;
 
@@ -34,50 +39,62 @@ struct Item {
     int n, h, c;  // sequence, key head, chunk of its query heads
 };
 
-// Sequences with nothing to read (len <= 0) or longer than their table row have no tiles;
-// paged_join_kernel writes their rows.
+// Sequences with nothing to read (len <= 0) or longer than their table row have no tiles
+// and no items; paged_join_kernel writes their rows.
 __device__ __forceinline__ int tiles_of(const PagedAttn& a, int n) {
     const int64_t len = a.lens[n];
     return len <= 0 || len > (int64_t)a.cache.max_pages * a.cache.page_size ? 0 : (int)((len + kTile - 1) / kTile);
 }
 
-__device__ __forceinline__ int64_t run_of(int64_t total, int workers) {
-    const int64_t r = (total + workers - 1) / workers;
-    return r < kMinTiles ? kMinTiles : r;
+// Where the work of a call lies: the empty places of an item, the length of a run, the places
+// before each sequence. The first worker leaves it in the workspace for the join.
+using Plan = PagedPlan;
+__device__ __forceinline__ int places_of(int tiles, int empty) { return tiles == 0 ? 0 : tiles + empty; }
+
+__device__ __forceinline__ int64_t div_up(int64_t a, int b) {
+    return a >> 31 == 0 ? (int64_t)(((uint32_t)a + (uint32_t)b - 1) / (uint32_t)b) : (a + b - 1) / b;
 }
 
-// Sum of the tiles of the sequences [0, n) and of all; every thread of the block gets both.
-template <int THREADS>
-__device__ __forceinline__ void tile_sums(const PagedAttn& a, int n, int64_t& before, int64_t& all) {
-    __shared__ int64_t sums[2][THREADS / 32];
-    int64_t b = 0, t = 0;
-    for (int i = threadIdx.x; i < a.cache.num_seqs; i += THREADS) {
-        const int v = tiles_of(a, i);
-        t += v;
-        if (i < n) b += v;
-    }
+// Sums of two numbers over the block, to every thread.
+__device__ __forceinline__ void block_sums(int64_t& x, int64_t& y) {
+    __shared__ int64_t sums[2][kWarps];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        b += __shfl_xor_sync(0xffffffffu, b, o);
-        t += __shfl_xor_sync(0xffffffffu, t, o);
+        x += __shfl_xor_sync(0xffffffffu, x, o);
+        y += __shfl_xor_sync(0xffffffffu, y, o);
     }
-    if (threadIdx.x % 32 == 0) sums[0][threadIdx.x / 32] = b, sums[1][threadIdx.x / 32] = t;
+    if (threadIdx.x % 32 == 0) sums[0][threadIdx.x / 32] = x, sums[1][threadIdx.x / 32] = y;
     __syncthreads();
-    before = all = 0;
+    x = y = 0;
 #pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) before += sums[0][w], all += sums[1][w];
+    for (int w = 0; w < kWarps; ++w) x += sums[0][w], y += sums[1][w];
 }
 
-// The sequence that holds tile `start` of the row (times `per` for each of its
-// tiles), and the number of tiles before it. start < total.
-__device__ __forceinline__ void find_sequence(const PagedAttn& a, int64_t start, int per, int& n, int64_t& before) {
+// This worker's run [start, end) and the sequence that holds its first place (each sequence has
+// `per` items), with the places before that sequence. False when there is nothing to do.
+__device__ __forceinline__ bool find_run(const PagedAttn& a, int per, int64_t& start, int64_t& end, int& n,
+                                         int64_t& before, int& empty) {
     __shared__ int64_t warp_sum[kWarps];
     __shared__ int found_n;
     __shared__ int64_t found_before;
+    const int mine = (int)threadIdx.x < a.cache.num_seqs ? tiles_of(a, threadIdx.x) : 0;
+    int64_t tiles = mine, items = mine > 0;
+    for (int i = threadIdx.x + kThreads; i < a.cache.num_seqs; i += kThreads) {
+        const int t = tiles_of(a, i);
+        tiles += t, items += t > 0;
+    }
+    block_sums(tiles, items);
+    empty = tiles * per >= (int64_t)kPlacesFrom * gridDim.x ? kItemPlaces : 0;
+    const int64_t total = (tiles + items * empty) * per, run = div_up(total, gridDim.x);
+    const bool first = blockIdx.x == 0;
+    if (first && threadIdx.x == 0) *a.plan = Plan{run, empty};
+    start = run * blockIdx.x;
+    end = min(total, start + run);
+    if (start >= end) return false;
     int64_t carry = 0;
     for (int base = 0;; base += kThreads) {
         const int i = base + threadIdx.x;
-        const int64_t v = i < a.cache.num_seqs ? (int64_t)tiles_of(a, i) * per : 0;
+        const int64_t v = (int64_t)places_of(base == 0 ? mine : i < a.cache.num_seqs ? tiles_of(a, i) : 0, empty) * per;
         int64_t incl = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -94,12 +111,14 @@ __device__ __forceinline__ void find_sequence(const PagedAttn& a, int64_t start,
         }
         incl += prev + carry;
         if (incl - v <= start && start < incl) found_n = i, found_before = incl - v;
+        if (first && i < a.cache.num_seqs) a.starts[i] = incl - v;
         carry += block;
         __syncthreads();
-        if (start < carry || base + kThreads >= a.cache.num_seqs) break;
+        if ((start < carry && !first) || base + kThreads >= a.cache.num_seqs) break;
     }
     n = found_n;
     before = found_before;
+    return true;
 }
 
 // Element offset of key `key` of sequence n in the cache; kNone at or past len, kBad when
@@ -379,6 +398,30 @@ struct AttnF32 {
         float f[kWarps][GH];
     };
 
+    static constexpr bool kAhead = DV <= 4 && DV * GH <= 16;
+
+    // This lane's elements of a value row; zero without a row.
+    static __device__ __forceinline__ void load_v(float (&v)[DV], const float* vh, int64_t o, int lane, int D) {
+#pragma unroll
+        for (int x = 0; x < DV; ++x) v[x] = 0.f;
+        if (o < 0) return;
+        if constexpr (DV == 2) {
+            if (2 * lane < D) {
+                const float2 u = *reinterpret_cast<const float2*>(vh + o + 2 * lane);
+                v[0] = u.x, v[1] = u.y;
+            }
+        } else {
+#pragma unroll
+            for (int x = 0; x < DV; x += 4) {
+                const int d = 32 * x + 4 * lane;
+                if (d < D) {
+                    const float4 u = *reinterpret_cast<const float4*>(vh + o + d);
+                    v[x] = u.x, v[x + 1] = u.y, v[x + 2] = u.z, v[x + 3] = u.w;
+                }
+            }
+        }
+    }
+
     const PagedAttn& a;
     Scratch& sm;
     __device__ __forceinline__ AttnF32(const PagedAttn& args, Scratch& scratch) : a(args), sm(scratch) {}
@@ -416,6 +459,12 @@ struct AttnF32 {
             const uint32_t bad = __ballot_sync(0xffffffffu, off == kBad);
             const uint32_t none = __ballot_sync(0xffffffffu, off == kNone);
             const int64_t o0 = __shfl_sync(0xffffffffu, off, g), o1 = __shfl_sync(0xffffffffu, off, g + 8);
+            // The values are on their way while the scores are taken, where the registers allow it.
+            float v[kWarpKeys][DV];
+            if constexpr (kAhead) {
+#pragma unroll
+                for (int kk = 0; kk < kWarpKeys; ++kk) load_v(v[kk], vh, __shfl_sync(0xffffffffu, off, kk), lane, D);
+            }
             float s0[GH], s1[GH];
 #pragma unroll
             for (int h = 0; h < GH; ++h) s0[h] = s1[h] = 0.f;
@@ -479,32 +528,12 @@ struct AttnF32 {
             }
 #pragma unroll
             for (int kk = 0; kk < kWarpKeys; ++kk) {
-                const int64_t o = __shfl_sync(0xffffffffu, off, kk);
-                float v[DV];
-#pragma unroll
-                for (int x = 0; x < DV; ++x) v[x] = 0.f;
-                if (o >= 0) {
-                    if constexpr (DV == 2) {
-                        if (2 * lane < D) {
-                            const float2 u = *reinterpret_cast<const float2*>(vh + o + 2 * lane);
-                            v[0] = u.x, v[1] = u.y;
-                        }
-                    } else {
-#pragma unroll
-                        for (int x = 0; x < DV; x += 4) {
-                            const int d = 32 * x + 4 * lane;
-                            if (d < D) {
-                                const float4 u = *reinterpret_cast<const float4*>(vh + o + d);
-                                v[x] = u.x, v[x + 1] = u.y, v[x + 2] = u.z, v[x + 3] = u.w;
-                            }
-                        }
-                    }
-                }
+                if constexpr (!kAhead) load_v(v[kk], vh, __shfl_sync(0xffffffffu, off, kk), lane, D);
 #pragma unroll
                 for (int h = 0; h < GH; ++h) {
                     const float p = sm.p[warp][kk][h];
 #pragma unroll
-                    for (int x = 0; x < DV; ++x) acc[h][x] = fmaf(p, v[x], acc[h][x]);
+                    for (int x = 0; x < DV; ++x) acc[h][x] = fmaf(p, v[kk][x], acc[h][x]);
                 }
             }
             __syncwarp();
@@ -524,33 +553,36 @@ struct AttnF32 {
 
 template <typename T, typename W>
 __device__ __forceinline__ void paged_worker(const PagedAttn& a, W& w, Parts<W::HB, W::kD>& sp) {
+    after_prior_kernels();
+    may_start_next();  // the join, which waits for all workers
     const int chunks = (a.G + W::HB - 1) / W::HB;
     const int per = a.cache.H * chunks;
-    int64_t before, total;
-    tile_sums<kThreads>(a, 0, before, total);
-    total *= per;
-    const int64_t run = run_of(total, gridDim.x);
-    const int64_t start = run * blockIdx.x, end = min(total, start + run);
-    if (start >= end) return;
-    int n;
-    find_sequence(a, start, per, n, before);
-    int T_n = tiles_of(a, n);
-    int item = (int)((start - before) / T_n), tile = (int)((start - before) % T_n);
+    int64_t start, end, before;
+    int n, empty;
+    if (!find_run(a, per, start, end, n, before, empty)) return;
+    int tiles = tiles_of(a, n), places = places_of(tiles, empty);
+    int item = (int)((start - before) / places), place = (int)((start - before) - (int64_t)item * places);
     for (int64_t at = start; at < end;) {
-        const int tiles = (int)min((int64_t)(T_n - tile), end - at);
-        const Item it{n, item / chunks, item % chunks};
-        w.run(it, tile, tiles, sp);
-        __syncthreads();
-        finish_item<T, W::HB, W::kD>(a, sp, it, tiles == T_n, 2 * blockIdx.x + (at != start));
-        __syncthreads();
-        at += tiles;
-        tile = 0;
+        const int take = (int)min((int64_t)(places - place), end - at);
+        const int first = max(place - empty, 0), last = place + take - empty;  // tiles [first, last)
+        if (last > first) {
+            const Item it{n, item / chunks, item % chunks};
+            w.run(it, first, last - first, sp);
+            __syncthreads();
+            // The worker's second part is the one whose first tile it has.
+            finish_item<T, W::HB, W::kD>(a, sp, it, last - first == tiles,
+                                         2 * blockIdx.x + (first == 0 && at - place + empty > start));
+            __syncthreads();
+        }
+        at += take;
+        place = 0;
         if (++item == per && at < end) {
             item = 0;
             do {
                 if (++n == a.cache.num_seqs) return;
-                T_n = tiles_of(a, n);
-            } while (T_n == 0);
+                tiles = tiles_of(a, n);
+            } while (tiles == 0);
+            places = places_of(tiles, empty);
         }
     }
 }
@@ -572,48 +604,60 @@ __global__ void __launch_bounds__(kThreads) paged_attn_f32_kernel(PagedAttn a) {
 }
 
 // One CTA a query head of a sequence: the join of its item's parts, the zeros of an
-// empty sequence, or the NaN of one that is longer than its table row.
-constexpr int kJoinThreads = 256;
+// empty sequence, or the NaN of one that is longer than its table row. It is launched with the
+// workers and waits for them here.
+constexpr int kJoinWarps = 8;  // at most
 template <typename T, int HB>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedAttn a, int workers) {
-    constexpr int kJoinWarps = kJoinThreads / 32;
+__global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(PagedAttn a, int workers) {
     __shared__ float so[kJoinWarps][256];
     __shared__ float2 sml[kJoinWarps];
+    may_start_next();
+    const int threads = blockDim.x, warps = threads / 32;
     const int n = blockIdx.x / a.Hq, hq = blockIdx.x % a.Hq, D = a.cache.D;
-    const int chunks = (a.G + HB - 1) / HB, per = a.cache.H * chunks;
+    const int chunks = (a.G + HB - 1) / HB;
     T* o = (T*)a.o + (int64_t)n * a.o_sn + (int64_t)hq * a.o_sh;
     float* lse = a.lse ? a.lse + (int64_t)n * a.Hq + hq : nullptr;
-    const int T_n = tiles_of(a, n);
-    if (T_n == 0) {
+    after_prior_kernels();
+    const int tiles = tiles_of(a, n), in_group = hq % a.G;
+    if (tiles == 0) {
         const bool empty = a.lens[n] <= 0;
         const float nan = __int_as_float(0x7fffffff);
-        for (int d = threadIdx.x; d < D; d += kJoinThreads) o[d] = T(empty ? 0.f : nan);
+        for (int d = threadIdx.x; d < D; d += threads) o[d] = T(empty ? 0.f : nan);
         if (threadIdx.x == 0 && lse) *lse = empty ? -INFINITY : nan;
         return;
     }
-    int64_t before, total;
-    tile_sums<kJoinThreads>(a, n, before, total);
-    const int64_t run = run_of(total * per, workers);
-    const int in_group = hq % a.G;
-    const int64_t first = before * per + ((int64_t)(hq / a.G) * chunks + in_group / HB) * T_n, last = first + T_n - 1;
-    const int w0 = (int)(first / run), w1 = min((int)(last / run), workers - 1);
+    const int64_t run = a.plan->run;
+    const int empty = (int)a.plan->empty;
+    const int64_t first = a.starts[n] + ((int64_t)(hq / a.G) * chunks + in_group / HB) * places_of(tiles, empty) + empty;
+    const int w0 = (int)(first / run), w1 = min((int)((first + tiles - 1) / run), workers - 1);
     if (w0 == w1) return;  // one worker had it all
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, head = in_group % HB;
     float m = -INFINITY, l = 0.f, acc[8];
 #pragma unroll
     for (int x = 0; x < 8; ++x) acc[x] = 0.f;
-    // Warp w takes the parts w0 + w, w0 + w + 8, ...; lane l the elements l, l + 32, ...
-    for (int w = w0 + warp; w <= w1; w += kJoinWarps) {
-        const int slot = 2 * w + (first > run * w);
-        const float* part = a.part + (int64_t)slot * HB * (D + 2);
-        const float2 ml = reinterpret_cast<const float2*>(part + HB * D)[head];
-        const float mn = fmaxf(m, ml.x);
-        const float f0 = exp2f(m - safe_max(mn)), f1 = exp2f(ml.x - safe_max(mn));
-        m = mn;
-        l = l * f0 + ml.y * f1;
+    // Warp w takes the parts w0 + w, w0 + w + warps, ..., two at once; lane l the elements l, l + 32, ...
+    auto part_of = [&](int w) { return a.part + (int64_t)(2 * w + (first > run * w)) * HB * (D + 2); };
+    for (int w = w0 + warp; w <= w1; w += 2 * warps) {
+        const bool two = w + warps <= w1;
+        const float *p0 = part_of(w), *p1 = two ? part_of(w + warps) : p0;
+        const float2 ml0 = reinterpret_cast<const float2*>(p0 + HB * D)[head];
+        const float2 ml1 = reinterpret_cast<const float2*>(p1 + HB * D)[head];
+        float v0[8], v1[8];
 #pragma unroll
         for (int x = 0; x < 8; ++x)
-            if (lane + 32 * x < D) acc[x] = acc[x] * f0 + part[head * D + lane + 32 * x] * f1;
+            if (lane + 32 * x < D) v0[x] = p0[head * D + lane + 32 * x], v1[x] = p1[head * D + lane + 32 * x];
+        const float mn = two ? fmaxf(fmaxf(m, ml0.x), ml1.x) : fmaxf(m, ml0.x);
+        const float f = exp2f(m - safe_max(mn)), f0 = exp2f(ml0.x - safe_max(mn));
+        const float f1 = exp2f(ml1.x - safe_max(mn));
+        m = mn;
+        l = l * f + ml0.y * f0;
+        if (two) l += ml1.y * f1;
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+            if (lane + 32 * x < D) {
+                acc[x] = acc[x] * f + v0[x] * f0;
+                if (two) acc[x] += v1[x] * f1;
+            }
     }
 #pragma unroll
     for (int x = 0; x < 8; ++x)
@@ -621,19 +665,19 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedAttn a, i
     if (lane == 0) sml[warp] = make_float2(m, l);
     __syncthreads();
     m = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, sml[w].x);
+    for (int w = 0; w < warps; ++w) m = fmaxf(m, sml[w].x);
     l = 0.f;
     float f[kJoinWarps];
 #pragma unroll
     for (int w = 0; w < kJoinWarps; ++w) {
-        f[w] = exp2f(sml[w].x - safe_max(m));
-        l += f[w] * sml[w].y;
+        f[w] = w < warps ? exp2f(sml[w].x - safe_max(m)) : 0.f;
+        if (w < warps) l += f[w] * sml[w].y;
     }
-    for (int d = threadIdx.x; d < D; d += kJoinThreads) {
+    for (int d = threadIdx.x; d < D; d += threads) {
         float s = 0.f;
 #pragma unroll
-        for (int w = 0; w < kJoinWarps; ++w) s += f[w] * so[w][d];
+        for (int w = 0; w < kJoinWarps; ++w)
+            if (w < warps) s += f[w] * so[w][d];
         o[d] = T(s / l);
     }
     if (threadIdx.x == 0 && lse) *lse = (m + log2f(l)) * kLn2;
@@ -650,12 +694,10 @@ cudaError_t launch(cudaStream_t st, int sm_count, const PagedAttn& a) {
     }
     int workers = sm_count * resident;
     if (workers > kMaxWorkers) workers = kMaxWorkers;
-    KERNEL<<<workers, kThreads, 0, st>>>(a);
-    note_launch();
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    paged_join_kernel<T, HB><<<(unsigned)(a.cache.num_seqs * a.Hq), kJoinThreads, 0, st>>>(a, workers);
-    note_launch();
-    return cudaGetLastError();
+    if ((e = launch_overlapped(st, KERNEL, dim3((unsigned)workers), kThreads, 0, 0, a)) != cudaSuccess) return e;
+    // Many rows: smaller CTAs, so that they fit at once.
+    const int rows = a.cache.num_seqs * a.Hq, threads = rows > 8 * sm_count ? 16 * kJoinWarps : 32 * kJoinWarps;
+    return launch_overlapped(st, paged_join_kernel<T, HB>, dim3((unsigned)rows), threads, 0, 0, a, workers);
 }
 
 // Query heads that one worker takes at once: a multiple of the mma's 8 columns in bf16
@@ -667,11 +709,17 @@ int heads_at_once(hx_dtype dt, int G, int D) {
 
 }  // namespace
 
-uint64_t paged_attn_workspace_bytes(hx_dtype dt, int Hq, int Hkv, int D) {
-    return (uint64_t)2 * kMaxWorkers * heads_at_once(dt, Hq / Hkv, D) * (D + 2) * sizeof(float);
+// The plan, then the workers' parts.
+static uint64_t plan_bytes(int num_seqs) { return (sizeof(Plan) + (uint64_t)num_seqs * sizeof(int64_t) + 255) / 256 * 256; }
+
+uint64_t paged_attn_workspace_bytes(hx_dtype dt, int Hq, int Hkv, int D, int num_seqs) {
+    return plan_bytes(num_seqs) + (uint64_t)2 * kMaxWorkers * heads_at_once(dt, Hq / Hkv, D) * (D + 2) * sizeof(float);
 }
 
-cudaError_t paged_attn(cudaStream_t st, int sm_count, hx_dtype dt, const PagedAttn& a) {
+cudaError_t paged_attn(cudaStream_t st, int sm_count, hx_dtype dt, PagedAttn a, void* workspace) {
+    a.plan = (Plan*)workspace;
+    a.starts = (int64_t*)(a.plan + 1);
+    a.part = (float*)((char*)workspace + plan_bytes(a.cache.num_seqs));
     const int D = a.cache.D, hb = heads_at_once(dt, a.G, D);
     if (dt == HX_BF16) {
         if (hb == 16)
