@@ -113,6 +113,9 @@ _contexts: dict[int, CudaContext] = {}
 def context(device: Optional[int] = None) -> CudaContext:
     """The cached context of `device` (default: torch's current device)."""
     dev = torch.cuda.current_device() if device is None else int(device)
+    c = _contexts.get(dev)
+    if c is not None:
+        return c
     with _ctx_lock:
         c = _contexts.get(dev)
         if c is None:

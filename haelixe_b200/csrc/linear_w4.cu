@@ -117,6 +117,12 @@ struct X8<float> {
     }
 };
 
+// 4 bytes, or 4 zero bytes.
+__device__ __forceinline__ void copy4_async(void* smem, const void* global, bool valid) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(smem)),
+                 "l"(global), "r"(valid ? 4 : 0)
+                 : "memory");
+}
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait;" ::: "memory"); }
 
@@ -158,7 +164,8 @@ __device__ __forceinline__ int column_of(int g) { return 4 * ((g >> 1) | ((g & 1
 // lie in one group of scales, so that their products are scaled once. grid: (column
 // tiles x cluster, passes of 8 NT rows).
 // VEC: the rows of x and of packed are multiples of 16 bytes and x, packed and scales are
-// aligned, as TMA needs. Otherwise wn is 1 and each warp fills its stage with plain loads.
+// aligned, as TMA needs. Otherwise wn is 1 and each warp fills its stages with 4-byte asynchronous
+// copies of its own (bf16 x of an odd width with plain loads).
 template <typename T, int NT, int CH, int L, bool VEC>
 __global__ void __launch_bounds__(kThreads, sizeof(T) * NT * CH <= 8 ? 2 : 1) linear_w4_kernel(const __grid_constant__ Args a) {
     constexpr int R = 8 * NT, PARTS = X8<T>::PARTS, kBoxK = 128 / sizeof(T);  // k of a box of x
@@ -215,23 +222,43 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * NT * CH <= 8 ? 2 : 1) li
                                          kUnitK * u + c * kBoxK, r0);
             }
         } else {
-            for (int k = 0; k < kUnitRows; ++k)
+#pragma unroll 4
+            for (int k = 0; k < kUnitRows; ++k) {
+                const int o = kUnitRows * u + k;
+                const uint32_t* from = a.packed + (int64_t)min(o, octets - 1) * a.out;
 #pragma unroll
                 for (int c = 0; c < CH; ++c) {
-                    const int n = n0 + 32 * c + lane, o = kUnitRows * u + k;
-                    reinterpret_cast<uint32_t*>(st + c * kBox + k * 128)[lane ^ (4 * (k & 7))] =
-                        n < a.out && o < octets ? a.packed[(int64_t)o * a.out + n] : 0u;
+                    const int n = n0 + 32 * c + lane;
+                    copy4_async(st + c * kBox + k * 128 + 4 * (lane ^ (4 * (k & 7))), from + min(n, a.out - 1),
+                                n < a.out && o < octets);
                 }
-            for (int r = 0; r < R; ++r)
+            }
+            // x: pairs of bf16 where the rows allow it, else single elements
+            constexpr int kPer = 4 / sizeof(T);
+            const bool words = sizeof(T) == 4 || (a.in % 2 == 0 && ((uintptr_t)a.x & 3) == 0);
+            for (int r = 0; r < rows; ++r) {
+                const T* from = (const T*)a.x + (int64_t)(r0 + r) * a.in;
+                auto place = [&](int k) {  // of element k of the unit, which its pair follows
+                    return st + lay.w_bytes + (k / kBoxK) * R * 128 + r * 128 +
+                           16 * ((k % kBoxK) * (int)sizeof(T) / 16 ^ (r & 7)) + (k * (int)sizeof(T)) % 16;
+                };
+                if (words) {
 #pragma unroll
-                for (int k = lane; k < kUnitK; k += 32) {
-                    const int chunk = (k % kBoxK) * (int)sizeof(T) / 16 ^ (r & 7), at = kUnitK * u + k;
-                    reinterpret_cast<T*>(st + lay.w_bytes + (k / kBoxK) * R * 128 + r * 128 + chunk * 16)[k % (16 / sizeof(T))] =
-                        r < rows && at < a.in ? ((const T*)a.x)[(int64_t)(r0 + r) * a.in + at] : T(0.f);
+                    for (int k = kPer * lane; k < kUnitK; k += 32 * kPer) {
+                        const int at = kUnitK * u + k;
+                        copy4_async(place(k), from + (at < a.in ? at : 0), at < a.in);
+                    }
+                } else {
+#pragma unroll
+                    for (int k = lane; k < kUnitK; k += 32) {
+                        const int at = kUnitK * u + k;
+                        *reinterpret_cast<T*>(place(k)) = at < a.in ? from[at] : T(0.f);
+                    }
                 }
-            __syncwarp();
+            }
         }
     };
+    auto copies_commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
 
     int col[CH];
 #pragma unroll
@@ -266,19 +293,23 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * NT * CH <= 8 ? 2 : 1) li
 
     const Unpack weight;
     uint32_t issued = 0, done = 0;  // units of this group
-    if constexpr (VEC) {
-        for (int u = first; u < units && issued < kStages; u += stride) copy_unit(u, issued++);
+    for (int u = first; issued < kStages; u += stride) {
+        if (u < units) copy_unit(u, issued);
+        if (VEC && u >= units) break;
+        if constexpr (!VEC) copies_commit();
+        ++issued;
     }
     if (first < units) {
 #pragma unroll
         for (int l = 0; l < kUnit / L; ++l) load_scales(first, l);
     }
     for (int u = first; u < units; u += stride) {
-        const int i = VEC ? done % kStages : 0;
+        const int i = done % kStages;
         if constexpr (VEC) {
             if (!ptx::mbar_wait(full(i), done / kStages & 1, abort_flag, a.status, 50)) break;
         } else {
-            copy_unit(u, 0);
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+            __syncwarp();
         }
         ++done;
         const unsigned char* ws = stages + i * lay.stage + CH * sub * kBox + t * 128;
@@ -350,6 +381,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * NT * CH <= 8 ? 2 : 1) li
                 copy_unit(next, i);
                 ++issued;
             }
+        } else {
+            if (u + kStages * stride < units) copy_unit(u + kStages * stride, i);
+            copies_commit();
         }
     }
     if constexpr (VEC)  // after an expired wait alone: no copy outlives the stages

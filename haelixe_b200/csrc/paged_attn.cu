@@ -606,7 +606,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_f32_kernel(PagedAttn a) {
 // One CTA a query head of a sequence: the join of its item's parts, the zeros of an
 // empty sequence, or the NaN of one that is longer than its table row. It is launched with the
 // workers and waits for them here.
-constexpr int kJoinWarps = 8;  // at most
+constexpr int kJoinWarps = 16;  // at most
 template <typename T, int HB>
 __global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(PagedAttn a, int workers) {
     __shared__ float so[kJoinWarps][256];
@@ -635,28 +635,37 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(PagedAttn a
     float m = -INFINITY, l = 0.f, acc[8];
 #pragma unroll
     for (int x = 0; x < 8; ++x) acc[x] = 0.f;
-    // Warp w takes the parts w0 + w, w0 + w + warps, ..., two at once; lane l the elements l, l + 32, ...
-    auto part_of = [&](int w) { return a.part + (int64_t)(2 * w + (first > run * w)) * HB * (D + 2); };
-    for (int w = w0 + warp; w <= w1; w += 2 * warps) {
-        const bool two = w + warps <= w1;
-        const float *p0 = part_of(w), *p1 = two ? part_of(w + warps) : p0;
-        const float2 ml0 = reinterpret_cast<const float2*>(p0 + HB * D)[head];
-        const float2 ml1 = reinterpret_cast<const float2*>(p1 + HB * D)[head];
-        float v0[8], v1[8];
+    // Warp w takes the parts w0 + w, w0 + w + warps, ..., four at once; lane l the elements l, l + 32, ...
+    constexpr int kAtOnce = 4;
+    for (int w = w0 + warp; w <= w1; w += kAtOnce * warps) {
+        float2 ml[kAtOnce];
+        float v[kAtOnce][8];
 #pragma unroll
-        for (int x = 0; x < 8; ++x)
-            if (lane + 32 * x < D) v0[x] = p0[head * D + lane + 32 * x], v1[x] = p1[head * D + lane + 32 * x];
-        const float mn = two ? fmaxf(fmaxf(m, ml0.x), ml1.x) : fmaxf(m, ml0.x);
-        const float f = exp2f(m - safe_max(mn)), f0 = exp2f(ml0.x - safe_max(mn));
-        const float f1 = exp2f(ml1.x - safe_max(mn));
+        for (int k = 0; k < kAtOnce; ++k) {
+            const int wk = w + k * warps;
+            ml[k] = make_float2(-INFINITY, 0.f);
+            if (wk <= w1) {
+                const float* part = a.part + (int64_t)(2 * wk + (first > run * wk)) * HB * (D + 2);
+                ml[k] = reinterpret_cast<const float2*>(part + HB * D)[head];
+#pragma unroll
+                for (int x = 0; x < 8; ++x) v[k][x] = lane + 32 * x < D ? part[head * D + lane + 32 * x] : 0.f;
+            }
+        }
+        float mn = m;
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) mn = fmaxf(mn, ml[k].x);
+        const float f = exp2f(m - safe_max(mn));
         m = mn;
-        l = l * f + ml0.y * f0;
-        if (two) l += ml1.y * f1;
+        l *= f;
 #pragma unroll
-        for (int x = 0; x < 8; ++x)
-            if (lane + 32 * x < D) {
-                acc[x] = acc[x] * f + v0[x] * f0;
-                if (two) acc[x] += v1[x] * f1;
+        for (int x = 0; x < 8; ++x) acc[x] *= f;
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k)
+            if (w + k * warps <= w1) {
+                const float fk = exp2f(ml[k].x - safe_max(mn));
+                l += ml[k].y * fk;
+#pragma unroll
+                for (int x = 0; x < 8; ++x) acc[x] = fmaf(v[k][x], fk, acc[x]);
             }
     }
 #pragma unroll
@@ -695,8 +704,8 @@ cudaError_t launch(cudaStream_t st, int sm_count, const PagedAttn& a) {
     int workers = sm_count * resident;
     if (workers > kMaxWorkers) workers = kMaxWorkers;
     if ((e = launch_overlapped(st, KERNEL, dim3((unsigned)workers), kThreads, 0, 0, a)) != cudaSuccess) return e;
-    // Many rows: smaller CTAs, so that they fit at once.
-    const int rows = a.cache.num_seqs * a.Hq, threads = rows > 8 * sm_count ? 16 * kJoinWarps : 32 * kJoinWarps;
+    // Many rows: smaller CTAs, so that they fit at once. Few: as many warps as an item's parts may need.
+    const int rows = a.cache.num_seqs * a.Hq, threads = rows > 8 * sm_count ? 128 : rows > sm_count ? 256 : 512;
     return launch_overlapped(st, paged_join_kernel<T, HB>, dim3((unsigned)rows), threads, 0, 0, a, workers);
 }
 

@@ -46,7 +46,7 @@ def _context_of(t: torch.Tensor):
         raise RuntimeError("the attention block runs on CUDA tensors")
     if t.dtype not in _DTYPES:
         raise TypeError(f"unsupported dtype {t.dtype}; f32 and bf16 are supported")
-    return context(t.device.index)
+    return context(t.get_device())
 
 
 class _RMSNormFn(torch.autograd.Function):
@@ -196,21 +196,23 @@ class TokenLogprobs(NamedTuple):
 def _token_logprobs(logits, flat, top_k, with_stats):
     rows, classes = logits.shape
     stride = logits.stride(0) if rows > 1 else classes
-    dev = logits.device
-    logprob, entropy = (torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(2))
-    stats = torch.empty(rows, 3, dtype=torch.float32, device=dev) if with_stats else None
+    c = _context_of(logits)
+    logprob = logits.new_empty(rows, dtype=torch.float32)
+    entropy = torch.empty_like(logprob)
+    stats = logits.new_empty((rows, 3), dtype=torch.float32) if with_stats else None
     ids = top = None
     if top_k:
-        ids = torch.empty(rows, top_k, dtype=torch.int32, device=dev)
-        top = torch.empty(rows, top_k, dtype=torch.float32, device=dev)
-    c = _context_of(logits)
+        ids = logits.new_empty((rows, top_k), dtype=torch.int32)
+        top = logits.new_empty((rows, top_k), dtype=torch.float32)
     with c.lock:
         c.use_stream()
-        N.check(N.lib().hx_token_logprobs_fwd(c.handle, _DTYPES[logits.dtype], logits.data_ptr(), stride,
-                                              flat.data_ptr(), logprob.data_ptr(), entropy.data_ptr(),
-                                              stats.data_ptr() if with_stats else None, top_k,
-                                              ids.data_ptr() if top_k else None, top.data_ptr() if top_k else None,
-                                              rows, classes), c.handle)
+        st = N.lib().hx_token_logprobs_fwd(c.handle, _DTYPES[logits.dtype], logits.data_ptr(), stride, flat.data_ptr(),
+                                           logprob.data_ptr(), entropy.data_ptr(),
+                                           stats.data_ptr() if with_stats else None, top_k,
+                                           ids.data_ptr() if top_k else None, top.data_ptr() if top_k else None,
+                                           rows, classes)
+        if st:
+            N.check(st, c.handle)
     return logprob, entropy, ids, top, stats
 
 
@@ -275,10 +277,12 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0) 
         raise ValueError("logits must be [rows, classes] with contiguous rows")
     if logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]:
         logits = logits.contiguous()
-    flat = _ids(targets)
+    flat = targets
+    if targets.dtype is not torch.int32 or targets.dim() != 1 or not targets.is_contiguous():
+        flat = _ids(targets)
     if flat.numel() != logits.shape[0]:
         raise ValueError("targets length must match the number of logit rows")
-    if flat.device != logits.device:
+    if flat.get_device() != logits.get_device():
         raise ValueError("targets must be on the logits' device")
     top_k = int(top_k)
     if not 0 <= top_k <= min(32, logits.shape[1]):
@@ -314,39 +318,47 @@ def linear_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, group
     """`linear` with 4-bit weights (quantize_w4's layout), for the few rows of a decode
     step: x [..., in] -> [..., out], x, scales, bias and residual of one dtype.
     For inference: it has no backward and refuses tensors that would need one."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, scales, bias, residual)):
+    if torch.is_grad_enabled() and (x.requires_grad or scales.requires_grad or (bias is not None and bias.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
         raise RuntimeError("linear_w4 has no backward: call it under torch.no_grad()")
     c = _context_of(x)
-    in_f, out_f = x.shape[-1], packed.shape[-1]
+    lead, in_f, out_f = x.shape[:-1], x.shape[-1], packed.shape[-1]
     if group <= 0 or group % 32:
         raise ValueError("group must be a multiple of 32")
-    if packed.dtype != torch.int32 or packed.shape != (-(-in_f // 8), out_f) or not packed.is_contiguous():
+    if packed.dtype is not torch.int32 or packed.shape != (-(-in_f // 8), out_f) or not packed.is_contiguous():
         raise ValueError(f"packed must be contiguous int32 [{-(-in_f // 8)}, out] for {in_f} inputs")
     if scales.shape != (-(-in_f // group), out_f) or not scales.is_contiguous():
         raise ValueError(f"scales must be contiguous [{-(-in_f // group)}, {out_f}]")
-    shape = (*x.shape[:-1], out_f)
-    if bias is not None and (bias.shape != (out_f,) or not bias.is_contiguous()):
-        raise ValueError(f"bias must be a contiguous vector of {out_f}")
-    if residual is not None and residual.shape != shape:
-        raise ValueError(f"residual must be {shape}")
-    for t in (scales, bias, residual):
-        if t is not None and t.dtype != x.dtype:
-            raise ValueError("x, scales, bias and residual must share a dtype")
-    for t in (packed, scales, bias, residual):
-        if t is not None and t.device != x.device:
-            raise ValueError("all operands must be on x's device")
-    x = x.contiguous()
+    dt, dev = x.dtype, x.get_device()
+    shape = (*lead, out_f)
+    if bias is not None:
+        if bias.shape != (out_f,) or not bias.is_contiguous():
+            raise ValueError(f"bias must be a contiguous vector of {out_f}")
+        if bias.dtype is not dt or bias.get_device() != dev:
+            raise ValueError("bias must have x's dtype and device")
     if residual is not None:
+        if residual.shape != shape:
+            raise ValueError(f"residual must be {shape}")
+        if residual.dtype is not dt or residual.get_device() != dev:
+            raise ValueError("residual must have x's dtype and device")
         residual = residual.contiguous()
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    if y.numel() == 0:
+    if scales.dtype is not dt or scales.get_device() != dev or packed.get_device() != dev:
+        raise ValueError("packed and scales must be on x's device, scales in its dtype")
+    x = x.contiguous()
+    y = x.new_empty(shape)
+    rows = 1
+    for n in lead:
+        rows *= n
+    if rows == 0 or out_f == 0:
         return y
     with c.lock:
         c.use_stream()
-        N.check(N.lib().hx_linear_w4_fwd(c.handle, _DTYPES[x.dtype], x.data_ptr(), packed.data_ptr(), scales.data_ptr(),
-                                         None if bias is None else bias.data_ptr(),
-                                         None if residual is None else residual.data_ptr(), y.data_ptr(),
-                                         x.numel() // in_f, in_f, out_f, group), c.handle)
+        st = N.lib().hx_linear_w4_fwd(c.handle, _DTYPES[dt], x.data_ptr(), packed.data_ptr(), scales.data_ptr(),
+                                      None if bias is None else bias.data_ptr(),
+                                      None if residual is None else residual.data_ptr(), y.data_ptr(), rows, in_f, out_f,
+                                      group)
+        if st:
+            N.check(st, c.handle)
     return y
 
 

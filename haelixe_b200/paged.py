@@ -23,11 +23,6 @@ from . import _native as N
 from .attention import _DTYPES, context
 
 
-def _no_grad_needed(who: str, *ts: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        raise RuntimeError(f"{who} has no backward: call it under torch.no_grad()")
-
-
 class PagedKVCache:
     """Keys and values of many sequences in pages, and the table that maps them.
 
@@ -66,6 +61,8 @@ class PagedKVCache:
                                block_table.stride(0) if seqs > 1 else columns, pages, slots, heads, dim, seqs, columns)
         self._ref = ctypes.byref(self._c)
         self._dt = _DTYPES[k.dtype]
+        self._dev = k.get_device()
+        self._ctx = context(self._dev)
         self._workspace: dict[int, int] = {}  # bytes by query heads
         self.dtype, self.device = k.dtype, k.device
         self.num_seqs, self.heads, self.head_dim = seqs, heads, dim
@@ -103,28 +100,40 @@ class PagedKVCache:
         return n
 
 
-def _rows(cache: PagedKVCache, who: str, name: str, t: torch.Tensor, rows: int, heads: Optional[int]) -> N.Rows:
-    if t.dim() != 3 or t.shape[0] != rows or t.shape[2] != cache.head_dim or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{who}: {name} must be [{rows}, {heads or 'heads'}, {cache.head_dim}], got {tuple(t.shape)}")
-    if t.dtype != cache.dtype or t.device != cache.device:
+# The calls are made once a layer and token, so their checks are kept to a few
+# attribute reads. Operands go to the library as hx_rows (address, stride of a row,
+# stride of a head), side by side in one array.
+_Rows2, _Rows4 = ctypes.c_int64 * 6, ctypes.c_int64 * 12
+_ROWS = ctypes.sizeof(N.Rows)
+
+
+def _rows(cache: PagedKVCache, who: str, name: str, t: torch.Tensor, rows: int, heads: int):
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != rows or shape[1] != heads or shape[2] != cache.head_dim:
+        raise ValueError(f"{who}: {name} must be [{rows}, {heads}, {cache.head_dim}], got {tuple(shape)}")
+    if t.dtype is not cache.dtype or t.get_device() != cache._dev:
         raise ValueError(f"{who}: {name} must have the cache's dtype and device")
     s0, s1, s2 = t.stride()
     if s2 != 1:
         raise ValueError(f"{who}: the head dimension of {name} must be contiguous")
     # The stride of a dimension of size 1 never moves an address.
-    if t.shape[1] == 1:
+    if heads == 1:
         s1 = cache.head_dim
     if rows == 1:
-        s0 = t.shape[1] * s1
-    return N.Rows(t.data_ptr(), s0, s1)
+        s0 = heads * s1
+    return t.data_ptr(), s0, s1
 
 
-def _indices(cache: PagedKVCache, who: str, name: str, t: torch.Tensor, n: int):
-    if t.dtype != torch.int32:
+def _indices(cache: PagedKVCache, who: str, name: str, t: torch.Tensor, n: int) -> int:
+    if t.dtype is not torch.int32:
         raise TypeError(f"{who}: {name} must be int32")
-    if t.dim() != 1 or t.shape[0] != n or t.device != cache.device or not t.is_contiguous():
+    if t.dim() != 1 or t.shape[0] != n or t.get_device() != cache._dev or not t.is_contiguous():
         raise ValueError(f"{who}: {name} must be a contiguous vector of {n} on the cache's device")
     return t.data_ptr()
+
+
+def _no_backward(who: str) -> None:
+    raise RuntimeError(f"{who} has no backward: call it under torch.no_grad()")
 
 
 def paged_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, seq_ids: torch.Tensor,
@@ -141,30 +150,37 @@ def paged_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, seq_ids:
     nothing to the cache and NaN to its row of out_q.
     """
     who = "paged_append"
-    _no_grad_needed(who, k, v, q)
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad)):
+        _no_backward(who)
     n = k.shape[0]
     kr, vr = _rows(cache, who, "k", k, n, cache.heads), _rows(cache, who, "v", v, n, cache.heads)
     ids, pos = _indices(cache, who, "seq_ids", seq_ids, n), _indices(cache, who, "positions", positions, n)
-    heads, qr, orr = 0, None, None
-    if q is not None:
-        qr = _rows(cache, who, "q", q, n, None)
-        heads = q.shape[1]
-        if out_q is None:
-            out_q = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        orr = _rows(cache, who, "out_q", out_q, n, heads)
-        qr, orr = ctypes.byref(qr), ctypes.byref(orr)
-    elif out_q is not None:
-        raise ValueError("paged_append: out_q without q")
     base = 0.0
     if rope_base is not None:
         base = float(rope_base)
         if not base > 0.0:
             raise ValueError("paged_append: rope_base must be positive")
-    ctx = context(cache.device.index)
+    if q is not None:
+        heads = q.shape[1] if q.dim() == 3 else 0
+        qr = _rows(cache, who, "q", q, n, heads)
+        if out_q is None:
+            out_q = torch.empty_like(q)
+        rows = _Rows4(*kr, *vr, *qr, *_rows(cache, who, "out_q", out_q, n, heads))
+        at = ctypes.addressof(rows)
+        q_at, out_at = at + 2 * _ROWS, at + 3 * _ROWS
+    else:
+        if out_q is not None:
+            raise ValueError("paged_append: out_q without q")
+        rows = _Rows2(*kr, *vr)
+        at = ctypes.addressof(rows)
+        heads, q_at, out_at = 0, None, None
+    ctx = cache._ctx
     with ctx.lock:
         ctx.use_stream()
-        N.check(N.lib().hx_paged_append(ctx.handle, cache._dt, cache._ref, n, ctypes.byref(kr), ctypes.byref(vr), ids,
-                                        pos, heads, qr, orr, base), ctx.handle)
+        st = N.lib().hx_paged_append(ctx.handle, cache._dt, cache._ref, n, at, at + _ROWS, ids, pos, heads, q_at, out_at,
+                                     base)
+        if st:
+            N.check(st, ctx.handle)
     return out_q
 
 
@@ -179,24 +195,27 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, seq_lens: torch.Tensor
     the cache holds at or past seq_lens is not read.
     """
     who = "paged_attention"
-    _no_grad_needed(who, q)
-    qr = _rows(cache, who, "q", q, cache.num_seqs, None)
-    heads = q.shape[1]
-    lens = _indices(cache, who, "seq_lens", seq_lens, cache.num_seqs)
+    if q.requires_grad and torch.is_grad_enabled():
+        _no_backward(who)
+    n, heads = cache.num_seqs, q.shape[1] if q.dim() == 3 else 0
+    qr = _rows(cache, who, "q", q, n, heads)
+    lens = _indices(cache, who, "seq_lens", seq_lens, n)
     need = cache.workspace_bytes(heads)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    orr = _rows(cache, who, "out", out, cache.num_seqs, heads)
+        out = torch.empty_like(q)
+    rows = _Rows2(*qr, *_rows(cache, who, "out", out, n, heads))
     if lse is None:
-        lse = torch.empty(q.shape[0], heads, dtype=torch.float32, device=q.device)
-    elif lse.shape != q.shape[:2] or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
+        lse = q.new_empty((n, heads), dtype=torch.float32)
+    elif lse.shape != (n, heads) or lse.dtype is not torch.float32 or lse.get_device() != cache._dev or not lse.is_contiguous():
         raise ValueError("paged_attention: lse must be a contiguous f32 [sequences, query heads]")
     # A tensor of the current stream, so that calls on other streams and captured graphs have their own.
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-    ctx = context(cache.device.index)
+    ws = q.new_empty(need, dtype=torch.uint8)
+    at = ctypes.addressof(rows)
+    ctx = cache._ctx
     with ctx.lock:
         ctx.use_stream()
-        N.check(N.lib().hx_paged_attention(ctx.handle, cache._dt, cache._ref, heads, ctypes.byref(qr),
-                                           ctypes.byref(orr), lse.data_ptr(), lens, float(scale), ws.data_ptr(), need),
-                ctx.handle)
+        st = N.lib().hx_paged_attention(ctx.handle, cache._dt, cache._ref, heads, at, at + _ROWS, lse.data_ptr(), lens,
+                                        scale, ws.data_ptr(), need)
+        if st:
+            N.check(st, ctx.handle)
     return out, lse
