@@ -5,7 +5,9 @@ kernels/rms_norm.rs), `Linear` (src/nn/linear.rs), `MultiHeadAttention`
 (src/nn/attention.rs:46-98), `FeedForward` (src/nn/mlp.rs) and
 `TransformerBlock` (src/nn/transformer.rs), plus the pieces a language-model
 training step over a block stack needs: a token `Embedding` (the reference
-has none), `cross_entropy` (src/tensor.rs:754-801) and `BlockStack`. Every op
+has none), `cross_entropy` (src/tensor.rs:754-801) and `BlockStack`, and those
+that it answers with: `prefill` and `decode` over paged key/value caches,
+`token_logprobs`, and Linear weights in 4 bits (`LinearW4`). Every op
 runs on the GPU through the library's C ABI: RMSNorm and GELU kernels, Linear
 as cuBLAS GEMMs (weights stored [in, out] as in linear.rs:41) with the bias
 and the block's residual add folded into the GEMM's C operand, and the fused
@@ -24,6 +26,7 @@ import torch
 
 from . import _native as N
 from .attention import _DTYPES, context, flash_attention
+from .paged import PagedKVCache, paged_append, paged_attention
 
 
 def _p(t: Optional[torch.Tensor]):
@@ -410,6 +413,23 @@ class Linear:
         return [self.weight, self.bias]
 
 
+class LinearW4:
+    """A Linear for inference with its weight in 4 bits (quantize_w4); bias as it was."""
+
+    def __init__(self, linear: Linear, group: int = 128):
+        self.group = int(group)
+        self.packed, self.scales = quantize_w4(linear.weight, self.group)
+        self.bias = linear.bias.detach()
+
+    def forward(self, x, residual=None):
+        return linear_w4(x, self.packed, self.scales, self.group, self.bias, residual)
+
+    __call__ = forward
+
+    def parameters(self):
+        return []
+
+
 class MultiHeadAttention:
     """src/nn/attention.rs:5-98: pre-RMSNorm, Q/K/V projections, heads as strided
     views, RoPE (base 10000, attention.rs:76) on Q and K, the fused attention
@@ -441,6 +461,30 @@ class MultiHeadAttention:
         return self.out_proj(o.transpose(1, 2).reshape(B, S, Hd), residual)
 
     __call__ = forward
+
+    def prefill(self, x: torch.Tensor, cache: PagedKVCache, seq_ids: torch.Tensor, positions: torch.Tensor,
+                residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """forward of prompts [B, S, hidden] from position 0 whose rotated keys and values also enter
+        the cache: token (b, s) at positions[b * S + s] of seq_ids[b * S + s], padding negative."""
+        B, S, Hd = x.shape
+        H, D = self.num_heads, self.head_dim
+        n = self.norm(x)
+        q, k, v = (p(n).view(B, S, H, D) for p in (self.q_proj, self.k_proj, self.v_proj))
+        paged_append(cache, k.view(-1, H, D), v.view(-1, H, D), seq_ids, positions, rope_base=self.rope_base)
+        o = flash_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), 1.0 / math.sqrt(D), True,
+                            rope_base=self.rope_base)
+        return self.out_proj(o.transpose(1, 2).reshape(B, S, Hd), residual)
+
+    def decode(self, x: torch.Tensor, cache: PagedKVCache, seq_ids: torch.Tensor, positions: torch.Tensor,
+               seq_lens: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """forward of one new token a sequence [sequences, hidden]: its keys and values enter the cache
+        and it attends to the seq_lens positions that are there then."""
+        T, H, D = x.shape[0], self.num_heads, self.head_dim
+        n = self.norm(x)
+        q, k, v = (p(n).view(T, H, D) for p in (self.q_proj, self.k_proj, self.v_proj))
+        paged_append(cache, k, v, seq_ids, positions, rope_base=self.rope_base, q=q, out_q=q)
+        o, _ = paged_attention(cache, q, seq_lens, 1.0 / math.sqrt(D))
+        return self.out_proj(o.view(T, H * D), residual)
 
     def parameters(self):
         return (self.norm.parameters() + self.q_proj.parameters() + self.k_proj.parameters()
@@ -483,6 +527,14 @@ class TransformerBlock:
         return self.mlp(self.norm2(x), residual=x)
 
     __call__ = forward
+
+    def prefill(self, x, cache, seq_ids, positions):
+        x = self.mha.prefill(self.norm1(x), cache, seq_ids, positions, residual=x)
+        return self.mlp(self.norm2(x), residual=x)
+
+    def decode(self, x, cache, seq_ids, positions, seq_lens):
+        x = self.mha.decode(self.norm1(x), cache, seq_ids, positions, seq_lens, residual=x)
+        return self.mlp(self.norm2(x), residual=x)
 
     def parameters(self):
         return (self.norm1.parameters() + self.mha.parameters() + self.norm2.parameters()
@@ -533,12 +585,66 @@ class BlockStack:
         x = self.embed(ids)
         for blk in self.blocks:
             x = blk(x)
-        return self.head(self.norm(x)).reshape(-1, self.head.weight.shape[1])
+        y = self.head(self.norm(x))
+        return y.reshape(-1, y.shape[-1])
 
     __call__ = forward
 
     def loss(self, ids: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
         return cross_entropy(self(ids), targets)
+
+    def caches(self, pages: int, slots: int, block_table: torch.Tensor) -> list:
+        """One PagedKVCache a block, all on one table."""
+        mha = self.blocks[0].mha
+        return [PagedKVCache.allocate(pages, slots, mha.num_heads, mha.head_dim, block_table, self.embed.weight.dtype)
+                for _ in self.blocks]
+
+    def _answers(self, caches) -> None:
+        if not all(b.mha.causal for b in self.blocks):
+            raise ValueError("answering from a cache needs causal blocks")
+        if len(caches) != len(self.blocks):
+            raise ValueError("one cache a block")
+
+    @torch.no_grad()
+    def prefill(self, ids: torch.Tensor, caches: list, lens: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Prompts [B, S] (row b is sequence b of the caches; its first lens[b] ids count, all without
+        lens) into the caches. Returns the logits [B, vocab] after each prompt's last token."""
+        self._answers(caches)
+        B, S = ids.shape
+        positions = torch.arange(S, dtype=torch.int32, device=ids.device).repeat(B)
+        seq_ids = torch.arange(B, dtype=torch.int32, device=ids.device).repeat_interleave(S)
+        last = torch.full((B,), S - 1, device=ids.device)
+        if lens is not None:
+            last = lens.to(torch.int64) - 1
+            seq_ids = torch.where(positions < lens.repeat_interleave(S), seq_ids, -1)
+        x = self.embed(ids)
+        for blk, cache in zip(self.blocks, caches):
+            x = blk.prefill(x, cache, seq_ids, positions)
+        x = x[torch.arange(B, device=ids.device), last]
+        return self.head(self.norm(x))
+
+    @torch.no_grad()
+    def decode(self, ids: torch.Tensor, caches: list, positions: torch.Tensor) -> torch.Tensor:
+        """One new token a sequence: ids [B], at positions [B] (int32; what the caches hold before them
+        is what each attends to, itself included). A negative position leaves its sequence out.
+        Returns the logits [B, vocab] (of a sequence that is left out: of no use)."""
+        self._answers(caches)
+        every = torch.arange(ids.shape[0], dtype=torch.int32, device=ids.device)
+        seq_ids = torch.where(positions < 0, -1, every)
+        seq_lens = positions.clamp(min=-1) + 1
+        x = self.embed(ids)
+        for blk, cache in zip(self.blocks, caches):
+            x = blk.decode(x, cache, seq_ids, positions, seq_lens)
+        return self.head(self.norm(x))
+
+    def quantize_w4(self, group: int = 128) -> "BlockStack":
+        """Puts every Linear's weight in 4 bits, for inference; the stack can then no longer be trained."""
+        for blk in self.blocks:
+            for part, names in ((blk.mha, ("q_proj", "k_proj", "v_proj", "out_proj")), (blk.mlp, ("linear1", "linear2"))):
+                for name in names:
+                    setattr(part, name, LinearW4(getattr(part, name), group))
+        self.head = LinearW4(self.head, group)
+        return self
 
     def parameters(self):
         ps = self.embed.parameters()

@@ -1,0 +1,151 @@
+"""A BlockStack answering token by token from paged caches: prefill, decode steps,
+log probabilities of the picked tokens, with plain and with 4-bit weights,
+against the whole forward pass over the same tokens.
+
+f32: max-abs 1e-3, as the layer tests; bf16: 2 % relative L2 error, since every
+intermediate is rounded to bf16 in both, at different places.
+"""
+import pytest
+import torch
+
+import haelixe_b200 as hx
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+VOCAB, HIDDEN, HEADS, LAYERS = 211, 128, 2, 2
+
+
+def _stack(dtype, causal=True):
+    return hx.nn.BlockStack(VOCAB, HIDDEN, HEADS, LAYERS, device="cuda", dtype=dtype, causal=causal, init_std=0.05, seed=3)
+
+
+def _near(got, want, dtype):
+    got, want = got.float(), want.float()
+    assert torch.isfinite(got).all()
+    if dtype == F32:
+        assert (got - want).abs().max() < 1e-3
+    else:
+        assert (got - want).norm() < 0.02 * want.norm()
+
+
+def _generate(stack, prompts, lens, steps, slots):
+    """Greedy tokens, their log probabilities and the logits of every step."""
+    B = prompts.shape[0]
+    columns = -(-(int(lens.max()) + steps) // slots)
+    table = torch.randperm(B * columns, device="cuda").to(torch.int32).view(B, columns)
+    caches = stack.caches(B * columns, slots, table)
+    logits = stack.prefill(prompts, caches, lens)
+    positions, tokens, logprobs, all_logits = lens.clone(), [], [], []
+    for _ in range(steps):
+        all_logits.append(logits)
+        best = hx.nn.token_logprobs(logits, torch.zeros(B, dtype=torch.int32, device="cuda"), 1).top_ids[:, 0]
+        logprobs.append(hx.nn.token_logprobs(logits, best).logprob)
+        tokens.append(best)
+        logits = stack.decode(best, caches, positions)
+        positions += 1
+    return torch.stack(tokens, 1), torch.stack(logprobs, 1), torch.stack(all_logits, 1)
+
+
+def _check_against_whole_passes(stack, prompts, lens, out, dtype):
+    tokens, logprobs, logits = out
+    for b in range(prompts.shape[0]):
+        n, steps = int(lens[b]), tokens.shape[1]
+        ids = torch.cat([prompts[b, :n].long(), tokens[b].long()])[None]
+        with torch.no_grad():
+            want = stack(ids)[n - 1:n - 1 + steps]
+        _near(logits[b], want, dtype)
+        lp = torch.log_softmax(logits[b].double(), -1).gather(1, tokens[b].long()[:, None])[:, 0]
+        assert (logprobs[b].double() - lp).abs().max() < 1e-5
+        assert torch.equal(tokens[b].long(), logits[b].float().argmax(-1))
+
+
+@pytest.mark.parametrize("dtype", [pytest.param(F32, id="f32"), pytest.param(BF16, id="bf16")])
+@pytest.mark.parametrize("slots", [16, 5])
+def test_generation_agrees_with_whole_passes(dtype, slots):
+    stack = _stack(dtype)
+    prompts = torch.randint(VOCAB, (3, 40), generator=torch.Generator().manual_seed(1)).cuda()
+    lens = torch.tensor([40, 1, 23], dtype=torch.int32, device="cuda")
+    with torch.no_grad():
+        out = _generate(stack, prompts, lens, 6, slots)
+    _check_against_whole_passes(stack, prompts, lens, out, dtype)
+
+
+@pytest.mark.parametrize("dtype", [pytest.param(F32, id="f32"), pytest.param(BF16, id="bf16")])
+def test_generation_with_4_bit_weights(dtype):
+    """Against the same stack with the weights that the 4 bits stand for."""
+    stack, plain = _stack(dtype), _stack(dtype)
+    for blk in plain.blocks:
+        for part in (blk.mha.q_proj, blk.mha.k_proj, blk.mha.v_proj, blk.mha.out_proj, blk.mlp.linear1, blk.mlp.linear2):
+            _through_4_bits(part)
+    _through_4_bits(plain.head)
+    stack.quantize_w4(32)
+    prompts = torch.randint(VOCAB, (2, 17), generator=torch.Generator().manual_seed(2)).cuda()
+    lens = torch.tensor([17, 9], dtype=torch.int32, device="cuda")
+    with torch.no_grad():
+        out = _generate(stack, prompts, lens, 4, 8)
+        _check_against_whole_passes(stack, prompts, lens, out, dtype)
+        _near(stack(prompts), plain(prompts), dtype)
+    assert sum(p.numel() for p in stack.blocks[0].mha.parameters()) == HIDDEN  # the norm's weight alone
+
+
+def _through_4_bits(linear):
+    packed, scales = hx.nn.quantize_w4(linear.weight, 32)
+    q = torch.stack([(packed >> (4 * i)) & 15 for i in range(8)], 1).flatten(0, 1)
+    w = (q - 8).float() * scales.float().repeat_interleave(32, 0)
+    linear.weight = w.to(linear.weight.dtype)  # bf16: (q - 8) * scale rounds once
+
+
+def test_a_sequence_left_out_keeps_its_cache():
+    stack = _stack(BF16)
+    prompts = torch.randint(VOCAB, (2, 12), generator=torch.Generator().manual_seed(4)).cuda()
+    table = torch.arange(4, dtype=torch.int32, device="cuda").view(2, 2)
+    caches = stack.caches(4, 16, table)
+    logits = stack.prefill(prompts, caches)
+    before = [(c.k[table[1].long()].clone(), c.v[table[1].long()].clone()) for c in caches]
+    ids = logits.float().argmax(-1)
+    stack.decode(ids, caches, torch.tensor([12, -1], dtype=torch.int32, device="cuda"))
+    for c, (k, v) in zip(caches, before):
+        assert torch.equal(c.k[table[1].long()], k) and torch.equal(c.v[table[1].long()], v)
+
+
+def test_decode_step_in_a_graph():
+    stack = _stack(BF16)
+    prompts = torch.randint(VOCAB, (2, 12), generator=torch.Generator().manual_seed(5)).cuda()
+    table = torch.arange(4, dtype=torch.int32, device="cuda").view(2, 2)
+    eager, graphed = stack.caches(4, 16, table), stack.caches(4, 16, table)
+    ids = stack.prefill(prompts, eager).float().argmax(-1)
+    stack.prefill(prompts, graphed)
+    at = torch.full((2,), 12, dtype=torch.int32, device="cuda")
+    step_ids, step_at = ids.clone(), at.clone()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        stack.decode(step_ids, graphed, step_at)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        logits = stack.decode(step_ids, graphed, step_at)
+    for _ in range(3):
+        want = stack.decode(ids, eager, at)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(logits, want)
+        ids = want.float().argmax(-1)
+        at += 1
+        step_ids.copy_(ids)
+        step_at += 1
+
+
+def test_refusals():
+    stack = _stack(BF16, causal=False)
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError):
+        stack.prefill(torch.zeros(1, 4, dtype=torch.int64, device="cuda"), stack.caches(1, 16, table))
+    stack = _stack(BF16)
+    with pytest.raises(ValueError):
+        stack.decode(torch.zeros(1, dtype=torch.int64, device="cuda"), stack.caches(1, 16, table)[:1],
+                     torch.zeros(1, dtype=torch.int32, device="cuda"))
+    with pytest.raises(RuntimeError):  # 4-bit weights have no backward
+        stack.quantize_w4(32).loss(torch.zeros(1, 4, dtype=torch.int64, device="cuda"),
+                                   torch.zeros(4, dtype=torch.int64, device="cuda"))
