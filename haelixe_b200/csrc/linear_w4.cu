@@ -46,6 +46,7 @@ struct Args {
     void* y;
     DeviceStatus* status;
     int rows, in, out, group, group_shift;  // group_shift: log2(group), -1 when not a power of two
+    bool vec_y;          // y on a boundary of 4 elements
     int wn_log, ks_log;  // log2 of the warps that share a unit, side by side, and of the cluster's size
 };
 
@@ -141,7 +142,7 @@ constexpr int kStages = 2;
 // (a warp's CH boxes after another's), then x as boxes of R rows of 128 bytes, each 128-byte
 // row with its 16-byte chunks exchanged by the row number (the TMA's swizzle). With
 // column_of a quarter warp's 16-byte reads of the words fall on all banks. The stages become the
-// groups' sums, [8 / wn][R][C + 1].
+// groups' sums, [8 / wn][R][C + 4].
 constexpr int kBox = kUnitRows * 128;
 struct Layout {
     int w_bytes, stage, recv, bars, total;  // bytes, then byte offsets
@@ -149,7 +150,7 @@ struct Layout {
         const int C = 32 * CH * wn, groups = kWarps / wn;
         w_bytes = CH * wn * kBox;
         stage = w_bytes + R * kUnitK * eb;
-        const int sums = groups * R * (C + 1) * 4;
+        const int sums = groups * R * (C + 4) * 4;
         recv = groups * kStages * stage;
         if (recv < sums) recv = (sums + 15) / 16 * 16;
         bars = recv + ((R * C + kThreads - 1) / kThreads + 7) * kThreads * 4;
@@ -390,28 +391,32 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * NT * CH <= 8 ? 2 : 1) li
         for (; done < issued; ++done) ptx::mbar_wait_drain(full(done % kStages), done / kStages & 1);
     __syncthreads();  // the stages are free: the groups' sums take their place
     float* sums = reinterpret_cast<float*>(smem);
+    const int pitch = C + 4;
     // acc[c][m][j][e]: column 32 c + column_of(g) + 2 m + e / 2 of the warp's, row 8 j + 2 t + e % 2
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    sums[(group * R + 8 * j + 2 * t + (e & 1)) * (C + 1) + 32 * (CH * sub + c) + column_of(g) + 2 * m + (e >> 1)] =
-                        acc[c][m][j][e];
+            for (int e = 0; e < 2; ++e)
+                *reinterpret_cast<float4*>(
+                    &sums[(group * R + 8 * j + 2 * t + e) * pitch + 32 * (CH * sub + c) + column_of(g)]) =
+                    make_float4(acc[c][0][j][e], acc[c][0][j][e + 2], acc[c][1][j][e], acc[c][1][j][e + 2]);
     if (ks > 1) cluster_wait();
     __syncthreads();
-    // Result r * C + n of the tile is in block (r * C + n) / 256, which CTA block % ks finishes:
-    // it receives its blocks from all CTAs of the cluster.
-    float* recv = reinterpret_cast<float*>(smem + lay.recv);
-    const int blocks = (((rows << c_log) + kThreads - 1) / kThreads + ks - 1) >> ks_log;
-    for (int at = threadIdx.x, block = 0; at < rows << c_log; at += kThreads, ++block) {
-        const int r = at >> c_log, n = at & (C - 1);
-        float v = 0.f;
-        for (int k = 0; k < groups; ++k) v += sums[(k * R + r) * (C + 1) + n];
-        float* to = &recv[(rank * blocks + (block >> ks_log)) * kThreads + threadIdx.x];
+    // Four results at a time: quad q of the tile, row by row, is in block q / 64, which CTA block % ks
+    // finishes: it receives its blocks from all CTAs of the cluster.
+    float4* recv = reinterpret_cast<float4*>(smem + lay.recv);
+    const int quads = (rows << c_log) / 4, mine = (((quads + 63) / 64 + ks - 1) >> ks_log) * 64;  // that a CTA finishes
+    for (int q = threadIdx.x; q < quads; q += kThreads) {
+        const int r = (4 * q) >> c_log, n = (4 * q) & (C - 1), block = q / 64;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int k = 0; k < groups; ++k) {
+            const float4 u = *reinterpret_cast<const float4*>(&sums[(k * R + r) * pitch + n]);
+            v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+        }
+        float4* to = &recv[rank * mine + (block >> ks_log) * 64 + q % 64];
         if (ks > 1)
             *cluster.map_shared_rank(to, block & (ks - 1)) = v;
         else
@@ -421,15 +426,26 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * NT * CH <= 8 ? 2 : 1) li
         cluster_arrive();
         cluster_wait();
     }
-    for (int k = 0; k < blocks; ++k) {
-        const int at = ((k << ks_log) + rank) * kThreads + threadIdx.x, r = at >> c_log, n = n0 + (at & (C - 1));
-        if (r >= rows || n >= a.out) continue;
-        float v = 0.f;
-        for (int i = 0; i < ks; ++i) v += recv[(i * blocks + k) * kThreads + threadIdx.x];
+    for (int i = threadIdx.x; i < mine; i += kThreads) {  // without a cluster: what this thread wrote
+        const int q = (((i / 64) << ks_log) + rank) * 64 + i % 64, r = (4 * q) >> c_log, n = n0 + ((4 * q) & (C - 1));
+        if (q >= quads || n >= a.out) continue;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int k = 0; k < ks; ++k) {
+            const float4 u = recv[k * mine + i];
+            v[0] += u.x, v[1] += u.y, v[2] += u.z, v[3] += u.w;
+        }
         const int64_t to = (int64_t)(r0 + r) * a.out + n;
-        if (a.bias) v += (float)((const T*)a.bias)[n];
-        if (a.residual) v += (float)((const T*)a.residual)[to];
-        ((T*)a.y)[to] = T(v);
+        S4<T> y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (!VEC && n + e >= a.out) break;
+            if (a.bias) v[e] += (float)((const T*)a.bias)[n + e];
+            if (a.residual) v[e] += (float)((const T*)a.residual)[to + e];
+            y.s[e] = T(v[e]);
+            if (!VEC || !a.vec_y) ((T*)a.y)[to + e] = y.s[e];
+        }
+        if (VEC && a.vec_y) *reinterpret_cast<S4<T>*>((T*)a.y + to) = y;
     }
 }
 
@@ -532,7 +548,8 @@ cudaError_t linear_w4(cudaStream_t st, int sm_count, DeviceStatus* status, hx_dt
                       const void* scales, const void* bias, const void* residual, void* y, int rows, int in, int out,
                       int group) {
     Args a{CUtensorMap{}, CUtensorMap{}, x, packed, scales, bias, residual, y, status, rows, in, out, group,
-                 (group & (group - 1)) == 0 ? __builtin_ctz((unsigned)group) : -1, 0, 0};
+                 (group & (group - 1)) == 0 ? __builtin_ctz((unsigned)group) : -1,
+           (uintptr_t)y % (dt == HX_F32 ? 16 : 8) == 0, 0, 0};
     const bool vec = (uintptr_t)x % 16 == 0 && (int64_t)in * (dt == HX_F32 ? 4 : 2) % 16 == 0 && (uintptr_t)packed % 16 == 0 && (uintptr_t)scales % 16 == 0 && out % 4 == 0;
     return dt == HX_F32 ? by_rows<float>(st, sm_count, a, vec) : by_rows<__nv_bfloat16>(st, sm_count, a, vec);
 }
