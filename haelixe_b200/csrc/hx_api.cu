@@ -821,6 +821,7 @@ int hx_paged_attention(hx_ctx* c, hx_dtype dt, const hx_paged_cache* cache, int 
     a.lens = seq_lens;
     a.Hq = Hq;
     a.G = Hq / cache->H;
+    a.o_vec = (uintptr_t)a.o % (4 * eb) == 0 && a.o_sn % 4 == 0 && a.o_sh % 4 == 0;
     a.scale_log2 = scale * 1.4426950408889634f;
     st = check_cuda(c, hx::paged_attn(c->stream, c->sm_count, dt, a, ws), who);
     if (workspace == nullptr) hx_free(c, ws);  // stream-ordered: the next user of the slab queues behind us

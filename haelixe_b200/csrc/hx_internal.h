@@ -166,6 +166,7 @@ struct PagedAttn {
     const int32_t* lens;
     int64_t q_sn, q_sh, o_sn, o_sh;
     int Hq, G;  // query heads, query heads of one key head
+    bool o_vec;  // rows of o on boundaries of 4 elements
     float scale_log2;
     // in the workspace, set by paged_attn
     PagedPlan* plan;

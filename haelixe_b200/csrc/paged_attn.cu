@@ -38,6 +38,12 @@ constexpr float kLn2 = 0.69314718055994530942f;
 struct Item {
     int n, h, c;  // sequence, key head, chunk of its query heads
 };
+// A run's part of an item: tiles [first, first + count) of a sequence of len keys. No tiles: no part.
+struct Part {
+    Item it;
+    int first, count, len, slot;
+    bool whole;
+};
 
 // Sequences with nothing to read (len <= 0) or longer than their table row have no tiles
 // and no items; paged_join_kernel writes their rows.
@@ -147,38 +153,63 @@ __device__ __forceinline__ uint4 ld_stream(const void* p) {
 // [HB][D + pad], (max in log2 units, sum) of each head.
 template <int HB, int DP>
 struct Parts {
-    static constexpr int kRow = DP + 2;
-    float o[kWarps][HB * kRow];
+    static constexpr int kRow = DP + 4;
+    alignas(16) float o[kWarps][HB * kRow];
     float2 ml[kWarps][HB];
 };
 
 __device__ __forceinline__ float safe_max(float m) { return m == -INFINITY ? 0.f : m; }
 
-// Joins the four warps' parts: the item's output, or the worker's part of it.
+// A part in the workspace: o of HB heads, then (max, sum) of each, a multiple of 16 bytes.
+__host__ __device__ constexpr int part_floats(int HB, int D) { return HB * (D + 4); }
+
+// 2^x to 2^-22, flushing denormals: for weights and probabilities.
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// Joins the four warps' parts: the item's output, or the worker's part of it. Four elements a thread.
 template <typename T, int HB, int DP>
 __device__ __forceinline__ void finish_item(const PagedAttn& a, const Parts<HB, DP>& sp, const Item& it, bool whole,
                                             int slot) {
-    const int D = a.cache.D;
+    const int D = a.cache.D, quads = D / 4;
     const int h0 = it.h * a.G + it.c * HB;
     const int heads = min(HB, a.G - it.c * HB);
-    for (int i = threadIdx.x; i < heads * D; i += kThreads) {
-        const int h = i / D, d = i - h * D;
-        float m = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sp.ml[w][h].x);
-        float l = 0.f, o = 0.f;
+    for (int i = threadIdx.x; i < heads * quads; i += kThreads) {
+        const int h = i / quads, d = 4 * (i - h * quads);
+        float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+        float2 ml[kWarps];
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            const float f = exp2f(sp.ml[w][h].x - safe_max(m));
-            l += f * sp.ml[w][h].y;
-            o += f * sp.o[w][h * Parts<HB, DP>::kRow + d];
+            ml[w] = sp.ml[w][h];
+            m = fmaxf(m, ml[w].x);
+        }
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float f = ex2(ml[w].x - safe_max(m));
+            const float4 u = *reinterpret_cast<const float4*>(&sp.o[w][h * Parts<HB, DP>::kRow + d]);
+            l = fmaf(f, ml[w].y, l);
+            o[0] = fmaf(f, u.x, o[0]), o[1] = fmaf(f, u.y, o[1]), o[2] = fmaf(f, u.z, o[2]), o[3] = fmaf(f, u.w, o[3]);
         }
         if (whole) {
-            ((T*)a.o)[(int64_t)it.n * a.o_sn + (int64_t)(h0 + h) * a.o_sh + d] = T(o / l);
+            T* to = (T*)a.o + (int64_t)it.n * a.o_sn + (int64_t)(h0 + h) * a.o_sh + d;
+            struct alignas(4 * sizeof(T)) Four {
+                T v[4];
+            } four;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) four.v[e] = T(o[e] / l);
+            if (a.o_vec) {
+                *reinterpret_cast<Four*>(to) = four;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) to[e] = four.v[e];
+            }
             if (d == 0 && a.lse) a.lse[(int64_t)it.n * a.Hq + h0 + h] = (m + log2f(l)) * kLn2;
         } else {
-            float* part = a.part + (int64_t)slot * HB * (D + 2);
-            part[h * D + d] = o;
+            float* part = a.part + (int64_t)slot * part_floats(HB, D);
+            *reinterpret_cast<float4*>(part + h * D + d) = make_float4(o[0], o[1], o[2], o[3]);
             if (d == 0) reinterpret_cast<float2*>(part + HB * D)[h] = make_float2(m, l);
         }
     }
@@ -194,7 +225,8 @@ __device__ __forceinline__ void finish_item(const PagedAttn& a, const Parts<HB, 
 // layout to the second's by an 8x8 transpose, as bf16 hi + lo, so that the
 // result carries only its own rounding.
 // K of the next step is loaded as soon as the scores are taken, V as soon as P V is,
-// so one of the two is always in flight.
+// so one of the two is always in flight; after the last step of an item those of the
+// worker's next one, so that they are there when the item is joined and stored.
 template <int DC, int NT>
 struct AttnBf16 {
     static constexpr int kD = 64 * DC;       // D rounded up; the rest reads as zero
@@ -205,9 +237,11 @@ struct AttnBf16 {
     float acc[NT][DC][4][4];
     float m[NT][2], l[NT][2];
     const PagedAttn& a;
+    // Where the loads are: this lane's key (of 16) of the next step, its row, its page's number.
     const int32_t* row;
     const __nv_bfloat16 *kh, *vh;
-    int len, g, t;
+    int64_t off;
+    int len, key, page, g, t;
 
     __device__ __forceinline__ AttnBf16(const PagedAttn& args) : a(args) {
         g = (threadIdx.x % 32) / 4;
@@ -224,7 +258,7 @@ struct AttnBf16 {
             k[1][b] = in && o1 >= 0 ? ld_stream(kh + o1 + d) : make_uint4(0, 0, 0, 0);
         }
     }
-    __device__ __forceinline__ void load_v(int64_t off, int c0) {
+    __device__ __forceinline__ void load_v(const __nv_bfloat16* vh, int64_t off, int c0) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int64_t o = __shfl_sync(0xffffffffu, off, 2 * t + (j & 1) + 8 * (j >> 1));
@@ -236,27 +270,45 @@ struct AttnBf16 {
         }
     }
 
-    __device__ __forceinline__ void run(const Item& it, int tile, int tiles, Parts<HB, kD>& sp) {
+    __device__ __forceinline__ const int32_t* row_of(const Part& p) const {
+        return a.cache.table + (int64_t)p.it.n * a.cache.table_stride;
+    }
+    // Key of this lane at step i of a part: 64 (first + i) + 16 warp + lane % 16.
+    __device__ __forceinline__ int first_key(const Part& p) const {
+        return p.first * kTile + threadIdx.x / 32 * kWarpKeys + threadIdx.x % 16;
+    }
+    // Moves to a part, whose first page number is pg, and loads its queries and first keys.
+    __device__ __forceinline__ void enter(const Part& p, int pg) {
         const PagedView& c = a.cache;
-        const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-        len = a.lens[it.n];
-        row = c.table + (int64_t)it.n * c.table_stride;
-        kh = (const __nv_bfloat16*)c.k + (int64_t)it.h * c.sh;
-        vh = (const __nv_bfloat16*)c.v + (int64_t)it.h * c.sh;
-        const int h0 = it.h * a.G + it.c * HB, heads = min(HB, a.G - it.c * HB);
-        // Key of this lane (16 of them) at step i: tile * 64 + 64 i + 16 warp + lane % 16.
-        int key = tile * kTile + warp * kWarpKeys + lane % 16;
-        int page = entry_of(c, row, key, len);
+        len = p.len;
+        row = row_of(p);
+        kh = (const __nv_bfloat16*)c.k + (int64_t)p.it.h * c.sh;
+        vh = (const __nv_bfloat16*)c.v + (int64_t)p.it.h * c.sh;
+        key = first_key(p);
+        off = offset_of(c, pg, key, len);
+        load_k(off);
+        const int h0 = p.it.h * a.G + p.it.c * HB, heads = min(HB, a.G - p.it.c * HB);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int b = 0; b < 2 * DC; ++b) {
                 const int d = 32 * b + 8 * t;
                 q[n][b] = 8 * n + g < heads && d < c.D
-                              ? *reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.q + (int64_t)it.n * a.q_sn +
+                              ? *reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.q + (int64_t)p.it.n * a.q_sn +
                                                                 (int64_t)(h0 + 8 * n + g) * a.q_sh + d)
                               : make_uint4(0, 0, 0, 0);
             }
+        page = entry_of(c, row, key + kTile, len);
+    }
+    __device__ __forceinline__ void begin(const Part& p) {
+        enter(p, entry_of(a.cache, row_of(p), first_key(p), p.len));
+        load_v(vh, off, 0);
+    }
+
+    __device__ __forceinline__ void run(const Part& part, const Part& next, Parts<HB, kD>& sp) {
+        const PagedView& c = a.cache;
+        const int warp = threadIdx.x / 32, tiles = part.count;
+        const int next_page = next.count ? entry_of(c, row_of(next), first_key(next), next.len) : 0;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             m[n][0] = m[n][1] = -INFINITY;
@@ -268,10 +320,6 @@ struct AttnBf16 {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) acc[n][x][e][r] = 0.f;
         }
-        int64_t off = offset_of(c, page, key, len);
-        load_k(off);
-        load_v(off, 0);
-        page = entry_of(c, row, key + kTile, len);
         for (int i = 0; i < tiles; ++i) {
             const uint32_t bad = __ballot_sync(0xffffffffu, off == kBad);
             const uint32_t none = __ballot_sync(0xffffffffu, off == kNone);
@@ -288,12 +336,15 @@ struct AttnBf16 {
                 }
             }
             const int64_t off_now = off;
+            const __nv_bfloat16* const vh_now = vh;
             const bool more = i + 1 < tiles;
             if (more) {
                 key += kTile;
                 off = offset_of(c, page, key, len);
                 load_k(off);
                 if (i + 2 < tiles) page = entry_of(c, row, key + kTile, len);
+            } else if (next.count) {
+                enter(next, next_page);
             }
             uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
@@ -316,7 +367,7 @@ struct AttnBf16 {
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         const float mn = fmaxf(m[n][r], mx[r]);
-                        const float f = exp2f(m[n][r] - safe_max(mn));
+                        const float f = ex2(m[n][r] - safe_max(mn));
                         m[n][r] = mn;
                         l[n][r] *= f;
 #pragma unroll
@@ -331,7 +382,7 @@ struct AttnBf16 {
                 const float m0 = safe_max(m[n][0]), m1 = safe_max(m[n][1]);
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const float p0 = exp2f(s[n][2 * r] - m0), p1 = exp2f(s[n][2 * r + 1] - m1);
+                    const float p0 = ex2(s[n][2 * r] - m0), p1 = ex2(s[n][2 * r + 1] - m1);
                     l[n][0] += p0;
                     l[n][1] += p1;
                     const uint32_t hi = pack_bf16(p0, p1);
@@ -342,7 +393,7 @@ struct AttnBf16 {
             }
 #pragma unroll
             for (int c0 = 0; c0 < DC; c0 += VC) {
-                if (c0 > 0) load_v(off_now, c0);
+                if (c0 > 0) load_v(vh_now, off_now, c0);
 #pragma unroll
                 for (int x = 0; x < VC; ++x) {
                     const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&v[0][x]);
@@ -361,7 +412,7 @@ struct AttnBf16 {
                     }
                 }
             }
-            if (more) load_v(off, 0);
+            if (more || next.count) load_v(vh, off, 0);
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -426,10 +477,12 @@ struct AttnF32 {
     Scratch& sm;
     __device__ __forceinline__ AttnF32(const PagedAttn& args, Scratch& scratch) : a(args), sm(scratch) {}
 
-    __device__ __forceinline__ void run(const Item& it, int tile, int tiles, Parts<HB, kD>& sp) {
+    __device__ __forceinline__ void begin(const Part&) {}
+    __device__ __forceinline__ void run(const Part& part, const Part&, Parts<HB, kD>& sp) {
         const PagedView& c = a.cache;
+        const Item it = part.it;
         const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
-        const int len = a.lens[it.n], D = c.D;
+        const int len = part.len, D = c.D, tile = part.first, tiles = part.count;
         const int32_t* row = c.table + (int64_t)it.n * c.table_stride;
         const float* kh = (const float*)c.k + (int64_t)it.h * c.sh;
         const float* vh = (const float*)c.v + (int64_t)it.h * c.sh;
@@ -562,33 +615,45 @@ __device__ __forceinline__ void paged_worker(const PagedAttn& a, W& w, Parts<W::
     if (!find_run(a, per, start, end, n, before, empty)) return;
     int tiles = tiles_of(a, n), places = places_of(tiles, empty);
     int item = (int)((start - before) / places), place = (int)((start - before) - (int64_t)item * places);
-    for (int64_t at = start; at < end;) {
-        const int take = (int)min((int64_t)(places - place), end - at);
-        const int first = max(place - empty, 0), last = place + take - empty;  // tiles [first, last)
-        if (last > first) {
-            const Item it{n, item / chunks, item % chunks};
-            w.run(it, first, last - first, sp);
-            __syncthreads();
-            // The worker's second part is the one whose first tile it has.
-            finish_item<T, W::HB, W::kD>(a, sp, it, last - first == tiles,
-                                         2 * blockIdx.x + (first == 0 && at - place + empty > start));
-            __syncthreads();
+    int64_t at = start;
+    auto next_part = [&]() -> Part {
+        while (at < end) {
+            const int take = (int)min((int64_t)(places - place), end - at);
+            const int first = max(place - empty, 0), last = place + take - empty;  // tiles [first, last)
+            // The worker's second slot is for the item whose first tile it has.
+            const Part p{Item{n, item / chunks, item % chunks}, first, max(last - first, 0), a.lens[n],
+                         2 * (int)blockIdx.x + (first == 0 && at - place + empty > start), last - first == tiles};
+            at += take;
+            place = 0;
+            if (++item == per && at < end) {
+                item = 0;
+                do {
+                    if (++n == a.cache.num_seqs) {
+                        at = end;
+                        break;
+                    }
+                    tiles = tiles_of(a, n);
+                } while (tiles == 0);
+                places = places_of(tiles, empty);
+            }
+            if (p.count) return p;
         }
-        at += take;
-        place = 0;
-        if (++item == per && at < end) {
-            item = 0;
-            do {
-                if (++n == a.cache.num_seqs) return;
-                tiles = tiles_of(a, n);
-            } while (tiles == 0);
-            places = places_of(tiles, empty);
-        }
+        return Part{Item{0, 0, 0}, 0, 0, 0, 0, false};
+    };
+    Part part = next_part();
+    if (part.count) w.begin(part);
+    while (part.count) {
+        const Part next = next_part();
+        w.run(part, next, sp);
+        __syncthreads();
+        finish_item<T, W::HB, W::kD>(a, sp, part.it, part.whole, part.slot);
+        __syncthreads();
+        part = next;
     }
 }
 
 template <int DC, int NT>
-__global__ void __launch_bounds__(kThreads) paged_attn_bf16_kernel(PagedAttn a) {
+__global__ void __launch_bounds__(kThreads, DC == 2 && NT == 1 ? 3 : DC == 1 && NT == 1 ? 4 : 1) paged_attn_bf16_kernel(PagedAttn a) {
     __shared__ Parts<8 * NT, 64 * DC> sp;
     AttnBf16<DC, NT> w(a);
     paged_worker<__nv_bfloat16>(a, w, sp);
@@ -645,7 +710,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(PagedAttn a
             const int wk = w + k * warps;
             ml[k] = make_float2(-INFINITY, 0.f);
             if (wk <= w1) {
-                const float* part = a.part + (int64_t)(2 * wk + (first > run * wk)) * HB * (D + 2);
+                const float* part = a.part + (int64_t)(2 * wk + (first > run * wk)) * part_floats(HB, D);
                 ml[k] = reinterpret_cast<const float2*>(part + HB * D)[head];
 #pragma unroll
                 for (int x = 0; x < 8; ++x) v[k][x] = lane + 32 * x < D ? part[head * D + lane + 32 * x] : 0.f;
@@ -722,7 +787,7 @@ int heads_at_once(hx_dtype dt, int G, int D) {
 static uint64_t plan_bytes(int num_seqs) { return (sizeof(Plan) + (uint64_t)num_seqs * sizeof(int64_t) + 255) / 256 * 256; }
 
 uint64_t paged_attn_workspace_bytes(hx_dtype dt, int Hq, int Hkv, int D, int num_seqs) {
-    return plan_bytes(num_seqs) + (uint64_t)2 * kMaxWorkers * heads_at_once(dt, Hq / Hkv, D) * (D + 2) * sizeof(float);
+    return plan_bytes(num_seqs) + (uint64_t)2 * kMaxWorkers * part_floats(heads_at_once(dt, Hq / Hkv, D), D) * sizeof(float);
 }
 
 cudaError_t paged_attn(cudaStream_t st, int sm_count, hx_dtype dt, PagedAttn a, void* workspace) {

@@ -492,3 +492,26 @@ def test_capture_without_a_workspace_is_refused():
     with torch.cuda.graph(graph):
         one += 1  # a graph of its own, beside the refused call
         assert call() == N.HX_ERR_INVALID
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_outputs_at_any_element(dtype):
+    """An output that starts at an odd element, with rows of an odd stride."""
+    lens = [90, 700, 0]
+    cache, ks, vs = _filled(70, dtype, lens, 16, 2, 64)
+    q = torch.randn(3, 4, 64, generator=_gen(1), device="cuda", dtype=dtype)
+    wide = torch.full((3, 4, 67), 5.0, device="cuda", dtype=dtype)
+    o, lse = hx.paged_attention(cache, q, _lens(*lens), 0.125, out=wide[:, :, 1:65])
+    _check(q, ks, vs, 0.125, o, lse)
+    assert (wide[:, :, 0] == 5).all() and (wide[:, :, 65:] == 5).all()
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("hk,group,dim", [(16, 1, 64), (16, 1, 40), (8, 2, 72), (5, 5, 128), (4, 16, 64)])
+def test_more_tiles_than_workers(dtype, hk, group, dim):
+    """Runs that end one item and begin the next, so that workers leave both of their parts."""
+    lens = [1500 - 97 * i for i in range(14)] + [3, 0, 700]
+    cache, ks, vs = _filled(71, dtype, lens, 24, hk, dim)
+    q = torch.randn(len(lens), hk * group, dim, generator=_gen(2), device="cuda", dtype=dtype)
+    o, lse = hx.paged_attention(cache, q, _lens(*lens), dim ** -0.5)
+    _check(q, ks, vs, dim ** -0.5, o, lse)

@@ -23,8 +23,8 @@ def _size(cache, dtype=N.HX_BF16, heads=8):
 def test_workspace_size_of_a_good_cache():
     st, n = _size(_cache())
     # A 256-byte multiple for 3 sequences, then two parts for each of up to 1024 workers, of 8 heads
-    # of (head_dim + max and sum) floats.
-    assert st == N.HX_OK and n == 256 + 2 * 1024 * 8 * (64 + 2) * 4
+    # of head_dim floats, the maximum and the sum, in 16-byte pieces.
+    assert st == N.HX_OK and n == 256 + 2 * 1024 * 8 * (64 + 4) * 4
 
 
 @pytest.mark.parametrize("over,status", [
