@@ -788,7 +788,8 @@ int hx_paged_attention(hx_ctx* c, hx_dtype dt, const hx_paged_cache* cache, int 
     const char* who = "hx_paged_attention";
     int st;
     if ((st = validate_cache(c, dt, cache, who)) || (st = paged_heads(c, cache, Hq, who))) return st;
-    if (!isfinite(scale)) return set_error(c, HX_ERR_INVALID, "%s: scale is not finite", who);
+    const float scale_log2 = scale * 1.4426950408889634f;
+    if (!isfinite(scale_log2)) return set_error(c, HX_ERR_INVALID, "%s: scale is not finite or too large", who);
     if (cache->num_seqs == 0) return HX_OK;
     if (!q || !o || !q->data || !o->data || !seq_lens)
         return set_error(c, HX_ERR_INVALID, "%s: NULL operand", who);
@@ -822,7 +823,7 @@ int hx_paged_attention(hx_ctx* c, hx_dtype dt, const hx_paged_cache* cache, int 
     a.Hq = Hq;
     a.G = Hq / cache->H;
     a.o_vec = (uintptr_t)a.o % (4 * eb) == 0 && a.o_sn % 4 == 0 && a.o_sh % 4 == 0;
-    a.scale_log2 = scale * 1.4426950408889634f;
+    a.scale_log2 = scale_log2;
     st = check_cuda(c, hx::paged_attn(c->stream, c->sm_count, dt, a, ws), who);
     if (workspace == nullptr) hx_free(c, ws);  // stream-ordered: the next user of the slab queues behind us
     return st;

@@ -45,11 +45,14 @@ struct Part {
     bool whole;
 };
 
-// Sequences with nothing to read (len <= 0) or longer than their table row have no tiles
-// and no items; paged_join_kernel writes their rows.
+// Sequences with nothing to read (len <= 0) or longer than their table row (or than 2^31 - 256, so
+// that a key past the last tile still is an int) have no tiles and no items; paged_join_kernel
+// writes their rows.
 __device__ __forceinline__ int tiles_of(const PagedAttn& a, int n) {
     const int64_t len = a.lens[n];
-    return len <= 0 || len > (int64_t)a.cache.max_pages * a.cache.page_size ? 0 : (int)((len + kTile - 1) / kTile);
+    return len <= 0 || len > (int64_t)a.cache.max_pages * a.cache.page_size || len > 0x7fffff00
+               ? 0
+               : (int)((len + kTile - 1) / kTile);
 }
 
 // Where the work of a call lies: the empty places of an item, the length of a run, the places
@@ -141,9 +144,11 @@ __device__ __forceinline__ int64_t offset_of(const PagedView& c, int page, int k
     return (int64_t)page * c.sp + (int64_t)slot * c.ss;
 }
 
+// Not through the read-only path: the kernel may have been launched while the one before it was
+// still writing the cache.
 __device__ __forceinline__ uint4 ld_stream(const void* p) {
     uint4 u;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
                  : "l"(p));
     return u;

@@ -607,8 +607,8 @@ class BlockStack:
 
     @torch.no_grad()
     def prefill(self, ids: torch.Tensor, caches: list, lens: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """Prompts [B, S] (row b is sequence b of the caches; its first lens[b] ids count, all without
-        lens) into the caches. Returns the logits [B, vocab] after each prompt's last token."""
+        """Prompts [B, S] (row b is sequence b of the caches; its first lens[b] >= 1 ids count, all
+        without lens; the table must hold them) into the caches. Returns the logits [B, vocab] after each prompt's last token."""
         self._answers(caches)
         B, S = ids.shape
         positions = torch.arange(S, dtype=torch.int32, device=ids.device).repeat(B)
@@ -627,7 +627,8 @@ class BlockStack:
     def decode(self, ids: torch.Tensor, caches: list, positions: torch.Tensor) -> torch.Tensor:
         """One new token a sequence: ids [B], at positions [B] (int32; what the caches hold before them
         is what each attends to, itself included). A negative position leaves its sequence out.
-        Returns the logits [B, vocab] (of a sequence that is left out: of no use)."""
+        Returns the logits [B, vocab]: of no use for a sequence that is left out, NaN for a position
+        outside the table."""
         self._answers(caches)
         every = torch.arange(ids.shape[0], dtype=torch.int32, device=ids.device)
         seq_ids = torch.where(positions < 0, -1, every)

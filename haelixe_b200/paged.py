@@ -9,8 +9,8 @@ positions (`paged_attention`, the formula of `Tensor::flash_attention`,
 src/tensor.rs:644-666, for one query a sequence).
 
 Both are for inference: they have no backward and refuse tensors that would
-need one. Calls of several host threads may overlap: each runs on its thread's
-current stream.
+need one. They may be called from several host threads at once: each call runs
+on its thread's current stream.
 """
 from __future__ import annotations
 
@@ -145,7 +145,8 @@ def paged_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, seq_ids:
     With rope_base, k is rotated by its position, and so is q [tokens, query
     heads, head_dim], in the same launch; the result is out_q (a new tensor by
     default; q itself for in place). A negative seq_id marks padding: nothing of
-    that token is written, its row of out_q included. A token whose sequence or
+    that token is written, its row of out_q included. No two tokens may have the same
+    place. A token whose sequence or
     position the table does not hold, or whose entry there is no page, writes
     nothing to the cache and NaN to its row of out_q.
     """
@@ -158,7 +159,7 @@ def paged_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, seq_ids:
     base = 0.0
     if rope_base is not None:
         base = float(rope_base)
-        if not base > 0.0:
+        if not base >= 1e-30:  # 0 stands for no rotation below
             raise ValueError("paged_append: rope_base must be positive")
     if q is not None:
         heads = q.shape[1] if q.dim() == 3 else 0

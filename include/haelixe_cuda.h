@@ -261,7 +261,8 @@ typedef struct hx_rows {
  * A token with a negative seq_id is padding: neither the cache nor its q_out
  * row is touched. A token without a slot (sequence or position outside the
  * table, an entry that is no page) writes nothing to the cache and NaN to its
- * q_out row. Two tokens of a call with the same slot leave either's values. */
+ * q_out row. Two tokens of a call must not have the
+ * same slot: it would hold a mixture of both. */
 int hx_paged_append(hx_ctx* ctx, hx_dtype dtype, const hx_paged_cache* cache, int tokens, const hx_rows* k,
                     const hx_rows* v, const int32_t* seq_ids, const int32_t* positions, int Hq, const hx_rows* q,
                     const hx_rows* q_out, float rope_base);
@@ -274,8 +275,8 @@ int hx_paged_attention_workspace_size(hx_dtype dtype, const hx_paged_cache* cach
  * hx_flash_attention_fwd for one query a sequence. Query head h reads key head
  * h / (Hq / H); Hq is a multiple of H. lse (f32 [num_seqs, Hq], may be NULL)
  * receives the log-sum-exp of the scaled scores. A sequence with seq_lens <= 0
- * gives zeros and an lse of -inf; one that is longer than its table row, or
- * that reads an entry that is no page, gives NaN. Positions at or past
+ * gives zeros and an lse of -inf; one that is longer than its table row (or
+ * than 2^31 - 256), or that reads an entry that is no page, gives NaN. Positions at or past
  * seq_lens are not read. The result does not depend on what else is in the
  * batch beyond f32 rounding, and equal calls give equal bits. workspace
  * (256-byte aligned) may be NULL, except during stream capture: the call then
@@ -305,8 +306,9 @@ int hx_linear_bwd(hx_ctx* ctx, hx_dtype dtype, const void* x, const void* w, con
  * of k = 8 o ... 8 o + 7, the first in the lowest 4 bits; those at or past in
  * are ignored. scales [ceil(in / group), out], b, residual and x are in
  * `dtype`; b and residual may be NULL, residual may alias y; group is a
- * multiple of 32. Sums in f32, one rounding. A weight is read once for each 32
- * rows: for many rows a bf16 weight and hx_linear_fwd are faster. */
+ * multiple of 32, rows at most 16 * 65535. Sums in f32, one rounding. A weight
+ * is read once for each 32 rows (16 in f32): for many rows a bf16 weight and
+ * hx_linear_fwd are faster. */
 int hx_linear_w4_fwd(hx_ctx* ctx, hx_dtype dtype, const void* x, const uint32_t* packed, const void* scales,
                      const void* b, const void* residual, void* y, int rows, int in_features, int out_features,
                      int group);

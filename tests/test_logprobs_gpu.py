@@ -330,3 +330,34 @@ def test_refusals_and_empty():
     assert L.hx_token_logprobs_bwd(c.handle, 0, p, 10, p, None, p, p, p, 10, 3, 10) == N.HX_ERR_INVALID
     assert L.hx_token_logprobs_bwd(c.handle, 0, p, 10, p, p, p, p, p, 9, 3, 10) == N.HX_ERR_INVALID
     assert L.hx_token_logprobs_fwd(None, 0, p, 10, p, p, p, None, 0, None, None, 3, 10) == N.HX_ERR_INVALID
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("classes", [5, 4099, 40000])
+def test_gradient_written_over_the_logits(dtype, classes):
+    """The library's backward with dlogits on the logits themselves gives what it gives beside them."""
+    x, t = _logits(9, classes, dtype), _targets(9, classes).to(torch.int32)
+    g = torch.randn(9, generator=_gen(1), device="cuda")
+    leaf = x.clone().requires_grad_()
+    r = hx.nn.token_logprobs(leaf, t)
+    (want,) = torch.autograd.grad([r.logprob, r.entropy], [leaf], [g, g])
+    stats, lp, h = (torch.empty(9, n, device="cuda") for n in (3, 1, 1))
+    c = hx.context()
+    c.use_stream()
+    d = 0 if dtype == F32 else 1
+    p = x.data_ptr()
+    N.check(N.lib().hx_token_logprobs_fwd(c.handle, d, p, classes, t.data_ptr(), lp.data_ptr(), h.data_ptr(), stats.data_ptr(),
+                                          0, None, None, 9, classes), c.handle)
+    N.check(N.lib().hx_token_logprobs_bwd(c.handle, d, p, classes, t.data_ptr(), stats.data_ptr(), g.data_ptr(), g.data_ptr(),
+                                          p, classes, 9, classes), c.handle)
+    assert torch.equal(x, want)
+
+
+def test_gradient_of_shared_rows():
+    """Rows that are one row expanded: its gradient is the sum."""
+    row = _logits(1, 50, F32).requires_grad_()
+    t, g = _targets(4, 50), torch.randn(4, generator=_gen(2), device="cuda")
+    (hx.nn.token_logprobs(row.expand(4, 50), t).logprob * g).sum().backward()
+    ref = Ref(row.detach().expand(4, 50), t)
+    want, off = ref.grad(g, None)
+    _close(row.grad, want.sum(0, keepdim=True), off.sum(0, keepdim=True) + 2.0 ** -22 * want.abs().sum(0, keepdim=True))

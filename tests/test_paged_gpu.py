@@ -515,3 +515,31 @@ def test_more_tiles_than_workers(dtype, hk, group, dim):
     q = torch.randn(len(lens), hk * group, dim, generator=_gen(2), device="cuda", dtype=dtype)
     o, lse = hx.paged_attention(cache, q, _lens(*lens), dim ** -0.5)
     _check(q, ks, vs, dim ** -0.5, o, lse)
+
+
+def test_steps_that_follow_each_other_see_each_others_writes():
+    """Append and attention in turn on one stream, with nothing between them: every step attends to
+    the token that the call before it wrote, to pages that earlier calls read."""
+    H, D, n = 4, 64, 300
+    table = torch.randperm(60, generator=_gen(3), device="cuda")[:40].to(torch.int32).view(2, 20)
+    cache = hx.PagedKVCache.allocate(60, 16, H, D, table, dtype=F32)
+    k, v, q = (torch.randn(n, 2, H, D, generator=_gen(s), device="cuda") for s in (4, 5, 6))
+    seq = _lens(0, 1)
+    at = [_lens(i, i) for i in range(n + 1)]
+    torch.cuda.synchronize()
+    outs = []
+    for i in range(n):
+        hx.paged_append(cache, k[i], v[i], seq, at[i])
+        outs.append(hx.paged_attention(cache, q[i], at[i + 1], 0.125))
+    for i in range(0, n, 23):
+        ks, vs = ([t[:i + 1, s] for s in range(2)] for t in (k, v))
+        _check(q[i], ks, vs, 0.125, *outs[i])
+
+
+def test_lengths_near_the_largest_integer():
+    """A table row of 2^31 positions on one page: lengths past 2^31 - 256 are refused with NaN."""
+    page = 1 << 20
+    table = torch.zeros(3, 2048, dtype=torch.int32, device="cuda")
+    cache = hx.PagedKVCache(*(torch.zeros(1, page, 1, 8, device="cuda", dtype=BF16) for _ in range(2)), table)
+    o, lse = hx.paged_attention(cache, torch.zeros(3, 1, 8, device="cuda", dtype=BF16), _lens(2**31 - 1, 5, 2**31 - 255), 1.0)
+    assert torch.isnan(o[[0, 2]]).all() and (o[1] == 0).all()
