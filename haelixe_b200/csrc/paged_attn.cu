@@ -230,8 +230,8 @@ __device__ __forceinline__ void finish_item(const PagedAttn& a, const Parts<HB, 
 // layout to the second's by an 8x8 transpose, as bf16 hi + lo, so that the
 // result carries only its own rounding.
 // K of the next step is loaded as soon as the scores are taken, V as soon as P V is,
-// so one of the two is always in flight; after the last step of an item those of the
-// worker's next one, so that they are there when the item is joined and stored.
+// so one of the two is always in flight. (Loading the worker's next item's while one is joined
+// and stored gained nothing: the SM's other workers are in the middle of theirs.)
 template <int DC, int NT>
 struct AttnBf16 {
     static constexpr int kD = 64 * DC;       // D rounded up; the rest reads as zero
@@ -242,11 +242,8 @@ struct AttnBf16 {
     float acc[NT][DC][4][4];
     float m[NT][2], l[NT][2];
     const PagedAttn& a;
-    // Where the loads are: this lane's key (of 16) of the next step, its row, its page's number.
-    const int32_t* row;
     const __nv_bfloat16 *kh, *vh;
-    int64_t off;
-    int len, key, page, g, t;
+    int g, t;
 
     __device__ __forceinline__ AttnBf16(const PagedAttn& args) : a(args) {
         g = (threadIdx.x % 32) / 4;
@@ -263,7 +260,7 @@ struct AttnBf16 {
             k[1][b] = in && o1 >= 0 ? ld_stream(kh + o1 + d) : make_uint4(0, 0, 0, 0);
         }
     }
-    __device__ __forceinline__ void load_v(const __nv_bfloat16* vh, int64_t off, int c0) {
+    __device__ __forceinline__ void load_v(int64_t off, int c0) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int64_t o = __shfl_sync(0xffffffffu, off, 2 * t + (j & 1) + 8 * (j >> 1));
@@ -275,45 +272,27 @@ struct AttnBf16 {
         }
     }
 
-    __device__ __forceinline__ const int32_t* row_of(const Part& p) const {
-        return a.cache.table + (int64_t)p.it.n * a.cache.table_stride;
-    }
-    // Key of this lane at step i of a part: 64 (first + i) + 16 warp + lane % 16.
-    __device__ __forceinline__ int first_key(const Part& p) const {
-        return p.first * kTile + threadIdx.x / 32 * kWarpKeys + threadIdx.x % 16;
-    }
-    // Moves to a part, whose first page number is pg, and loads its queries and first keys.
-    __device__ __forceinline__ void enter(const Part& p, int pg) {
+    __device__ __forceinline__ void run(const Part& part, Parts<HB, kD>& sp) {
         const PagedView& c = a.cache;
-        len = p.len;
-        row = row_of(p);
-        kh = (const __nv_bfloat16*)c.k + (int64_t)p.it.h * c.sh;
-        vh = (const __nv_bfloat16*)c.v + (int64_t)p.it.h * c.sh;
-        key = first_key(p);
-        off = offset_of(c, pg, key, len);
-        load_k(off);
-        const int h0 = p.it.h * a.G + p.it.c * HB, heads = min(HB, a.G - p.it.c * HB);
+        const Item& it = part.it;
+        const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, tiles = part.count, len = part.len;
+        const int32_t* row = c.table + (int64_t)it.n * c.table_stride;
+        kh = (const __nv_bfloat16*)c.k + (int64_t)it.h * c.sh;
+        vh = (const __nv_bfloat16*)c.v + (int64_t)it.h * c.sh;
+        const int h0 = it.h * a.G + it.c * HB, heads = min(HB, a.G - it.c * HB);
+        // Key of this lane (16 of them) at step i: 64 (first + i) + 16 warp + lane % 16.
+        int key = part.first * kTile + warp * kWarpKeys + lane % 16;
+        int page = entry_of(c, row, key, len);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int b = 0; b < 2 * DC; ++b) {
                 const int d = 32 * b + 8 * t;
                 q[n][b] = 8 * n + g < heads && d < c.D
-                              ? *reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.q + (int64_t)p.it.n * a.q_sn +
+                              ? *reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.q + (int64_t)it.n * a.q_sn +
                                                                 (int64_t)(h0 + 8 * n + g) * a.q_sh + d)
                               : make_uint4(0, 0, 0, 0);
             }
-        page = entry_of(c, row, key + kTile, len);
-    }
-    __device__ __forceinline__ void begin(const Part& p) {
-        enter(p, entry_of(a.cache, row_of(p), first_key(p), p.len));
-        load_v(vh, off, 0);
-    }
-
-    __device__ __forceinline__ void run(const Part& part, const Part& next, Parts<HB, kD>& sp) {
-        const PagedView& c = a.cache;
-        const int warp = threadIdx.x / 32, tiles = part.count;
-        const int next_page = next.count ? entry_of(c, row_of(next), first_key(next), next.len) : 0;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             m[n][0] = m[n][1] = -INFINITY;
@@ -325,6 +304,10 @@ struct AttnBf16 {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) acc[n][x][e][r] = 0.f;
         }
+        int64_t off = offset_of(c, page, key, len);
+        load_k(off);
+        load_v(off, 0);
+        page = entry_of(c, row, key + kTile, len);
         for (int i = 0; i < tiles; ++i) {
             const uint32_t bad = __ballot_sync(0xffffffffu, off == kBad);
             const uint32_t none = __ballot_sync(0xffffffffu, off == kNone);
@@ -341,15 +324,12 @@ struct AttnBf16 {
                 }
             }
             const int64_t off_now = off;
-            const __nv_bfloat16* const vh_now = vh;
             const bool more = i + 1 < tiles;
             if (more) {
                 key += kTile;
                 off = offset_of(c, page, key, len);
                 load_k(off);
                 if (i + 2 < tiles) page = entry_of(c, row, key + kTile, len);
-            } else if (next.count) {
-                enter(next, next_page);
             }
             uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
@@ -398,7 +378,7 @@ struct AttnBf16 {
             }
 #pragma unroll
             for (int c0 = 0; c0 < DC; c0 += VC) {
-                if (c0 > 0) load_v(vh_now, off_now, c0);
+                if (c0 > 0) load_v(off_now, c0);
 #pragma unroll
                 for (int x = 0; x < VC; ++x) {
                     const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&v[0][x]);
@@ -417,7 +397,7 @@ struct AttnBf16 {
                     }
                 }
             }
-            if (more || next.count) load_v(vh, off, 0);
+            if (more) load_v(off, 0);
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -482,8 +462,7 @@ struct AttnF32 {
     Scratch& sm;
     __device__ __forceinline__ AttnF32(const PagedAttn& args, Scratch& scratch) : a(args), sm(scratch) {}
 
-    __device__ __forceinline__ void begin(const Part&) {}
-    __device__ __forceinline__ void run(const Part& part, const Part&, Parts<HB, kD>& sp) {
+    __device__ __forceinline__ void run(const Part& part, Parts<HB, kD>& sp) {
         const PagedView& c = a.cache;
         const Item it = part.it;
         const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
@@ -645,15 +624,11 @@ __device__ __forceinline__ void paged_worker(const PagedAttn& a, W& w, Parts<W::
         }
         return Part{Item{0, 0, 0}, 0, 0, 0, 0, false};
     };
-    Part part = next_part();
-    if (part.count) w.begin(part);
-    while (part.count) {
-        const Part next = next_part();
-        w.run(part, next, sp);
+    for (Part part = next_part(); part.count; part = next_part()) {
+        w.run(part, sp);
         __syncthreads();
         finish_item<T, W::HB, W::kD>(a, sp, part.it, part.whole, part.slot);
         __syncthreads();
-        part = next;
     }
 }
 
