@@ -17,6 +17,7 @@
 // only moves when a score passes it by 2^8, so the accumulator is rarely rescaled.
 // Positions at or past len are never read: their pages may hold anything.
 #include <atomic>
+#include <type_traits>
 
 #include "hx_internal.h"
 #include "launch.h"
@@ -434,24 +435,27 @@ struct AttnF32 {
         float f[kWarps][GH];
     };
 
-    static constexpr bool kAhead = DV <= 4 && DV * GH <= 16;
+    static constexpr bool kAhead = DV == 2 && GH <= 4;
 
-    // This lane's elements of a value row; zero without a row.
-    static __device__ __forceinline__ void load_v(float (&v)[DV], const float* vh, int64_t o, int lane, int D) {
+    // This lane's elements of a value row. WHOLE: there is a row, of kD elements; else what is missing is zero.
+    template <bool WHOLE>
+    static __device__ __forceinline__ void load_v(float (&v)[DV], const float* row, bool there, int lane, int D) {
+        if constexpr (!WHOLE) {
 #pragma unroll
-        for (int x = 0; x < DV; ++x) v[x] = 0.f;
-        if (o < 0) return;
+            for (int x = 0; x < DV; ++x) v[x] = 0.f;
+            if (!there) return;
+        }
         if constexpr (DV == 2) {
-            if (2 * lane < D) {
-                const float2 u = *reinterpret_cast<const float2*>(vh + o + 2 * lane);
+            if (WHOLE || 2 * lane < D) {
+                const float2 u = *reinterpret_cast<const float2*>(row + 2 * lane);
                 v[0] = u.x, v[1] = u.y;
             }
         } else {
 #pragma unroll
             for (int x = 0; x < DV; x += 4) {
                 const int d = 32 * x + 4 * lane;
-                if (d < D) {
-                    const float4 u = *reinterpret_cast<const float4*>(vh + o + d);
+                if (WHOLE || d < D) {
+                    const float4 u = *reinterpret_cast<const float4*>(row + d);
                     v[x] = u.x, v[x + 1] = u.y, v[x + 2] = u.z, v[x + 3] = u.w;
                 }
             }
@@ -471,6 +475,56 @@ struct AttnF32 {
         const float* kh = (const float*)c.k + (int64_t)it.h * c.sh;
         const float* vh = (const float*)c.v + (int64_t)it.h * c.sh;
         const int h0 = it.h * a.G + it.c * HB, heads = min(HB, a.G - it.c * HB);
+        int key = tile * kTile + warp * kWarpKeys + lane % 16;
+        int page = entry_of(c, row, key, len);
+        int64_t off = 0;
+        // Keys and values a step ahead, as in bf16, where the registers allow it.
+        constexpr int kN = kD / 16;
+        float4 kx[kN], ky[kN];
+        float v[kWarpKeys][DV];
+        // Sixteen keys that are all there, of kD elements, ask nothing for each load, and on one page
+        // their rows follow each other. (The general way takes three times the instructions.)
+        bool whole = false, one_page = false;
+        auto locate = [&] {
+            whole = D == kD && __all_sync(0xffffffffu, off >= 0);
+            const int64_t off0 = __shfl_sync(0xffffffffu, off, 0);
+            one_page = __all_sync(0xffffffffu, off == off0 + lane % kWarpKeys * c.ss);
+        };
+        auto piece = [&](auto fast, int64_t o, int j) {
+            const int d = 16 * j + 4 * t;
+            if constexpr (decltype(fast)::value) return *reinterpret_cast<const float4*>(kh + o + d);
+            return o >= 0 && d < D ? *reinterpret_cast<const float4*>(kh + o + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+        };
+        auto load_k_as = [&](auto fast) {
+            const int64_t o0 = __shfl_sync(0xffffffffu, off, g), o1 = __shfl_sync(0xffffffffu, off, g + 8);
+#pragma unroll
+            for (int j = 0; j < kN; ++j) kx[j] = piece(fast, o0, j), ky[j] = piece(fast, o1, j);
+        };
+        auto load_k = [&] { whole ? load_k_as(std::true_type{}) : load_k_as(std::false_type{}); };
+        auto load_vs = [&] {
+            if (whole && one_page) {
+                const float* first = vh + __shfl_sync(0xffffffffu, off, 0);
+#pragma unroll
+                for (int kk = 0; kk < kWarpKeys; ++kk) load_v<true>(v[kk], first + kk * c.ss, true, lane, D);
+            } else if (whole) {
+#pragma unroll
+                for (int kk = 0; kk < kWarpKeys; ++kk)
+                    load_v<true>(v[kk], vh + __shfl_sync(0xffffffffu, off, kk), true, lane, D);
+            } else {
+#pragma unroll
+                for (int kk = 0; kk < kWarpKeys; ++kk) {
+                    const int64_t o = __shfl_sync(0xffffffffu, off, kk);
+                    load_v<false>(v[kk], vh + o, o >= 0, lane, D);
+                }
+            }
+        };
+        if constexpr (kAhead) {
+            off = offset_of(c, page, key, len);
+            locate();
+            load_k();
+            load_vs();
+            page = entry_of(c, row, key + kTile, len);
+        }
         for (int i = threadIdx.x; i < GH * kD; i += kThreads) {
             const int h = i / kD, d = i % kD;
             sm.q[h][d] = h < heads && d < D
@@ -487,39 +541,36 @@ struct AttnF32 {
         for (int h = 0; h < GH; ++h)
 #pragma unroll
             for (int x = 0; x < DV; ++x) acc[h][x] = 0.f;
-        int key = tile * kTile + warp * kWarpKeys + lane % 16;
-        int page = entry_of(c, row, key, len);
         for (int i = 0; i < tiles; ++i) {
-            const int64_t off = offset_of(c, page, key, len);
-            key += kTile;
-            if (i + 1 < tiles) page = entry_of(c, row, key, len);
+            if constexpr (!kAhead) {
+                off = offset_of(c, page, key, len);
+                locate();
+                key += kTile;
+                if (i + 1 < tiles) page = entry_of(c, row, key, len);
+            }
             const uint32_t bad = __ballot_sync(0xffffffffu, off == kBad);
             const uint32_t none = __ballot_sync(0xffffffffu, off == kNone);
             const int64_t o0 = __shfl_sync(0xffffffffu, off, g), o1 = __shfl_sync(0xffffffffu, off, g + 8);
-            // The values are on their way while the scores are taken, where the registers allow it.
-            float v[kWarpKeys][DV];
-            if constexpr (kAhead) {
-#pragma unroll
-                for (int kk = 0; kk < kWarpKeys; ++kk) load_v(v[kk], vh, __shfl_sync(0xffffffffu, off, kk), lane, D);
-            }
             float s0[GH], s1[GH];
 #pragma unroll
             for (int h = 0; h < GH; ++h) s0[h] = s1[h] = 0.f;
+            auto dots = [&](auto fast) {
 #pragma unroll
-            for (int j = 0; j < kD / 16; ++j) {
-                const int d = 16 * j + 4 * t;
-                float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-                if (d < D) {
-                    if (o0 >= 0) x = *reinterpret_cast<const float4*>(kh + o0 + d);
-                    if (o1 >= 0) y = *reinterpret_cast<const float4*>(kh + o1 + d);
-                }
+                for (int j = 0; j < kN; ++j) {
+                    const int d = 16 * j + 4 * t;
+                    const float4 x = kAhead ? kx[j] : piece(fast, o0, j), y = kAhead ? ky[j] : piece(fast, o1, j);
 #pragma unroll
-                for (int h = 0; h < GH; ++h) {
-                    const float4 w = *reinterpret_cast<const float4*>(&sm.q[h][d]);
-                    s0[h] = fmaf(x.x, w.x, fmaf(x.y, w.y, fmaf(x.z, w.z, fmaf(x.w, w.w, s0[h]))));
-                    s1[h] = fmaf(y.x, w.x, fmaf(y.y, w.y, fmaf(y.z, w.z, fmaf(y.w, w.w, s1[h]))));
+                    for (int h = 0; h < GH; ++h) {
+                        const float4 w = *reinterpret_cast<const float4*>(&sm.q[h][d]);
+                        s0[h] = fmaf(x.x, w.x, fmaf(x.y, w.y, fmaf(x.z, w.z, fmaf(x.w, w.w, s0[h]))));
+                        s1[h] = fmaf(y.x, w.x, fmaf(y.y, w.y, fmaf(y.z, w.z, fmaf(y.w, w.w, s1[h]))));
+                    }
                 }
-            }
+            };
+            if (kAhead || !whole)
+                dots(std::false_type{});
+            else
+                dots(std::true_type{});
 #pragma unroll
             for (int h = 0; h < GH; ++h) {
 #pragma unroll
@@ -528,6 +579,15 @@ struct AttnF32 {
                     s1[h] += __shfl_xor_sync(0xffffffffu, s1[h], o);
                 }
                 if (t == 0) sm.s[warp][h][g] = s0[h], sm.s[warp][h][g + 8] = s1[h];
+            }
+            const bool more = i + 1 < tiles;
+            if constexpr (!kAhead) load_vs();
+            if (kAhead && more) {
+                key += kTile;
+                off = offset_of(c, page, key, len);
+                locate();
+                load_k();
+                if (i + 2 < tiles) page = entry_of(c, row, key + kTile, len);
             }
             __syncwarp();
             float f = 1.f;
@@ -565,7 +625,6 @@ struct AttnF32 {
             }
 #pragma unroll
             for (int kk = 0; kk < kWarpKeys; ++kk) {
-                if constexpr (!kAhead) load_v(v[kk], vh, __shfl_sync(0xffffffffu, off, kk), lane, D);
 #pragma unroll
                 for (int h = 0; h < GH; ++h) {
                     const float p = sm.p[warp][kk][h];
@@ -573,6 +632,7 @@ struct AttnF32 {
                     for (int x = 0; x < DV; ++x) acc[h][x] = fmaf(p, v[kk][x], acc[h][x]);
                 }
             }
+            if (kAhead && more) load_vs();
             __syncwarp();
         }
         l += __shfl_xor_sync(0xffffffffu, l, 1);
