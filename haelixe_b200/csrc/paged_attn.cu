@@ -251,26 +251,36 @@ struct AttnBf16 {
         t = threadIdx.x % 4;
     }
 
+    // WHOLE: the step's keys are all there and of kD elements, so no load asks for anything.
+    template <bool WHOLE>
     __device__ __forceinline__ void load_k(int64_t off) {
         const int64_t o0 = __shfl_sync(0xffffffffu, off, g), o1 = __shfl_sync(0xffffffffu, off, g + 8);
+        const __nv_bfloat16 *k0 = kh + o0 + 8 * t, *k1 = kh + o1 + 8 * t;
 #pragma unroll
         for (int b = 0; b < 2 * DC; ++b) {
-            const int d = 32 * b + 8 * t;
-            const bool in = d < a.cache.D;
-            k[0][b] = in && o0 >= 0 ? ld_stream(kh + o0 + d) : make_uint4(0, 0, 0, 0);
-            k[1][b] = in && o1 >= 0 ? ld_stream(kh + o1 + d) : make_uint4(0, 0, 0, 0);
+            const bool in = WHOLE || 32 * b + 8 * t < a.cache.D;
+            k[0][b] = in && (WHOLE || o0 >= 0) ? ld_stream(k0 + 32 * b) : make_uint4(0, 0, 0, 0);
+            k[1][b] = in && (WHOLE || o1 >= 0) ? ld_stream(k1 + 32 * b) : make_uint4(0, 0, 0, 0);
         }
     }
+    template <bool WHOLE>
     __device__ __forceinline__ void load_v(int64_t off, int c0) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int64_t o = __shfl_sync(0xffffffffu, off, 2 * t + (j & 1) + 8 * (j >> 1));
+            const __nv_bfloat16* from = vh + o + 64 * c0 + 8 * g;
 #pragma unroll
-            for (int c = 0; c < VC; ++c) {
-                const int d = 64 * (c0 + c) + 8 * g;
-                v[j][c] = o >= 0 && d < a.cache.D ? ld_stream(vh + o + d) : make_uint4(0, 0, 0, 0);
-            }
+            for (int c = 0; c < VC; ++c)
+                v[j][c] = WHOLE || (o >= 0 && 64 * (c0 + c) + 8 * g < a.cache.D) ? ld_stream(from + 64 * c)
+                                                                               : make_uint4(0, 0, 0, 0);
         }
+    }
+    __device__ __forceinline__ bool is_whole(int64_t off) const {
+        return a.cache.D == kD && __all_sync(0xffffffffu, off >= 0);
+    }
+    __device__ __forceinline__ void load_k(int64_t off, bool whole) { whole ? load_k<true>(off) : load_k<false>(off); }
+    __device__ __forceinline__ void load_v(int64_t off, int c0, bool whole) {
+        whole ? load_v<true>(off, c0) : load_v<false>(off, c0);
     }
 
     __device__ __forceinline__ void run(const Part& part, Parts<HB, kD>& sp) {
@@ -306,8 +316,9 @@ struct AttnBf16 {
                     for (int r = 0; r < 4; ++r) acc[n][x][e][r] = 0.f;
         }
         int64_t off = offset_of(c, page, key, len);
-        load_k(off);
-        load_v(off, 0);
+        bool whole = is_whole(off);
+        load_k(off, whole);
+        load_v(off, 0, whole);
         page = entry_of(c, row, key + kTile, len);
         for (int i = 0; i < tiles; ++i) {
             const uint32_t bad = __ballot_sync(0xffffffffu, off == kBad);
@@ -325,22 +336,26 @@ struct AttnBf16 {
                 }
             }
             const int64_t off_now = off;
-            const bool more = i + 1 < tiles;
+            const bool more = i + 1 < tiles, whole_now = whole;
             if (more) {
                 key += kTile;
                 off = offset_of(c, page, key, len);
-                load_k(off);
+                whole = is_whole(off);
+                load_k(off, whole);
                 if (i + 2 < tiles) page = entry_of(c, row, key + kTile, len);
             }
             uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int kk = g + 8 * (r >> 1);
-                    s[n][r] *= a.scale_log2;
-                    if (bad >> kk & 1) s[n][r] = __int_as_float(0x7fffffff);
-                    if (none >> kk & 1) s[n][r] = -INFINITY;
+                for (int r = 0; r < 4; ++r) s[n][r] *= a.scale_log2;
+                if (!whole_now) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int kk = g + 8 * (r >> 1);
+                        if (bad >> kk & 1) s[n][r] = __int_as_float(0x7fffffff);
+                        if (none >> kk & 1) s[n][r] = -INFINITY;
+                    }
                 }
                 float mx[2];
 #pragma unroll
@@ -379,7 +394,7 @@ struct AttnBf16 {
             }
 #pragma unroll
             for (int c0 = 0; c0 < DC; c0 += VC) {
-                if (c0 > 0) load_v(off_now, c0);
+                if (c0 > 0) load_v(off_now, c0, whole_now);
 #pragma unroll
                 for (int x = 0; x < VC; ++x) {
                     const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&v[0][x]);
@@ -398,7 +413,7 @@ struct AttnBf16 {
                     }
                 }
             }
-            if (more) load_v(off, 0);
+            if (more) load_v(off, 0, whole);
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
