@@ -19,6 +19,8 @@
 // Ties go to the lower index.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "hx_internal.h"
 #include "launch.h"
 #include "mma_bf16.cuh"
@@ -277,15 +279,16 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(Fwd a) {
     };
     if (mine == 0 && !row.whole(0)) add_partial(0);
     const int end = row.end();
-    for (int j0 = mine < row.begin() ? mine + step : mine; j0 < end; j0 += kAhead * step) {
+    int j0 = mine < row.begin() ? mine + step : mine;
+    auto batch = [&](auto all) {  // kAhead pieces from j0 on; unless all are there, those that are
         uint4 u[kAhead];
         float top = -INFINITY;
 #pragma unroll
         for (int k = 0; k < kAhead; ++k)
-            if (j0 + k * step < end) u[k] = row.raw(j0 + k * step);
+            if (decltype(all)::value || j0 + k * step < end) u[k] = row.raw(j0 + k * step);
 #pragma unroll
         for (int k = 0; k < kAhead; ++k)
-            if (j0 + k * step < end) {
+            if (decltype(all)::value || j0 + k * step < end) {
                 const float t = RowView<T>::top(u[k]);
                 note(t, j0 + k * step);
                 top = fmaxf(top, t);
@@ -293,12 +296,14 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(Fwd a) {
         run.raise(top);
 #pragma unroll
         for (int k = 0; k < kAhead; ++k)
-            if (j0 + k * step < end) {
+            if (decltype(all)::value || j0 + k * step < end) {
                 float v[E];
                 RowView<T>::decode(u[k], v);
                 run.add(v);
             }
-    }
+    };
+    for (; j0 + (kAhead - 1) * step < end; j0 += kAhead * step) batch(std::true_type{});
+    if (j0 < end) batch(std::false_type{});
     const int last = row.pieces - 1;
     if (last > 0 && last >= end && last % step == mine) add_partial(last);
     Stats st = join_lanes<32>(run.stats());
@@ -536,20 +541,23 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_bwd_kernel(Bwd a) 
         return;
     }
     if (mine == 0 && !row.whole(0)) one(0);
-    for (int j0 = mine < row.begin() ? mine + step : mine; j0 < end; j0 += kAhead * step) {
+    int j0 = mine < row.begin() ? mine + step : mine;
+    auto batch = [&](auto all) {
         uint4 u[kAhead];
 #pragma unroll
         for (int k = 0; k < kAhead; ++k)
-            if (j0 + k * step < end) u[k] = row.raw(j0 + k * step);
+            if (decltype(all)::value || j0 + k * step < end) u[k] = row.raw(j0 + k * step);
 #pragma unroll
         for (int k = 0; k < kAhead; ++k)
-            if (j0 + k * step < end) {
+            if (decltype(all)::value || j0 + k * step < end) {
                 float v[E];
                 RowView<T>::decode(u[k], v);
                 gradient(v, row.first(j0 + k * step));
                 store_piece(out + row.first(j0 + k * step), v);
             }
-    }
+    };
+    for (; j0 + (kAhead - 1) * step < end; j0 += kAhead * step) batch(std::true_type{});
+    if (j0 < end) batch(std::false_type{});
     const int last = row.pieces - 1;
     if (last > 0 && last >= end && last % step == mine) one(last);
 }
