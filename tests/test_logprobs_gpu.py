@@ -121,6 +121,22 @@ def test_many_rows(dtype):
 
 
 @pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("rows,classes", [(1200, 5003), (1201, 20000), (160, 70001), (1185, 34007), (70, 9001)])
+def test_rows_and_lengths_of_each_kernel(dtype, rows, classes):
+    x, t = _logits(rows, classes, dtype), _targets(rows, classes)
+    _check(hx.nn.token_logprobs(x, t), x, t)
+    for k in (1, 20, 32):
+        r = hx.nn.token_logprobs(x, t, k)
+        _check(r, x, t)
+        _check_top(r, x, k)
+    # Ties all over: the slow way of putting the alternatives in order.
+    x = (x * 0.5).round()
+    r = hx.nn.token_logprobs(x, t, 32)
+    _check(r, x, t)
+    _check_top(r, x, 32)
+
+
+@pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("lead", [0, 1, 3, 8])
 def test_rows_cut_from_a_wider_buffer(dtype, lead):
     """What surrounds the rows is NaN, and each row starts at its own offset from a 16-byte boundary."""
