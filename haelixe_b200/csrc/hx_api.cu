@@ -7,6 +7,8 @@
 #include <string.h>
 
 #include <algorithm>
+#include <initializer_list>
+#include <utility>
 
 #include <cublas_v2.h>
 #include <nvtx3/nvToolsExt.h>
@@ -712,6 +714,28 @@ static int validate_cache(const hx_ctx* ctx, hx_dtype dt, const hx_paged_cache* 
     return HX_OK;
 }
 
+// Whether rows of `inner` elements that two or three strides place may overlap. A dimension of
+// size 1 places nothing.
+static bool rows_overlap(int64_t inner, std::initializer_list<std::pair<int64_t, int64_t>> strides_sizes) {
+    std::pair<int64_t, int64_t> dims[3];
+    int n = 0;
+    for (const auto& d : strides_sizes)
+        if (d.second > 1) dims[n++] = d;
+    std::sort(dims, dims + n);
+    for (int i = 0; i < n; ++i) {
+        if (dims[i].first < inner) return true;
+        inner += dims[i].first * (dims[i].second - 1);
+    }
+    return false;
+}
+static bool operand_overlaps(const hx_rows& r, int rows, int heads, int D) {
+    return rows_overlap(D, {{r.stride_row, rows}, {r.stride_head, heads}});
+}
+// Whether two operands that start at the same address are laid out differently.
+static bool clash(const hx_rows& a, const hx_rows& b, int rows, int heads) {
+    return a.data == b.data && ((rows > 1 && a.stride_row != b.stride_row) || (heads > 1 && a.stride_head != b.stride_head));
+}
+
 static hx::PagedView view_of(const hx_paged_cache& c) {
     hx::PagedView v;
     v.k = c.k;
@@ -746,6 +770,11 @@ int hx_paged_append(hx_ctx* c, hx_dtype dt, const hx_paged_cache* cache, int tok
     if (!k || !v || !k->data || !v->data || !seq_ids || !positions ||
         (Hq > 0 && (!q || !q_out || !q->data || !q_out->data)))
         return set_error(c, HX_ERR_INVALID, "%s: NULL operand", who);
+    if (rows_overlap(cache->D, {{cache->stride_head, cache->H}, {cache->stride_slot, cache->page_size},
+                                {cache->stride_page, cache->num_pages}}))
+        return set_error(c, HX_ERR_INVALID, "%s: rows of the cache share memory, so they cannot be written", who);
+    if (Hq > 0 && (operand_overlaps(*q_out, tokens, Hq, cache->D) || clash(*q, *q_out, tokens, Hq)))
+        return set_error(c, HX_ERR_INVALID, "%s: rows of q_out overlap each other, or q at other strides", who);
     DeviceGuard g(c->device);
     NvtxRange nv(who);
     LaunchCount lc(c);
@@ -796,6 +825,8 @@ int hx_paged_attention(hx_ctx* c, hx_dtype dt, const hx_paged_cache* cache, int 
     const int64_t eb = dt == HX_F32 ? 4 : 2;
     if (!aligned16(q->data) || (q->stride_row * eb) % 16 || (q->stride_head * eb) % 16)
         return set_error(c, HX_ERR_INVALID, "%s: q and its strides must be 16-byte aligned", who);
+    if (operand_overlaps(*o, cache->num_seqs, Hq, cache->D) || clash(*q, *o, cache->num_seqs, Hq))
+        return set_error(c, HX_ERR_INVALID, "%s: rows of o overlap each other, or q at other strides", who);
     DeviceGuard g(c->device);
     NvtxRange nv(who);
     LaunchCount lc(c);
@@ -973,6 +1004,8 @@ static int w4_args(hx_ctx* c, hx_dtype dt, int rows, int in, int out, int group,
     if (group <= 0 || group % 32)
         return set_error(c, HX_ERR_INVALID, "%s: group %d is not a multiple of 32", who, group);
     if (rows > 16 * 65535) return set_error(c, HX_ERR_UNSUPPORTED, "%s: more than %d rows", who, 16 * 65535);
+    if (in > 1 << 30 || out > 1 << 30 || group > 1 << 30)
+        return set_error(c, HX_ERR_UNSUPPORTED, "%s: in, out and group must be <= 2^30", who);
     return HX_OK;
 }
 
@@ -1160,6 +1193,8 @@ int hx_token_logprobs_bwd(hx_ctx* c, hx_dtype dt, const void* logits, int64_t ro
         return st;
     if (rows == 0) return HX_OK;
     if (!logits || !targets || !stats || !dlogits) return set_error(c, HX_ERR_INVALID, "%s: NULL operand", who);
+    if (logits == dlogits && rows > 1 && row_stride != drow_stride)
+        return set_error(c, HX_ERR_INVALID, "%s: dlogits over the logits needs their stride", who);
     DeviceGuard g(c->device);
     NvtxRange nv(who);
     LaunchCount lc(c);

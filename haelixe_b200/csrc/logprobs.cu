@@ -572,7 +572,7 @@ cudaError_t launch_fwd(cudaStream_t st, int sm_count, Fwd a, int rows) {
     // A warp a row: always where a CTA would have nothing to do for most of its threads, and up to
     // kWarpPieces pieces where the rows fill the GPU all the same.
     if (pieces <= 64 || (pieces <= kWarpPieces && rows >= 8 * sm_count))
-        return launch_overlapped(st, token_logprobs_warp_kernel<T, TOP>, dim3((unsigned)((rows + kWarps - 1) / kWarps)),
+        return launch_overlapped(st, token_logprobs_warp_kernel<T, TOP>, dim3(((unsigned)rows + kWarps - 1) / kWarps),
                                  kThreads, 0, 0, a, rows);
     a.splits = 1;
     while (a.splits < 8 && rows * (int64_t)a.splits < sm_count && pieces > kThreads * a.splits) a.splits *= 2;
@@ -609,7 +609,7 @@ cudaError_t token_logprobs_bwd(cudaStream_t st, int sm_count, hx_dtype dt, const
                                const float* g_entropy, void* dlogits, int64_t dstride, int rows, int classes) {
     const Bwd a{logits, dlogits, stride, dstride, targets, stats, g_logprob, g_entropy, classes};
     const int pieces = (int)(((int64_t)classes * (dt == HX_F32 ? 4 : 2) + 15) / 16) + 1;
-    int splits = (4 * sm_count + rows - 1) / rows;  // few rows: several CTAs each
+    int splits = (int)((4ll * sm_count + rows - 1) / rows);  // few rows: several CTAs each
     const int most = (pieces + kThreads - 1) / kThreads;
     if (splits > most) splits = most;
     const dim3 grid((unsigned)rows, (unsigned)splits);

@@ -127,7 +127,7 @@ cudaError_t launch(cudaStream_t st, int sm_count, const PagedAppend& a, int toke
     // One CTA a token; a few tokens are spread over more CTAs, so that the
     // heads of one token do not queue behind each other.
     const int total = (2 * a.cache.H + a.Hq) * (a.cache.D / 8);
-    int splits = (2 * sm_count + tokens - 1) / tokens;
+    int splits = (int)((2ll * sm_count + tokens - 1) / tokens);
     const int most = (total + kThreads - 1) / kThreads;
     if (splits > most) splits = most;
     const dim3 grid((unsigned)tokens, (unsigned)splits);

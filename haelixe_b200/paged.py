@@ -31,7 +31,7 @@ class PagedKVCache:
     view of [pages, heads, slots, head_dim] storage is as good. block_table:
     int32 [sequences, columns]; entry (s, c) is the page of positions
     [c * slots, (c + 1) * slots) of sequence s. The tensors stay the caller's:
-    their values, the table's among them, may change between calls.
+    their values, the table's among them, may change between calls, their memory may not.
     """
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor):
@@ -189,10 +189,11 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, seq_lens: torch.Tensor
                     out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None):
     """Attention of one query a sequence over its first seq_lens[s] cached positions.
 
-    q: [sequences, query heads, head_dim], query heads a multiple of the cache's;
-    seq_lens: int32 [sequences] on the device. Returns (o like q, lse f32
-    [sequences, query heads]). A length of 0 gives zeros and an lse of -inf; a
-    length past the table row, or a table entry that is no page, gives NaN. What
+    q: [sequences, query heads, head_dim], every row on a 16-byte boundary, query
+    heads a multiple of the cache's; seq_lens: int32 [sequences] on the device.
+    Returns (o like q, or out, which may be q itself; lse f32 [sequences, query
+    heads]). A length of 0 gives zeros and an lse of -inf; a length past the table
+    row, or a table entry that is no page, gives NaN. What
     the cache holds at or past seq_lens is not read.
     """
     who = "paged_attention"

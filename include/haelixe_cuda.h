@@ -257,12 +257,13 @@ typedef struct hx_rows {
  * int32). With rope_base > 0, k is rotated by its position first (the pairs of
  * hx_rope_fwd; the angle is formed in f64, so far positions keep their
  * accuracy), and q ([tokens, Hq, D]; NULL with Hq 0) is rotated into q_out
- * (which may be q itself). rope_base 0 writes k, and copies q, as they are.
+ * (which may be q itself, at its strides). rope_base 0 writes k, and copies q, as they are.
  * A token with a negative seq_id is padding: neither the cache nor its q_out
  * row is touched. A token without a slot (sequence or position outside the
  * table, an entry that is no page) writes nothing to the cache and NaN to its
  * q_out row. Two tokens of a call must not have the
- * same slot: it would hold a mixture of both. */
+ * same slot: it would hold a mixture of both; a cache whose strides give two
+ * slots or heads the same memory is refused. */
 int hx_paged_append(hx_ctx* ctx, hx_dtype dtype, const hx_paged_cache* cache, int tokens, const hx_rows* k,
                     const hx_rows* v, const int32_t* seq_ids, const int32_t* positions, int Hq, const hx_rows* q,
                     const hx_rows* q_out, float rope_base);
@@ -278,7 +279,8 @@ int hx_paged_attention_workspace_size(hx_dtype dtype, const hx_paged_cache* cach
  * gives zeros and an lse of -inf; one that is longer than its table row (or
  * than 2^31 - 256), or that reads an entry that is no page, gives NaN. Positions at or past
  * seq_lens are not read. The result does not depend on what else is in the
- * batch beyond f32 rounding, and equal calls give equal bits. workspace
+ * batch beyond rounding, and equal calls give equal bits. q and its strides
+ * (in bytes) are multiples of 16; o needs neither, and may be q itself at q's strides. workspace
  * (256-byte aligned) may be NULL, except during stream capture: the call then
  * takes it from the context's arena. Calls that overlap on the GPU need
  * workspaces of their own. */
@@ -306,9 +308,9 @@ int hx_linear_bwd(hx_ctx* ctx, hx_dtype dtype, const void* x, const void* w, con
  * of k = 8 o ... 8 o + 7, the first in the lowest 4 bits; those at or past in
  * are ignored. scales [ceil(in / group), out], b, residual and x are in
  * `dtype`; b and residual may be NULL, residual may alias y; group is a
- * multiple of 32, rows at most 16 * 65535. Sums in f32, one rounding. A weight
- * is read once for each 32 rows (16 in f32): for many rows a bf16 weight and
- * hx_linear_fwd are faster. */
+ * multiple of 32, rows at most 16 * 65535, the other sizes at most 2^30. Sums in
+ * f32, one rounding. A weight is read once for each 32 rows (16 in f32): for
+ * many rows a bf16 weight and hx_linear_fwd are faster. */
 int hx_linear_w4_fwd(hx_ctx* ctx, hx_dtype dtype, const void* x, const uint32_t* packed, const void* scales,
                      const void* b, const void* residual, void* y, int rows, int in_features, int out_features,
                      int group);
@@ -369,7 +371,7 @@ int hx_token_logprobs_fwd(hx_ctx* ctx, hx_dtype dtype, const void* logits, int64
 /* dlogits for the upstream gradients of logprob and entropy (f32 [rows]; NULL
  * for none): g_logprob (onehot - p) - g_entropy p (log p + entropy), in
  * `dtype`, every element of [rows, classes] written. dlogits may be logits
- * itself. A row whose target is >= classes gets NaN when g_logprob is given. */
+ * itself, at its stride. A row whose target is >= classes gets NaN when g_logprob is given. */
 int hx_token_logprobs_bwd(hx_ctx* ctx, hx_dtype dtype, const void* logits, int64_t row_stride,
                           const uint32_t* targets, const float* stats, const float* g_logprob,
                           const float* g_entropy, void* dlogits, int64_t drow_stride, int rows, int classes);

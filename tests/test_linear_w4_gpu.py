@@ -201,3 +201,11 @@ def test_refusals_and_empty():
     assert L.hx_linear_w4_fwd(c.handle, 1, p, None, p, None, None, p, 2, 64, 32, 32) == N.HX_ERR_INVALID
     assert L.hx_quantize_w4(c.handle, 1, p, None, p, 64, 32, 32) == N.HX_ERR_INVALID
     assert L.hx_quantize_w4(None, 1, p, p, p, 64, 32, 32) == N.HX_ERR_INVALID
+
+
+def test_sizes_past_the_limits_are_refused():
+    L, c, p = N.lib(), hx.context(), torch.zeros(64, device="cuda").data_ptr()
+    big = (1 << 30) + 32
+    for rows, i, o, group in ((1, big, 1, 32), (1, 32, big, 32), (1, 32, 32, big), (16 * 65535 + 1, 32, 32, 32)):
+        assert L.hx_linear_w4_fwd(c.handle, 0, p, p, p, None, None, p, rows, i, o, group) == N.HX_ERR_UNSUPPORTED
+    assert L.hx_quantize_w4(c.handle, 0, p, p, p, 32, 32, big) == N.HX_ERR_UNSUPPORTED

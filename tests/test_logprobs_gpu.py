@@ -377,3 +377,10 @@ def test_gradient_of_shared_rows():
     ref = Ref(row.detach().expand(4, 50), t)
     want, off = ref.grad(g, None)
     _close(row.grad, want.sum(0, keepdim=True), off.sum(0, keepdim=True) + 2.0 ** -22 * want.abs().sum(0, keepdim=True))
+
+
+def test_gradient_over_the_logits_at_another_stride_is_refused():
+    x, t = torch.randn(3, 12, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    L, c, f = N.lib(), hx.context(), torch.zeros(9, device="cuda")
+    p, q = x.data_ptr(), f.data_ptr()
+    assert L.hx_token_logprobs_bwd(c.handle, 0, p, 12, t.data_ptr(), q, q, None, p, 10, 3, 10) == N.HX_ERR_INVALID

@@ -543,3 +543,39 @@ def test_lengths_near_the_largest_integer():
     cache = hx.PagedKVCache(*(torch.zeros(1, page, 1, 8, device="cuda", dtype=BF16) for _ in range(2)), table)
     o, lse = hx.paged_attention(cache, torch.zeros(3, 1, 8, device="cuda", dtype=BF16), _lens(2**31 - 1, 5, 2**31 - 255), 1.0)
     assert torch.isnan(o[[0, 2]]).all() and (o[1] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("lens", [[40, 0, 7], [9000, 1, 333]])
+def test_attention_over_its_own_queries(dtype, lens):
+    """out may be q, for items that one worker has and for items that many share."""
+    cache, ks, vs = _filled(71, dtype, lens, 16, 2, 64)
+    q = torch.randn(len(lens), 6, 64, device="cuda", dtype=dtype, generator=_gen(72))
+    first = q.clone()
+    o, lse = hx.paged_attention(cache, q, _lens(*lens), 0.125, out=q)
+    assert o is q
+    _check(first, ks, vs, 0.125, o, lse)
+
+
+def test_outputs_that_share_memory_are_refused():
+    table = torch.zeros(2, 1, dtype=torch.int32, device="cuda")
+    k = torch.zeros(2, 16, 2, 64, device="cuda", dtype=BF16)
+    cache, lens, x = hx.PagedKVCache(k, k.clone(), table), _lens(1, 1), torch.zeros(2, 2, 64, device="cuda", dtype=BF16)
+    shared = torch.zeros(1, 2, 64, device="cuda", dtype=BF16).expand(2, 2, 64)
+    near = torch.zeros(2, 2, 128, device="cuda", dtype=BF16).as_strided((2, 2, 64), (96, 64, 1))
+    for out in (shared, near, x.transpose(0, 1)):  # the last is x at other strides
+        with pytest.raises(N.HxError):
+            hx.paged_attention(cache, x, lens, 1.0, out=out)
+        with pytest.raises(N.HxError):
+            hx.paged_append(cache, x, x, lens, lens, q=x, out_q=out)
+    # One set of keys for all heads: to read, not to write.
+    one = hx.PagedKVCache(k[:, :, :1].expand(2, 16, 2, 64), k[:, :, :1].expand(2, 16, 2, 64), table)
+    hx.paged_attention(one, x, lens, 1.0)
+    with pytest.raises(N.HxError):
+        hx.paged_append(one, x, x, lens, lens)
+    flat = torch.zeros(16, 2, 64, device="cuda", dtype=BF16).expand(2, 16, 2, 64)
+    with pytest.raises(N.HxError):
+        hx.paged_append(hx.PagedKVCache(flat, flat, table), x, x, lens, lens)
+    across = torch.empty(2, 2, 64, device="cuda", dtype=BF16).transpose(0, 1)  # strides in another order do not overlap
+    hx.paged_append(cache, x, x, _lens(0, 1), _lens(0, 1), q=x, out_q=across)
+    assert (across == 0).all()
