@@ -5,10 +5,11 @@
 // The weights' bytes bound it (half a byte for each, against 2 rows FLOP), so a
 // weight is read once for up to 32 rows and unpacking has to stay cheap: at half
 // a byte a weight the memory delivers about 90 weights a clock and SM. Two nibbles
-// become two bf16 in three instructions (0x4300 | q is 128 + q, minus 136), and the
+// become two bf16 in two instructions and a half (see Unpack), and the
 // warp's tensor product multiplies them, so that the f32 pipes only see one scale a
-// 32-deep step. The order of k inside a product is free as long as both operands
-// agree, so the weights go from a 16-byte global load (4 columns of 8 k) to fragments
+// group. 16 rows of 8192 x 8192 in groups of 64 take 15.4 us, of which reading is 5.6: bound by the
+// instructions that unpack and multiply, and by filling and joining within so short a call.
+// The order of k inside a product is free as long as both operands agree, so the weights go from a 16-byte global load (4 columns of 8 k) to fragments
 // with no shared memory. q - 8 and bf16 x are exact operands; f32 x is cut into
 // three bf16 that sum to it exactly, three products for one.
 //
@@ -45,27 +46,33 @@ struct Args {
     const void *scales, *bias, *residual;
     void* y;
     DeviceStatus* status;
-    int rows, in, out, group, group_shift;  // group_shift: log2(group), -1 when not a power of two
+    int rows, in, out, group, scale_rows;
+    int skip_rows, skip_rest;  // what the other groups of warps take between two units of one, in rows of scales and k
     bool vec_y;          // y on a boundary of 4 elements
     int wn_log, ks_log;  // log2 of the warps that share a unit, side by side, and of the cluster's size
 };
 
-// q - 8 of nibbles p and p + 4 of w, as bf16: one shift, one three-input logic operation
-// (w & nibbles | magic, both constants in registers) and one subtraction.
+// (q - 8) / 64 of nibbles p and p + 4 of w, as bf16. A nibble in the lowest 8 bits of a half, read
+// as a (denormal) bf16, is itself times 2^-133, or 2^-129 in the upper 4 bits: one logic operation
+// and one fused multiply-add, exact, and one shift for two of the four pairs. (Making 128 + q by a
+// shift and a logic operation and taking 136 from it is three for each.)
+constexpr float kWeightUnit = 64.f;
 struct Unpack {
-    uint32_t nibbles, magic, bias;
+    uint32_t low, high, minus_8;
     __device__ __forceinline__ Unpack() {
-        // Opaque to the compiler, which would split the operation to use immediates.
-        asm volatile("mov.b32 %0, 0x000f000f;" : "=r"(nibbles));
-        asm volatile("mov.b32 %0, 0x43004300;" : "=r"(magic));
-        asm volatile("mov.b32 %0, 0x43084308;" : "=r"(bias));  // 136
+        // Opaque to the compiler, so that they stay in registers.
+        asm volatile("mov.b32 %0, 0x7f007f00;" : "=r"(low));      // 2^127
+        asm volatile("mov.b32 %0, 0x7d007d00;" : "=r"(high));     // 2^123
+        asm volatile("mov.b32 %0, 0xbe00be00;" : "=r"(minus_8));  // -8 / 64
+    }
+    __device__ __forceinline__ uint32_t scaled(uint32_t bits, uint32_t by) const {
+        uint32_t u;
+        asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(u) : "r"(bits), "r"(by), "r"(minus_8));
+        return u;
     }
     __device__ __forceinline__ uint32_t operator()(uint32_t w, int p) const {
-        uint32_t u;
-        asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(u) : "r"(w >> (4 * p)), "r"(nibbles), "r"(magic));
-        const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u),
-                                         *reinterpret_cast<const __nv_bfloat162*>(&bias));
-        return *reinterpret_cast<const uint32_t*>(&v);
+        const uint32_t v = p < 2 ? w : w >> 8;
+        return p % 2 == 0 ? scaled(v & 0x000f000fu, low) : scaled(v & 0x00f000f0u, high);
     }
 };
 
@@ -267,10 +274,16 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * NT * CH <= 8 ? 2 : 1) li
         col[c] = n0 + 32 * (CH * sub + c) + column_of(g);
         if (VEC) col[c] = min(col[c], a.out - 4);
     }
-    S4<T> sc[kUnit / L][CH];
-    auto load_scales = [&](int u, int l) {
-        const int k = min(kUnitK * u + l * L * kStep, a.in - 1);
-        const T* p = (const T*)a.scales + (int64_t)(a.group_shift >= 0 ? k >> a.group_shift : k / a.group) * a.out;
+    // Steps of a pass of the inner loop, and its scales. It stays a loop: unrolled over a unit, the
+    // compiler moves so much of it ahead that registers spill (16 rows of 8192 x 8192 in groups of 64:
+    // 21.2 us).
+    constexpr int kPass = L == 1 ? 2 : L;
+    S4<T> sc[kPass / L][CH];
+    // Row of the next scales to load, and k from its first; between two units of this group of warps lie
+    // a.skip_rows rows and a.skip_rest k.
+    int scale_row = kUnitK * first / a.group, scale_rest = kUnitK * first - scale_row * a.group;
+    auto load_scales = [&](int l, bool last_of_unit) {
+        const T* p = (const T*)a.scales + (int64_t)min(scale_row, a.scale_rows - 1) * a.out;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             if constexpr (VEC) {
@@ -280,6 +293,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * NT * CH <= 8 ? 2 : 1) li
                 for (int i = 0; i < 4; ++i) sc[l][c].s[i] = col[c] + i < a.out ? p[col[c] + i] : T(0.f);
             }
         }
+        scale_rest += L * kStep + (last_of_unit ? a.skip_rest : 0);
+        scale_row += last_of_unit ? a.skip_rows : 0;
+        if (scale_rest >= a.group) scale_rest -= a.group, ++scale_row;
     };
 
     float acc[CH][2][NT][4];
@@ -302,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * NT * CH <= 8 ? 2 : 1) li
     }
     if (first < units) {
 #pragma unroll
-        for (int l = 0; l < kUnit / L; ++l) load_scales(first, l);
+        for (int l = 0; l < kPass / L; ++l) load_scales(l, (l + 1) * L == kUnit);
     }
     for (int u = first; u < units; u += stride) {
         const int i = done % kStages;
@@ -316,62 +332,67 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * NT * CH <= 8 ? 2 : 1) li
         const unsigned char* ws = stages + i * lay.stage + CH * sub * kBox + t * 128;
         const unsigned char* xs = stages + i * lay.stage + lay.w_bytes + g * 128;
         float d[CH][2][NT][4];
+#pragma unroll 1
+        for (int pass = 0; pass < kUnit / kPass; ++pass, ws += kPass * 4 * 128, xs += kPass * kStep / kBoxK * R * 128)
 #pragma unroll
-        for (int l = 0; l < kUnit; ++l) {
-            if (l % L == 0) {
+            for (int l = 0; l < kPass; ++l) {
+                if (l % L == 0) {
 #pragma unroll
-                for (int c = 0; c < CH; ++c)
+                    for (int c = 0; c < CH; ++c)
 #pragma unroll
-                    for (int m = 0; m < 2; ++m)
+                        for (int m = 0; m < 2; ++m)
 #pragma unroll
-                        for (int j = 0; j < NT; ++j)
+                            for (int j = 0; j < NT; ++j)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) d[c][m][j][e] = 0.f;
-            }
-            uint32_t b[NT][PARTS][4];
+                                for (int e = 0; e < 4; ++e) d[c][m][j][e] = 0.f;
+                }
+                uint32_t b[NT][PARTS][4];
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                X8<T> x;
-                x.load(xs + 8 * j * 128 + (l * kStep / kBoxK) * R * 128, (l * kStep % kBoxK + 8 * t) * sizeof(T) / 16, g);
-                x.words(b[j]);
-            }
-            uint32_t q[CH][4];
-#pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                const uint4 w =
-                    *reinterpret_cast<const uint4*>(ws + c * kBox + 4 * l * 128 + 16 * (column_of(g) / 4 ^ (4 * (l & 1) + t)));
-                q[c][0] = w.x, q[c][1] = w.y, q[c][2] = w.z, q[c][3] = w.w;
-            }
-            // All tiles' products of two nibble pairs before the next two: they do not wait for each other.
-#pragma unroll
-            for (int p = 0; p < 4; p += 2)
-#pragma unroll
-                for (int c = 0; c < CH; ++c)
-#pragma unroll
-                    for (int m = 0; m < 2; ++m) {
-                        const uint32_t a0 = weight(q[c][2 * m], p), a1 = weight(q[c][2 * m + 1], p);
-                        const uint32_t a2 = weight(q[c][2 * m], p + 1), a3 = weight(q[c][2 * m + 1], p + 1);
-#pragma unroll
-                        for (int j = 0; j < NT; ++j)
-#pragma unroll
-                            for (int k = PARTS - 1; k >= 0; --k)
-                                mma_bf16(d[c][m][j], a0, a1, a2, a3, b[j][k][p], b[j][k][p + 1]);
-                    }
-            if (l % L == L - 1) {
+                for (int j = 0; j < NT; ++j) {
+                    X8<T> x;
+                    x.load(xs + 8 * j * 128 + (l * kStep / kBoxK) * R * 128,
+                           (l * kStep % kBoxK + 8 * t) * sizeof(T) / 16, g);
+                    x.words(b[j]);
+                }
+                uint32_t q[CH][4];
 #pragma unroll
                 for (int c = 0; c < CH; ++c) {
-                    const S4<T> s = sc[l / L][c];
-#pragma unroll
-                    for (int m = 0; m < 2; ++m)
-#pragma unroll
-                        for (int j = 0; j < NT; ++j)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                acc[c][m][j][e] = fmaf((float)s.s[2 * m + (e >> 1)], d[c][m][j][e], acc[c][m][j][e]);
+                    const uint4 w = *reinterpret_cast<const uint4*>(
+                        ws + c * kBox + 4 * l * 128 + 16 * (column_of(g) / 4 ^ (4 * (l & 1) + t)));
+                    q[c][0] = w.x, q[c][1] = w.y, q[c][2] = w.z, q[c][3] = w.w;
                 }
-                if (u + stride < units) load_scales(u + stride, l / L);
+                // All tiles' products of two nibble pairs before the next two: they do not wait for each other.
+#pragma unroll
+                for (int p = 0; p < 4; p += 2)
+#pragma unroll
+                    for (int c = 0; c < CH; ++c)
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) {
+                            const uint32_t a0 = weight(q[c][2 * m], p), a1 = weight(q[c][2 * m + 1], p);
+                            const uint32_t a2 = weight(q[c][2 * m], p + 1), a3 = weight(q[c][2 * m + 1], p + 1);
+#pragma unroll
+                            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                                for (int k = PARTS - 1; k >= 0; --k)
+                                    mma_bf16(d[c][m][j], a0, a1, a2, a3, b[j][k][p], b[j][k][p + 1]);
+                        }
+                if (l % L == L - 1) {
+#pragma unroll
+                    for (int c = 0; c < CH; ++c) {
+                        const S4<T> s = sc[l / L][c];
+#pragma unroll
+                        for (int m = 0; m < 2; ++m)
+#pragma unroll
+                            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    acc[c][m][j][e] = fmaf((float)s.s[2 * m + (e >> 1)], d[c][m][j][e], acc[c][m][j][e]);
+                    }
+                    // Those of the next pass; past the last unit they are of no use. The unit's last ones are
+                    // loaded in its last pass but one.
+                    load_scales(l / L, l == kPass - 1 && pass == (kUnit / kPass == 1 ? 0 : kUnit / kPass - 2));
+                }
             }
-        }
         __syncwarp();  // all lanes have read the stage
         if constexpr (VEC) {
             if (lane == 0) ptx::mbar_arrive(empty(i));
@@ -440,6 +461,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * NT * CH <= 8 ? 2 : 1) li
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if (!VEC && n + e >= a.out) break;
+            v[e] *= kWeightUnit;
             if (a.bias) v[e] += (float)((const T*)a.bias)[n + e];
             if (a.residual) v[e] += (float)((const T*)a.residual)[to + e];
             y.s[e] = T(v[e]);
@@ -494,13 +516,15 @@ cudaError_t launch(cudaStream_t st, int sm_count, Args a) {
     const int units = (a.in + kUnitK - 1) / kUnitK, R = 8 * NT;
     auto tiles = [&] { return (a.out + (32 * CH << a.wn_log) - 1) / (32 * CH << a.wn_log); };
     // Two warps share a unit, or none where the columns are too few to occupy the SMs (8192 x
-    // 2048 in f32, 5 rows: 8.6 us against 12.1 with two). k is split as long as all CTAs are
-    // resident at once, two an SM, and every group keeps two units (8192 x 8192, 16 rows: 25.0 us
-    // at 128 CTAs, 19.5 at 256, 23.6 at 512).
+    // 2048 in f32, 5 rows: 7.6 us against 11.0 with two). k is split as long as all CTAs are
+    // resident at once, two an SM, and every group keeps two units (8192 x 8192, 16 rows: 16.8 us
+    // at 128 CTAs, 15.5 at 256, 19.5 at 512).
     a.wn_log = VEC ? 1 : 0;
     if (VEC && 4 * tiles() < sm_count) a.wn_log = 0;
     const int groups = kWarps >> a.wn_log;
     while (a.ks_log < 3 && tiles() << a.ks_log <= sm_count && units >= 4 * groups << a.ks_log) ++a.ks_log;
+    const int skip = ((groups << a.ks_log) - 1) * kUnitK;
+    a.skip_rows = skip / a.group, a.skip_rest = skip % a.group;
     const int bytes = Layout(R, CH, 1 << a.wn_log, sizeof(T)).total;
     static std::atomic<int> allowed[64];  // by device: the shared memory the kernel may have so far
     int dev = 0;
@@ -548,7 +572,7 @@ cudaError_t linear_w4(cudaStream_t st, int sm_count, DeviceStatus* status, hx_dt
                       const void* scales, const void* bias, const void* residual, void* y, int rows, int in, int out,
                       int group) {
     Args a{CUtensorMap{}, CUtensorMap{}, x, packed, scales, bias, residual, y, status, rows, in, out, group,
-                 (group & (group - 1)) == 0 ? __builtin_ctz((unsigned)group) : -1,
+                 (in + group - 1) / group, 0, 0,
            (uintptr_t)y % (dt == HX_F32 ? 16 : 8) == 0, 0, 0};
     const bool vec = (uintptr_t)x % 16 == 0 && (int64_t)in * (dt == HX_F32 ? 4 : 2) % 16 == 0 && (uintptr_t)packed % 16 == 0 && (uintptr_t)scales % 16 == 0 && out % 4 == 0;
     return dt == HX_F32 ? by_rows<float>(st, sm_count, a, vec) : by_rows<__nv_bfloat16>(st, sm_count, a, vec);
