@@ -6,7 +6,7 @@
 // the work has to be even over the SMs although lengths differ and are known
 // on the device alone. The (sequence, key head, up to HB of its query heads)
 // items are cut into tiles of 64 keys, the tiles of all items are numbered in a row,
-// each item's after a few empty places that stand for the time an item takes
+// each item's after an empty place that stands for the time an item takes
 // besides its keys, and every worker (a 4-warp CTA, as many as are resident at
 // once) takes an equal run of them. A run that holds all of an item writes its
 // result; the others write (max, sum, unnormalised o) to the workspace, at most
@@ -29,10 +29,10 @@ namespace {
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kWarpKeys = 16, kTile = kWarps * kWarpKeys;
 constexpr int kMaxWorkers = 1024;
-// Empty places of an item, where workers have several tiles each: 64 sequences of 1 to 8192 keys
-// take 79 us without, 52 with 2, 56 with 4. With less to do than that none, so that it is
-// spread as far as it goes.
-constexpr int kItemPlaces = 2, kPlacesFrom = 4;
+// Empty places of an item, where every worker has a tile: 64 sequences of 1 to 8192 keys take 65 us
+// without and 50 with 1 or 2; 256 of 1 to 1024 take 62 without, 51 with 1, 55 with 2, 59 with 3. With
+// less to do than that none, so that it is spread as far as it goes.
+constexpr int kItemPlaces = 1;
 constexpr float kLazy = 8.f;  // log2 growth of the maximum that triggers a rescale
 constexpr float kLn2 = 0.69314718055994530942f;
 
@@ -94,7 +94,7 @@ __device__ __forceinline__ bool find_run(const PagedAttn& a, int per, int64_t& s
         tiles += t, items += t > 0;
     }
     block_sums(tiles, items);
-    empty = tiles * per >= (int64_t)kPlacesFrom * gridDim.x ? kItemPlaces : 0;
+    empty = tiles * per >= gridDim.x ? kItemPlaces : 0;
     const int64_t total = (tiles + items * empty) * per, run = div_up(total, gridDim.x);
     const bool first = blockIdx.x == 0;
     if (first && threadIdx.x == 0) *a.plan = Plan{run, empty};
