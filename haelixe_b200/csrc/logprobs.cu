@@ -7,7 +7,7 @@
 // both, if a logit costs no more than about nine instructions, one of them the
 // exponential (7 TB/s of bf16 are 13 logits a clock and SM). So the differences,
 // products and sums run two to an instruction (f32x2), and whole 16-byte
-// pieces are loaded four ahead. The forward keeps (m, s, w) running, so the row is
+// pieces are loaded four at a time, the next four before these are added. The forward keeps (m, s, w) running, so the row is
 // read once; both terms of H are positive, so nothing cancels. Sums are f32,
 // per thread and then joined in a tree, the same for every call. A few rows are
 // split over a cluster of CTAs each, which join through distributed shared memory.
@@ -36,7 +36,7 @@ constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f
 constexpr float kLowest = -3.402823466e+38f;
 constexpr float kFloor = -1.0e4f;  // exp2 of it is 0; keeps 0 * (-inf) out of the sums
 constexpr unsigned kAll = 0xffffffffu;
-constexpr int kAhead = 4;  // pieces of a thread in flight
+constexpr int kAhead = 4;  // pieces of a thread that are loaded at once
 
 // max that keeps a NaN (fmaxf drops it).
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -232,9 +232,6 @@ struct Fwd {
     int classes, top, splits;  // splits: CTAs of a row, one cluster
 };
 
-// 8192 rows of 2500 bf16 (313 pieces) take 12 us by warps and 30 by CTAs, 1500 rows of 5000
-// (626 pieces) 9.2 and 6.7.
-constexpr int kWarpPieces = 512;
 constexpr int kHits = 128;  // logits that reach the bound, before the slow way
 
 // A CTA of THREADS a row, or of a share of it. grid: rows x splits.
@@ -281,12 +278,14 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
     if (mine == 0 && !row.whole(0)) add_partial(0);
     const int end = row.end();
     int j0 = mine < row.begin() ? mine + step : mine;
-    auto batch = [&](auto all) {  // kAhead pieces from j0 on; unless all are there, those that are
-        uint4 u[kAhead];
-        float top = -INFINITY;
+    uint4 u[kAhead];
+    auto load = [&](int j, auto all) {
 #pragma unroll
         for (int k = 0; k < kAhead; ++k)
-            if (decltype(all)::value || j0 + k * step < end) u[k] = row.raw(j0 + k * step);
+            if (decltype(all)::value || j + k * step < end) u[k] = row.raw(j + k * step);
+    };
+    auto batch = [&](auto all, auto next) {  // kAhead pieces from j0 on; unless all are there, those that are
+        float top = -INFINITY;
 #pragma unroll
         for (int k = 0; k < kAhead; ++k)
             if (decltype(all)::value || j0 + k * step < end) {
@@ -295,16 +294,26 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
                 top = fmaxf(top, t);
             }
         run.raise(top);
+        const uint4 now[kAhead] = {u[0], u[1], u[2], u[3]};
+        next();
 #pragma unroll
         for (int k = 0; k < kAhead; ++k)
             if (decltype(all)::value || j0 + k * step < end) {
                 float v[E];
-                RowView<T>::decode(u[k], v);
+                RowView<T>::decode(now[k], v);
                 run.add(v);
             }
     };
-    for (; j0 + (kAhead - 1) * step < end; j0 += kAhead * step) batch(std::true_type{});
-    if (j0 < end) batch(std::false_type{});
+    const int full = kAhead * step, tail = end - (kAhead - 1) * step;
+    if (j0 < tail) {
+        load(j0, std::true_type{});
+        for (; j0 + full < tail; j0 += full) batch(std::true_type{}, [&] { load(j0 + full, std::true_type{}); });
+        batch(std::true_type{}, [&] { load(j0 + full, std::false_type{}); });
+        j0 += full;
+    } else {
+        load(j0, std::false_type{});
+    }
+    if (j0 < end) batch(std::false_type{}, [] {});
     const int last = row.pieces - 1;
     if (last > 0 && last >= end && last % step == mine) add_partial(last);
     Stats st = join_lanes<32>(run.stats());
@@ -319,13 +328,16 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
         if (warp == 0) chosen[lane] = k;
         __syncthreads();
         const uint64_t bound = chosen[a.top - 1];
-        // The chosen threads' pieces again, each by a warp; a piece's element counts when
-        // (its order, ~its piece) reaches the bound.
+        // The chosen threads' pieces again, a thread's by so many lanes as it has pieces; a piece's element
+        // counts when (its order, ~its piece) reaches the bound.
+        const int each = (row.pieces + step - 1) >> (__ffs(step) - 1), lanes_log = each >= 32 ? 5 : 32 - __clz(each - 1);
         auto scan = [&](auto&& take) {
-            for (int c = warp; c < a.top; c += WARPS) {
-                if (chosen[c] == 0) break;
-                for (int j0 = (int)(~(uint32_t)chosen[c] % step); j0 < row.pieces; j0 += 32 * step) {
-                    const int j = j0 + lane * step;
+            for (int c0 = warp << (5 - lanes_log); c0 < a.top; c0 += WARPS << (5 - lanes_log)) {
+                const int c = c0 + (lane >> lanes_log), j0 = (lane & ((1 << lanes_log) - 1)) * step;
+                const uint64_t chose = c < a.top ? chosen[c] : 0;
+                const int from = chose != 0 ? (int)(~(uint32_t)chose & (uint32_t)(step - 1)) + j0 : row.pieces;
+                for (int n = 0; n < each; n += 1 << lanes_log) {
+                    const int j = from + n * step;
                     float v[E];
                     if (j < row.pieces) row.load(j, v, -INFINITY);
 #pragma unroll
@@ -565,29 +577,34 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_bwd_kernel(Bwd a) 
 
 template <typename T, bool TOP>
 cudaError_t launch_fwd(cudaStream_t st, int sm_count, Fwd a, int rows) {
-    // Rows that do not occupy the SMs are split over a cluster each, as long as every thread keeps
-    // a piece. More splits only repeat the joins (515 rows of 131071 f32 with 20
-    // alternatives: 70 us whole, 72 in two, 103 in eight).
     const int pieces = (int)(((int64_t)a.classes * (int)sizeof(T) + 15) / 16) + 1;
-    // A warp a row: always where a CTA would have nothing to do for most of its threads, and up to
-    // kWarpPieces pieces where the rows fill the GPU all the same.
-    if (pieces <= 64 || (pieces <= kWarpPieces && rows >= 8 * sm_count))
+    const bool many = rows >= 8 * sm_count;  // enough for every place on the SMs
+    // A warp a row where a CTA's joins would cost more than its threads gain: 8192 rows of 1200 bf16 (151
+    // pieces) take 9.3 us by warps and 13.3 by 128 threads, of 2500 15.4 and 17.9; with 5 alternatives,
+    // whose list costs a warp more, of 800 26.8 and 31.5, of 1800 40.8 and 33.0. A few hundred rows
+    // are better off with CTAs (300 of 400: 2.4 and 2.2 us, with alternatives 7.8 and 4.6) unless they are
+    // very short (of 50: 2.4 and 2.9).
+    if (pieces <= (many ? TOP ? 128 : 256 : TOP ? 0 : 32))
         return launch_overlapped(st, token_logprobs_warp_kernel<T, TOP>, dim3(((unsigned)rows + kWarps - 1) / kWarps),
                                  kThreads, 0, 0, a, rows);
     a.splits = 1;
-    while (a.splits < 8 && rows * (int64_t)a.splits < sm_count && pieces > kThreads * a.splits) a.splits *= 2;
-    // Rows enough for every place on the SMs: smaller CTAs, whose joins cost less (8192 rows of 5000
-    // bf16: 22 us against 30, with 20 alternatives 80 against 102; of 32000: 92 against 100), up
-    // to 4096 pieces. Very long rows with alternatives: larger ones, so that less of the row is looked
-    // at again (515 rows of 131071 f32 with 20: 62 us against
-    // 70).
-    if (rows >= 8 * sm_count && pieces <= 4096)
+    // Smaller CTAs join for less, as long as they are enough to load what the bandwidth allows: 8192
+    // rows of 5000 bf16 take 22 us by 128 threads and 31 by 256, with 20 alternatives 53 and 74; of 32000
+    // 89 and 94, 145 and 157; of 65000 with alternatives 291 and 251. 600 rows of 5000 with 5 alternatives take
+    // 7.9 and 9.5 us, 600 of 16000 without 8.6 and 6.9.
+    if (pieces <= (many ? 4096 : rows >= sm_count ? 1024 : kThreads))
         return launch_overlapped(st, token_logprobs_kernel<T, TOP, kThreads / 2>, dim3((unsigned)rows), kThreads / 2, 0, 0, a);
+    // Very long rows with alternatives: larger ones, so that less of the row is looked at again (515
+    // rows of 131071 f32 with 20: 57 us against 62).
     if constexpr (TOP) {
         if (rows >= sm_count && pieces > 8192)
             return launch_overlapped(st, token_logprobs_kernel<T, TOP, 2 * kThreads>, dim3((unsigned)rows), 2 * kThreads, 0,
                                      0, a);
     }
+    // Rows that do not occupy the SMs are split over a cluster each, as long as every thread keeps
+    // a piece. More splits only repeat the joins (515 rows of 131071 f32 with 20
+    // alternatives: 62 us whole, 64 in two, 91 in eight).
+    while (a.splits < 8 && rows * (int64_t)a.splits < sm_count && pieces > kThreads * a.splits) a.splits *= 2;
     return launch_overlapped(st, token_logprobs_kernel<T, TOP, kThreads>, dim3((unsigned)rows * (unsigned)a.splits),
                              kThreads, 0, a.splits > 1 ? a.splits : 0, a);
 }

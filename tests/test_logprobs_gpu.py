@@ -384,3 +384,9 @@ def test_gradient_over_the_logits_at_another_stride_is_refused():
     L, c, f = N.lib(), hx.context(), torch.zeros(9, device="cuda")
     p, q = x.data_ptr(), f.data_ptr()
     assert L.hx_token_logprobs_bwd(c.handle, 0, p, 12, t.data_ptr(), q, q, None, p, 10, 3, 10) == N.HX_ERR_INVALID
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("rows,classes", [(1300, 300), (1300, 1000), (1300, 2100), (700, 5003), (150, 4001), (40, 400), (600, 60), (1, 129)])
+def test_rows_and_lengths_where_the_kernel_changes(dtype, rows, classes):
+    test_rows_and_lengths_of_each_kernel(dtype, rows, classes)
