@@ -7,8 +7,8 @@
 // both, if a logit costs no more than about nine instructions, one of them the
 // exponential (7 TB/s of bf16 are 13 logits a clock and SM). So the differences,
 // products and sums run two to an instruction (f32x2), and whole 16-byte
-// pieces are loaded four at a time, the next four before these are added. The forward keeps (m, s, w) running, so the row is
-// read once; both terms of H are positive, so nothing cancels. Sums are f32,
+// pieces are loaded four at a time, in the forward the next four before these are
+// added. It keeps (m, s, w) running, so the row is read once; both terms of H are positive, so nothing cancels. Sums are f32,
 // per thread and then joined in a tree, the same for every call. A few rows are
 // split over a cluster of CTAs each, which join through distributed shared memory.
 //
