@@ -15,6 +15,7 @@ on its thread's current stream.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional
 
 import torch
@@ -101,16 +102,14 @@ class PagedKVCache:
 
 
 # The calls are made once a layer and token, so their checks are kept to a few
-# attribute reads. Operands go to the library as hx_rows (address, stride of a row,
-# stride of a head), side by side in one array.
-_Rows2, _Rows4 = ctypes.c_int64 * 6, ctypes.c_int64 * 12
-_ROWS = ctypes.sizeof(N.Rows)
+# attribute reads. Operands go to the library as hx_rows: address, stride of a row, stride of a
+# head, packed into bytes, which cost a fraction of a ctypes structure.
+_pack_rows = struct.Struct("Pqq").pack
 
 
-def _rows(cache: PagedKVCache, who: str, name: str, t: torch.Tensor, rows: int, heads: int):
-    shape = t.shape
-    if len(shape) != 3 or shape[0] != rows or shape[1] != heads or shape[2] != cache.head_dim:
-        raise ValueError(f"{who}: {name} must be [{rows}, {heads}, {cache.head_dim}], got {tuple(shape)}")
+def _rows(cache: PagedKVCache, who: str, name: str, t: torch.Tensor, rows: int, heads: int) -> bytes:
+    if t.shape != (rows, heads, cache.head_dim):
+        raise ValueError(f"{who}: {name} must be [{rows}, {heads}, {cache.head_dim}], got {tuple(t.shape)}")
     if t.dtype is not cache.dtype or t.get_device() != cache._dev:
         raise ValueError(f"{who}: {name} must have the cache's dtype and device")
     s0, s1, s2 = t.stride()
@@ -121,7 +120,7 @@ def _rows(cache: PagedKVCache, who: str, name: str, t: torch.Tensor, rows: int, 
         s1 = cache.head_dim
     if rows == 1:
         s0 = heads * s1
-    return t.data_ptr(), s0, s1
+    return _pack_rows(t.data_ptr(), s0, s1)
 
 
 def _indices(cache: PagedKVCache, who: str, name: str, t: torch.Tensor, n: int) -> int:
@@ -166,20 +165,15 @@ def paged_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, seq_ids:
         qr = _rows(cache, who, "q", q, n, heads)
         if out_q is None:
             out_q = torch.empty_like(q)
-        rows = _Rows4(*kr, *vr, *qr, *_rows(cache, who, "out_q", out_q, n, heads))
-        at = ctypes.addressof(rows)
-        q_at, out_at = at + 2 * _ROWS, at + 3 * _ROWS
+        outr = qr if out_q is q else _rows(cache, who, "out_q", out_q, n, heads)
     else:
         if out_q is not None:
             raise ValueError("paged_append: out_q without q")
-        rows = _Rows2(*kr, *vr)
-        at = ctypes.addressof(rows)
-        heads, q_at, out_at = 0, None, None
+        heads, qr, outr = 0, None, None
     ctx = cache._ctx
     with ctx.lock:
         ctx.use_stream()
-        st = N.lib().hx_paged_append(ctx.handle, cache._dt, cache._ref, n, at, at + _ROWS, ids, pos, heads, q_at, out_at,
-                                     base)
+        st = N.lib().hx_paged_append(ctx.handle, cache._dt, cache._ref, n, kr, vr, ids, pos, heads, qr, outr, base)
         if st:
             N.check(st, ctx.handle)
     return out_q
@@ -205,19 +199,18 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, seq_lens: torch.Tensor
     need = cache.workspace_bytes(heads)
     if out is None:
         out = torch.empty_like(q)
-    rows = _Rows2(*qr, *_rows(cache, who, "out", out, n, heads))
+    outr = qr if out is q else _rows(cache, who, "out", out, n, heads)
     if lse is None:
         lse = q.new_empty((n, heads), dtype=torch.float32)
     elif lse.shape != (n, heads) or lse.dtype is not torch.float32 or lse.get_device() != cache._dev or not lse.is_contiguous():
         raise ValueError("paged_attention: lse must be a contiguous f32 [sequences, query heads]")
     # A tensor of the current stream, so that calls on other streams and captured graphs have their own.
     ws = q.new_empty(need, dtype=torch.uint8)
-    at = ctypes.addressof(rows)
     ctx = cache._ctx
     with ctx.lock:
         ctx.use_stream()
-        st = N.lib().hx_paged_attention(ctx.handle, cache._dt, cache._ref, heads, at, at + _ROWS, lse.data_ptr(), lens,
-                                        scale, ws.data_ptr(), need)
+        st = N.lib().hx_paged_attention(ctx.handle, cache._dt, cache._ref, heads, qr, outr, lse.data_ptr(), lens, scale,
+                                        ws.data_ptr(), need)
         if st:
             N.check(st, ctx.handle)
     return out, lse
