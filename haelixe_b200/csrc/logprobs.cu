@@ -260,9 +260,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
     Running run;
     float best_v = -INFINITY;
     int best_j = -1;
-    auto note = [&](float top, int j) {  // a piece's largest logit
+    auto note = [&](float top, int j) {  // a piece's largest logit; NaN, of a piece of nothing else, ranks as -inf
         if constexpr (TOP) {
-            if (top > best_v || best_j < 0) best_j = j, best_v = top;
+            if (top > best_v || best_j < 0) best_j = j, best_v = fmaxf(top, -INFINITY);
         }
     };
     auto add_partial = [&](int j) {

@@ -390,3 +390,21 @@ def test_gradient_over_the_logits_at_another_stride_is_refused():
 @pytest.mark.parametrize("rows,classes", [(1300, 300), (1300, 1000), (1300, 2100), (700, 5003), (150, 4001), (40, 400), (600, 60), (1, 129)])
 def test_rows_and_lengths_where_the_kernel_changes(dtype, rows, classes):
     test_rows_and_lengths_of_each_kernel(dtype, rows, classes)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("rows,classes", [(5, 5003), (1, 131072), (160, 20000), (1200, 5003), (1300, 300), (515, 131071)])
+def test_pieces_made_of_nan(dtype, rows, classes):
+    """Whole 16-byte pieces of NaN, among them the first that a thread reads, with the likeliest classes in later
+    pieces of the same threads (every kernel steps by a power of two of pieces): NaN ranks as -inf."""
+    E = 8 if dtype == BF16 else 4
+    x = _logits(rows, classes, dtype)
+    x[:, :41 * E] = float("nan")
+    for r in range(min(rows, 6)):
+        at = torch.arange(5 * E + E // 2, classes, (32 << r) * E, device="cuda")[1:]
+        x[r, at] = 20 + torch.arange(len(at), device="cuda").to(dtype)
+    t = _targets(rows, classes)
+    for k in (1, 20):
+        r = hx.nn.token_logprobs(x, t, k)
+        assert torch.equal(r.top_ids.long(), _order(x)[:, :k])
+        assert torch.isnan(r.logprob).all() and torch.isnan(r.entropy).all() and torch.isnan(r.top_logprobs).all()
