@@ -176,6 +176,12 @@ __device__ __forceinline__ float ex2(float x) {
     return r;
 }
 
+// Bits whose upper half is the largest bf16 below p > 0; 0 of 0, NaN of NaN.
+__device__ __forceinline__ uint32_t below(float p) {
+    const uint32_t u = __float_as_uint(p);
+    return u - min(u, 1u);
+}
+
 // Joins the four warps' parts: the item's output, or the worker's part of it. Four elements a thread.
 template <typename T, int HB, int DP>
 __device__ __forceinline__ void finish_item(const PagedAttn& a, const Parts<HB, DP>& sp, const Item& it, bool whole,
@@ -229,7 +235,9 @@ __device__ __forceinline__ void finish_item(const PagedAttn& a, const Parts<HB, 
 // use the same one, so lane t's 16 bytes of a key row are its columns of two products,
 // and V^T pairs the keys 2t, 2t+1 by two byte permutes. P goes from the first product's
 // layout to the second's by an 8x8 transpose, as bf16 hi + lo, so that the
-// result carries only its own rounding.
+// result carries only its own rounding. hi is the largest bf16 below p, not the nearest, and so lo is
+// more than 0: both products with an infinite value then are that infinity (0 times it, or less than 0,
+// would make NaN of it, for weights above 2^-110).
 // K of the next step is loaded as soon as the scores are taken, V as soon as P V is,
 // so one of the two is always in flight. (Loading the worker's next item's while one is joined
 // and stored gained nothing: the SM's other workers are in the middle of theirs.)
@@ -386,7 +394,7 @@ struct AttnBf16 {
                     const float p0 = ex2(s[n][2 * r] - m0), p1 = ex2(s[n][2 * r + 1] - m1);
                     l[n][0] += p0;
                     l[n][1] += p1;
-                    const uint32_t hi = pack_bf16(p0, p1);
+                    const uint32_t hi = pair_hi(below(p0), below(p1));
                     const float2 back = unpack_bf16(hi);
                     ph[n][r] = transpose8x8(hi);
                     pl[n][r] = transpose8x8(pack_bf16(p0 - back.x, p1 - back.y));

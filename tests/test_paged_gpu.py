@@ -579,3 +579,35 @@ def test_outputs_that_share_memory_are_refused():
     across = torch.empty(2, 2, 64, device="cuda", dtype=BF16).transpose(0, 1)  # strides in another order do not overlap
     hx.paged_append(cache, x, x, _lens(0, 1), _lens(0, 1), q=x, out_q=across)
     assert (across == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("dim,group", [(64, 2), (128, 12), (256, 1)])
+def test_infinite_values_keep_their_sign(dtype, dim, group):
+    """An infinite value makes its element infinite whatever its weight (from 1 to 2^-86 here); both signs, or NaN, give NaN."""
+    inf, nan = float("inf"), float("nan")
+    lens = [1, 200, 200, 5000, 200, 90]
+    cache, ks, vs = _filled(81, dtype, lens, 16, 1, dim)
+    t = cache.block_table.long()
+    q = torch.randn(len(lens), group, dim, generator=_gen(82), device="cuda", dtype=dtype)
+    q[1] = 0  # equal weights, each one bf16 number exactly
+    q[5] = 0
+    q[5, :, 0] = 1
+    k = ks[5].clone()
+    k[:, 0, 0] = 0
+    k[7, 0, 0] = -60.0 * dim ** 0.5  # this key weighs e^-60 of the others
+    j = torch.arange(90, device="cuda")
+    cache.k[t[5][j // 16], j % 16], ks[5] = k, k
+    for s, at, d, value in [(0, 0, 3, inf), (1, 150, 3, inf), (1, 0, 9, -inf), (2, 150, 3, inf), (2, 77, 9, -inf),
+                            (2, 150, 17, nan), (3, 4321, 3, inf), (3, 0, 9, -inf), (3, 17, 21, inf), (3, 4900, 21, -inf),
+                            (4, 10, 21, inf), (4, 20, 21, -inf), (5, 7, 3, inf), (5, 7, 9, -inf)]:
+        cache.v[t[s, at // 16], at % 16, 0, d] = value
+        vs[s][at, 0, d] = value
+    o, lse = hx.paged_attention(cache, q, _lens(*lens), dim ** -0.5)
+    want, rl, off, off_lse = _reference(q, ks, vs, dim ** -0.5)
+    assert torch.equal(torch.isnan(o), torch.isnan(want))
+    assert torch.equal(torch.isinf(o), torch.isinf(want)) and torch.isinf(want).sum() == group * 9
+    assert torch.equal(o[torch.isinf(want)].double(), want[torch.isinf(want)])
+    live = torch.isfinite(want)
+    assert ((o.double() - want).abs() <= torch.finfo(dtype).eps / 2 * (want.abs() + off) + off)[live].all()
+    assert ((lse.double() - rl).abs() <= off_lse + 2.0 ** -24 * rl.abs()).all()
