@@ -33,7 +33,11 @@ constexpr int kMaxWorkers = 1024;
 // without and 50 with 1 or 2; 256 of 1 to 1024 take 62 without, 51 with 1, 55 with 2, 59 with 3. With
 // less to do than that none, so that it is spread as far as it goes.
 constexpr int kItemPlaces = 1;
-constexpr float kLazy = 8.f;  // log2 growth of the maximum that triggers a rescale
+constexpr int kLazy = 8;  // log2 growth of the maximum that triggers a rescale
+// The weights of the values are 2^shrink_of(len) of the probabilities, so that they add up to less than 1
+// and no sum passes the largest value, however large that is; the division by the probabilities' sum takes it
+// back. A power of two, so it changes no bit of a result unless values are under 2^-100 or so.
+__device__ __forceinline__ int shrink_of(int len) { return __clz(len) - 32 - kLazy; }
 constexpr float kLn2 = 0.69314718055994530942f;
 
 struct Item {
@@ -185,7 +189,7 @@ __device__ __forceinline__ uint32_t below(float p) {
 // Joins the four warps' parts: the item's output, or the worker's part of it. Four elements a thread.
 template <typename T, int HB, int DP>
 __device__ __forceinline__ void finish_item(const PagedAttn& a, const Parts<HB, DP>& sp, const Item& it, bool whole,
-                                            int slot) {
+                                            int len, int slot) {
     const int D = a.cache.D, quads = D / 4;
     const int h0 = it.h * a.G + it.c * HB;
     const int heads = min(HB, a.G - it.c * HB);
@@ -211,7 +215,7 @@ __device__ __forceinline__ void finish_item(const PagedAttn& a, const Parts<HB, 
                 T v[4];
             } four;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) four.v[e] = T(o[e] / l);
+            for (int e = 0; e < 4; ++e) four.v[e] = T(o[e] / l * exp2f((float)-shrink_of(len)));
             if (a.o_vec) {
                 *reinterpret_cast<Four*>(to) = four;
             } else {
@@ -237,7 +241,7 @@ __device__ __forceinline__ void finish_item(const PagedAttn& a, const Parts<HB, 
 // layout to the second's by an 8x8 transpose, as bf16 hi + lo, so that the
 // result carries only its own rounding. hi is the largest bf16 below p, not the nearest, and so lo is
 // more than 0: both products with an infinite value then are that infinity (0 times it, or less than 0,
-// would make NaN of it, for weights above 2^-110).
+// would make NaN of it; it still does for weights under 2^-110 of 1).
 // K of the next step is loaded as soon as the scores are taken, V as soon as P V is,
 // so one of the two is always in flight. (Loading the worker's next item's while one is joined
 // and stored gained nothing: the SM's other workers are in the middle of theirs.)
@@ -323,6 +327,7 @@ struct AttnBf16 {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) acc[n][x][e][r] = 0.f;
         }
+        const float shrink = exp2f((float)shrink_of(len));
         int64_t off = offset_of(c, page, key, len);
         bool whole = is_whole(off);
         load_k(off, whole);
@@ -372,7 +377,7 @@ struct AttnBf16 {
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], o));
                 }
-                if (__any_sync(0xffffffffu, mx[0] > m[n][0] + kLazy || mx[1] > m[n][1] + kLazy)) {
+                if (__any_sync(0xffffffffu, mx[0] > m[n][0] + (float)kLazy || mx[1] > m[n][1] + (float)kLazy)) {
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         const float mn = fmaxf(m[n][r], mx[r]);
@@ -391,9 +396,10 @@ struct AttnBf16 {
                 const float m0 = safe_max(m[n][0]), m1 = safe_max(m[n][1]);
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const float p0 = ex2(s[n][2 * r] - m0), p1 = ex2(s[n][2 * r + 1] - m1);
+                    float p0 = ex2(s[n][2 * r] - m0), p1 = ex2(s[n][2 * r + 1] - m1);
                     l[n][0] += p0;
                     l[n][1] += p1;
+                    p0 *= shrink, p1 *= shrink;
                     const uint32_t hi = pair_hi(below(p0), below(p1));
                     const float2 back = unpack_bf16(hi);
                     ph[n][r] = transpose8x8(hi);
@@ -558,6 +564,7 @@ struct AttnF32 {
         // max and sum of head lane / 4 (the same in its four lanes, the sum after the loop)
         const int hs = lane / 4;
         const bool has = hs < GH;
+        const float shrink = exp2f((float)shrink_of(len));
         float m = -INFINITY, l = 0.f;
         float acc[GH][DV];
 #pragma unroll
@@ -635,7 +642,7 @@ struct AttnF32 {
                 for (int r = 0; r < 4; ++r) {
                     const float p = exp2f(s[r] - safe_max(m));
                     l += p;
-                    sm.p[warp][4 * t + r][hs] = p;
+                    sm.p[warp][4 * t + r][hs] = p * shrink;
                 }
                 if (t == 0) sm.f[warp][hs] = f;
             }
@@ -710,7 +717,7 @@ __device__ __forceinline__ void paged_worker(const PagedAttn& a, W& w, Parts<W::
     for (Part part = next_part(); part.count; part = next_part()) {
         w.run(part, sp);
         __syncthreads();
-        finish_item<T, W::HB, W::kD>(a, sp, part.it, part.whole, part.slot);
+        finish_item<T, W::HB, W::kD>(a, sp, part.it, part.whole, part.len, part.slot);
         __syncthreads();
     }
 }
@@ -815,7 +822,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(PagedAttn a
 #pragma unroll
         for (int w = 0; w < kJoinWarps; ++w)
             if (w < warps) s += f[w] * so[w][d];
-        o[d] = T(s / l);
+        o[d] = T(s / l * exp2f((float)-shrink_of(a.lens[n])));
     }
     if (threadIdx.x == 0 && lse) *lse = (m + log2f(l)) * kLn2;
 }

@@ -611,3 +611,25 @@ def test_infinite_values_keep_their_sign(dtype, dim, group):
     live = torch.isfinite(want)
     assert ((o.double() - want).abs() <= torch.finfo(dtype).eps / 2 * (want.abs() + off) + off)[live].all()
     assert ((lse.double() - rl).abs() <= off_lse + 2.0 ** -24 * rl.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("dim,group", [(64, 1), (128, 4), (128, 12), (256, 1)])
+@pytest.mark.parametrize("lens", [[1, 40, 700], [30000, 5]])
+def test_values_near_the_largest(dtype, dim, group, lens):
+    """The result is a mean of the values, so it is finite where they are, however large: sums of weights
+    that are not yet divided by their total must not overflow."""
+    cache, ks, vs = _filled(83, dtype, lens, 16, 2, dim)
+    t = cache.block_table.long()
+    for s, n in enumerate(lens):
+        j = torch.arange(n, device="cuda")
+        # Of one sign in every second element, of both in the others; keys that score ever higher in sequence 0.
+        v = (1 + torch.rand(n, 2, dim, generator=_gen(84 + s), device="cuda")) * 2.0 ** 126
+        v[..., 1::2] *= torch.sign(torch.randn(n, 2, dim // 2, generator=_gen(94 + s), device="cuda"))
+        vs[s] = v.to(dtype)
+        cache.v[t[s][j // 16], j % 16] = vs[s]
+    q = torch.randn(len(lens), 2 * group, dim, generator=_gen(85), device="cuda", dtype=dtype)
+    o, lse = hx.paged_attention(cache, q, _lens(*lens), 4 * dim ** -0.5)
+    _check(q, ks, vs, 4 * dim ** -0.5, o, lse)
+    again = hx.paged_attention(cache, q, _lens(*lens), 4 * dim ** -0.5)
+    assert torch.equal(o, again[0]) and torch.equal(lse, again[1])
