@@ -25,10 +25,18 @@ import threading
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 
 _DTYPES = {torch.float32: N.HX_F32, torch.bfloat16: N.HX_BF16}
+
+
+def has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether one of them is a dual tensor of forward-mode differentiation, which requires_grad does not
+    show. (Outside a dual level none is, and one attribute is read.)"""
+    return forward_ad._current_level >= 0 and \
+        any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 class CudaAllocation:

@@ -25,7 +25,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _native as N
-from .attention import _DTYPES, context, flash_attention
+from .attention import _DTYPES, context, flash_attention, has_tangent
 from .paged import PagedKVCache, paged_append, paged_attention
 
 
@@ -290,7 +290,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0) 
     top_k = int(top_k)
     if not 0 <= top_k <= min(32, logits.shape[1]):
         raise ValueError("top_k must be 0 to 32 and at most the number of classes")
-    if logits.requires_grad and torch.is_grad_enabled():
+    # A dual tensor goes there too: autograd refuses it, for there is no forward-mode derivative.
+    if logits.requires_grad and torch.is_grad_enabled() or has_tangent(logits):
         return TokenLogprobs(*_TokenLogprobsFn.apply(logits, flat, top_k))
     return TokenLogprobs(*_token_logprobs(logits, flat, top_k, False)[:4])
 
@@ -324,6 +325,8 @@ def linear_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, group
     if torch.is_grad_enabled() and (x.requires_grad or scales.requires_grad or (bias is not None and bias.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
         raise RuntimeError("linear_w4 has no backward: call it under torch.no_grad()")
+    if has_tangent(x, scales, bias, residual):
+        raise RuntimeError("linear_w4 has no forward-mode derivative")
     c = _context_of(x)
     lead, in_f, out_f = x.shape[:-1], x.shape[-1], packed.shape[-1]
     if group <= 0 or group % 32:

@@ -21,7 +21,7 @@ from typing import Optional
 import torch
 
 from . import _native as N
-from .attention import _DTYPES, context
+from .attention import _DTYPES, context, has_tangent
 
 
 class PagedKVCache:
@@ -135,6 +135,10 @@ def _no_backward(who: str) -> None:
     raise RuntimeError(f"{who} has no backward: call it under torch.no_grad()")
 
 
+def _no_forward_mode(who: str) -> None:
+    raise RuntimeError(f"{who} has no forward-mode derivative")
+
+
 def paged_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, seq_ids: torch.Tensor,
                  positions: torch.Tensor, rope_base: Optional[float] = None, q: Optional[torch.Tensor] = None,
                  out_q: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
@@ -152,6 +156,8 @@ def paged_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, seq_ids:
     who = "paged_append"
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad)):
         _no_backward(who)
+    if has_tangent(k, v, q):
+        _no_forward_mode(who)
     n = k.shape[0]
     kr, vr = _rows(cache, who, "k", k, n, cache.heads), _rows(cache, who, "v", v, n, cache.heads)
     ids, pos = _indices(cache, who, "seq_ids", seq_ids, n), _indices(cache, who, "positions", positions, n)
@@ -193,6 +199,8 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, seq_lens: torch.Tensor
     who = "paged_attention"
     if q.requires_grad and torch.is_grad_enabled():
         _no_backward(who)
+    if has_tangent(q):
+        _no_forward_mode(who)
     n, heads = cache.num_seqs, q.shape[1] if q.dim() == 3 else 0
     qr = _rows(cache, who, "q", q, n, heads)
     lens = _indices(cache, who, "seq_lens", seq_lens, n)

@@ -209,3 +209,17 @@ def test_sizes_past_the_limits_are_refused():
     for rows, i, o, group in ((1, big, 1, 32), (1, 32, big, 32), (1, 32, 32, big), (16 * 65535 + 1, 32, 32, 32)):
         assert L.hx_linear_w4_fwd(c.handle, 0, p, p, p, None, None, p, rows, i, o, group) == N.HX_ERR_UNSUPPORTED
     assert L.hx_quantize_w4(c.handle, 0, p, p, p, 32, 32, big) == N.HX_ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("mode", [torch.enable_grad, torch.no_grad])
+def test_forward_mode_is_refused(mode):
+    """A dual tensor does not require a gradient, but its tangent must not be lost."""
+    x, packed, scales = _make(2, 64, 32, 32, BF16)
+    bias, res = torch.zeros(32, device="cuda", dtype=BF16), torch.zeros(2, 32, device="cuda", dtype=BF16)
+    args = dict(x=x, scales=scales, bias=bias, residual=res)
+    with mode(), torch.autograd.forward_ad.dual_level():
+        for name, a in args.items():
+            dual = torch.autograd.forward_ad.make_dual(a, torch.ones_like(a))
+            with pytest.raises(RuntimeError):
+                hx.nn.linear_w4(packed=packed, group=32, **{**args, name: dual})
+        hx.nn.linear_w4(packed=packed, group=32, **args)  # without a tangent

@@ -408,3 +408,14 @@ def test_pieces_made_of_nan(dtype, rows, classes):
         r = hx.nn.token_logprobs(x, t, k)
         assert torch.equal(r.top_ids.long(), _order(x)[:, :k])
         assert torch.isnan(r.logprob).all() and torch.isnan(r.entropy).all() and torch.isnan(r.top_logprobs).all()
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor does not require a gradient, but its tangent must not be lost."""
+    x, t = _logits(3, 10, F32), _targets(3, 10)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode(), pytest.raises(NotImplementedError):
+                hx.nn.token_logprobs(dual, t, 2)
+        _check(hx.nn.token_logprobs(x, t), x, t)  # without a tangent

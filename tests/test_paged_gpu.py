@@ -633,3 +633,20 @@ def test_values_near_the_largest(dtype, dim, group, lens):
     _check(q, ks, vs, 4 * dim ** -0.5, o, lse)
     again = hx.paged_attention(cache, q, _lens(*lens), 4 * dim ** -0.5)
     assert torch.equal(o, again[0]) and torch.equal(lse, again[1])
+
+
+@pytest.mark.parametrize("mode", [torch.enable_grad, torch.no_grad])
+def test_forward_mode_is_refused(mode):
+    """A dual tensor does not require a gradient, but its tangent must not be lost."""
+    table = torch.zeros(2, 1, dtype=torch.int32, device="cuda")
+    k = torch.zeros(2, 16, 2, 64, device="cuda", dtype=BF16)
+    cache, lens, x = hx.PagedKVCache(k, k.clone(), table), _lens(1, 1), torch.zeros(2, 2, 64, device="cuda", dtype=BF16)
+    with mode(), torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for bad in (lambda: hx.paged_attention(cache, dual, lens, 1.0), lambda: hx.paged_append(cache, dual, x, lens, lens),
+                    lambda: hx.paged_append(cache, x, dual, lens, lens),
+                    lambda: hx.paged_append(cache, x, x, lens, lens, q=dual)):
+            with pytest.raises(RuntimeError):
+                bad()
+        hx.paged_append(cache, x, x, _lens(0, 1), _lens(0, 0), q=x)  # without a tangent
+        hx.paged_attention(cache, x, lens, 1.0)

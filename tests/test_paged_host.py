@@ -75,3 +75,13 @@ def test_cpu_tensors_are_refused():
     k = torch.zeros(2, 16, 1, 64)
     with pytest.raises(RuntimeError):
         hx.PagedKVCache(k, k, torch.zeros(1, 2, dtype=torch.int32))
+
+
+def test_a_tangent_is_seen():
+    x = torch.ones(3)
+    assert not hx.attention.has_tangent(x, None)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, x)
+        assert not dual.requires_grad and not hx.attention.has_tangent(x, None)
+        assert hx.attention.has_tangent(None, dual) and hx.attention.has_tangent(dual[1:], x)
+    assert not hx.attention.has_tangent(x)
