@@ -66,7 +66,7 @@ class CudaContext:
         N.check(st)
         self.handle = h.value
         self._stream = None  # raw stream last handed to hx_ctx_set_stream
-        self.lock = threading.Lock()  # held from use_stream to the call that follows it
+        self.lock = threading.Lock()  # held from use_stream to the call that follows it and its error message
 
     def close(self) -> None:
         if self.handle:
@@ -87,6 +87,14 @@ class CudaContext:
         if raw != self._stream:
             N.check(N.lib().hx_ctx_set_stream(self.handle, ctypes.c_void_p(raw)), self.handle)
             self._stream = raw
+
+    def call(self, fn, *args) -> None:
+        """The library's `fn` with this context first, on the calling thread's current stream: from any thread."""
+        with self.lock:
+            self.use_stream()
+            st = fn(self.handle, *args)
+            if st:
+                N.check(st, self.handle)
 
     def sync(self) -> None:
         N.check(N.lib().hx_sync(self.handle), self.handle)
@@ -182,24 +190,18 @@ def _check_outputs(ref: torch.Tensor, *outs: Optional[torch.Tensor]) -> None:
             raise ValueError("output tensors must have the inputs' shape, strides, dtype and device")
 
 
-def _ptr(t: Optional[torch.Tensor]):
-    return ctypes.c_void_p(t.data_ptr()) if t is not None else None
-
-
 def attn_forward(q, k, v, scale: float, causal: bool = False, out=None, lse=None):
     """Runs the fused forward. Returns (o, lse[B*H*S] f32)."""
     _check_operands(q, k, v)
     ctx = context(q.device.index)
-    ctx.use_stream()
     shp = _shape_of(q)
     _check_outputs(q, out)
     if out is None:
         out = _like(q)
     if lse is None:
         lse = torch.empty(shp.B * shp.H * shp.S, device=q.device, dtype=torch.float32)
-    N.check(N.lib().hx_attn_fwd_strided(ctx.handle, _DTYPES[q.dtype], ctypes.byref(shp),
-                                        _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse),
-                                        float(scale), int(bool(causal))), ctx.handle)
+    ctx.call(N.lib().hx_attn_fwd_strided, _DTYPES[q.dtype], ctypes.byref(shp), q.data_ptr(), k.data_ptr(),
+             v.data_ptr(), out.data_ptr(), lse.data_ptr(), float(scale), int(bool(causal)))
     return out, lse
 
 
@@ -215,23 +217,17 @@ def attn_backward(q, k, v, o, lse, dout, scale: float, causal: bool = False,
         dout = _like(q).copy_(dout)
     _check_operands(q, k, v, o, dout)
     ctx = context(q.device.index)
-    ctx.use_stream()
     shp = _shape_of(q)
     _check_outputs(q, dq, dk, dv)
     dq = _like(q) if dq is None else dq
     dk = _like(q) if dk is None else dk
     dv = _like(q) if dv is None else dv
+    args = (_DTYPES[q.dtype], ctypes.byref(shp), *(t.data_ptr() for t in (q, k, v, o, dout, lse, dq, dk, dv)), None, 0,
+            float(scale), int(bool(causal)))
     if rope_base is None:
-        N.check(N.lib().hx_attn_bwd_strided(ctx.handle, _DTYPES[q.dtype], ctypes.byref(shp),
-                                            _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(dout),
-                                            _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv), None, 0,
-                                            float(scale), int(bool(causal))), ctx.handle)
+        ctx.call(N.lib().hx_attn_bwd_strided, *args)
     else:
-        N.check(N.lib().hx_attn_bwd_rope_strided(ctx.handle, _DTYPES[q.dtype], ctypes.byref(shp),
-                                                 _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(dout),
-                                                 _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv), None, 0,
-                                                 float(scale), int(bool(causal)),
-                                                 float(rope_base)), ctx.handle)
+        ctx.call(N.lib().hx_attn_bwd_rope_strided, *args, float(rope_base))
     return dq, dk, dv
 
 
@@ -325,12 +321,10 @@ def rope_forward(x: torch.Tensor, base: float, out: Optional[torch.Tensor] = Non
     """Interleaved-pair RoPE on [BH,S,D] / [B,H,S,D] (kernels/rope.rs:5-44)."""
     _check_operands(x)
     ctx = context(x.device.index)
-    ctx.use_stream()
     _check_outputs(x, out)
     out = _like(x) if out is None else out
     shp = _shape_of(x)
-    N.check(N.lib().hx_rope_fwd(ctx.handle, _DTYPES[x.dtype], ctypes.byref(shp), _ptr(x),
-                                _ptr(out), float(base)), ctx.handle)
+    ctx.call(N.lib().hx_rope_fwd, _DTYPES[x.dtype], ctypes.byref(shp), x.data_ptr(), out.data_ptr(), float(base))
     return out
 
 
@@ -341,7 +335,6 @@ def rope_forward_qk(q: torch.Tensor, k: torch.Tensor, base: float, out_q: Option
     if q.shape != k.shape or not _same_strides(q, k):
         raise ValueError("q and k must have the same shape and strides")
     ctx = context(q.device.index)
-    ctx.use_stream()
     _check_outputs(q, out_q)
     _check_outputs(k, out_k)
     out_q = _like(q) if out_q is None else out_q
@@ -349,8 +342,8 @@ def rope_forward_qk(q: torch.Tensor, k: torch.Tensor, base: float, out_q: Option
     if not (_same_strides(out_q, q) and _same_strides(out_k, k)):
         raise ValueError("outputs must have the strides of the inputs")
     shp = _shape_of(q)
-    N.check(N.lib().hx_rope_fwd_qk(ctx.handle, _DTYPES[q.dtype], ctypes.byref(shp), _ptr(q), _ptr(k),
-                                   _ptr(out_q), _ptr(out_k), float(base)), ctx.handle)
+    ctx.call(N.lib().hx_rope_fwd_qk, _DTYPES[q.dtype], ctypes.byref(shp), q.data_ptr(), k.data_ptr(),
+             out_q.data_ptr(), out_k.data_ptr(), float(base))
     return out_q, out_k
 
 
@@ -358,10 +351,8 @@ def rope_backward(g: torch.Tensor, base: float, out: Optional[torch.Tensor] = No
     """Inverse rotation (kernels/rope.rs:46-82)."""
     _check_operands(g)
     ctx = context(g.device.index)
-    ctx.use_stream()
     _check_outputs(g, out)
     out = _like(g) if out is None else out
     shp = _shape_of(g)
-    N.check(N.lib().hx_rope_bwd(ctx.handle, _DTYPES[g.dtype], ctypes.byref(shp), _ptr(g),
-                                _ptr(out), float(base)), ctx.handle)
+    ctx.call(N.lib().hx_rope_bwd, _DTYPES[g.dtype], ctypes.byref(shp), g.data_ptr(), out.data_ptr(), float(base))
     return out

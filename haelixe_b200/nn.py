@@ -18,7 +18,6 @@ through torch.autograd, one Function per op, like the reference's `Op` nodes.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import NamedTuple, Optional
 
@@ -29,22 +28,13 @@ from .attention import _DTYPES, context, flash_attention, has_tangent
 from .paged import PagedKVCache, paged_append, paged_attention
 
 
-def _p(t: Optional[torch.Tensor]):
-    return ctypes.c_void_p(t.data_ptr()) if t is not None else None
-
-
-def _ctx(t: torch.Tensor):
-    if not t.is_cuda:
-        raise RuntimeError("the attention block runs on CUDA tensors")
-    if t.dtype not in _DTYPES:
-        raise TypeError(f"unsupported dtype {t.dtype}; f32 and bf16 are supported")
-    c = context(t.device.index)
-    c.use_stream()
-    return c
+def _p(t: Optional[torch.Tensor]) -> Optional[int]:
+    """t's address; the caller keeps t until the call is made."""
+    return None if t is None else t.data_ptr()
 
 
 def _context_of(t: torch.Tensor):
-    """The context of t's device; the caller holds its lock from use_stream to the call."""
+    """The context of t's device."""
     if not t.is_cuda:
         raise RuntimeError("the attention block runs on CUDA tensors")
     if t.dtype not in _DTYPES:
@@ -55,12 +45,13 @@ def _context_of(t: torch.Tensor):
 class _RMSNormFn(torch.autograd.Function):
     @staticmethod
     def forward(fctx, x, w, eps):
-        c = _ctx(x)
+        c = _context_of(x)
         x = x.contiguous()
         hidden = x.shape[-1]
         y = torch.empty_like(x)
-        N.check(N.lib().hx_rmsnorm_fwd(c.handle, _DTYPES[x.dtype], _p(x), _p(w.contiguous()), _p(y),
-                                       x.numel() // hidden, hidden, float(eps)), c.handle)
+        wc = w.contiguous()
+        c.call(N.lib().hx_rmsnorm_fwd, _DTYPES[x.dtype], x.data_ptr(), wc.data_ptr(), y.data_ptr(), x.numel() // hidden,
+               hidden, float(eps))
         fctx.save_for_backward(x, w)
         fctx.eps = eps
         return y
@@ -68,31 +59,32 @@ class _RMSNormFn(torch.autograd.Function):
     @staticmethod
     def backward(fctx, dy):
         x, w = fctx.saved_tensors
-        c = _ctx(x)
+        c = _context_of(x)
         dy = dy.contiguous()
         hidden = x.shape[-1]
         dx = torch.empty_like(x)
         dw = torch.empty(hidden, dtype=torch.float32, device=x.device)
-        N.check(N.lib().hx_rmsnorm_bwd(c.handle, _DTYPES[x.dtype], _p(dy), _p(x), _p(w.contiguous()), _p(dx),
-                                       _p(dw), x.numel() // hidden, hidden, float(fctx.eps)), c.handle)
+        wc = w.contiguous()
+        c.call(N.lib().hx_rmsnorm_bwd, _DTYPES[x.dtype], dy.data_ptr(), x.data_ptr(), wc.data_ptr(), dx.data_ptr(),
+               dw.data_ptr(), x.numel() // hidden, hidden, float(fctx.eps))
         return dx, dw.to(w.dtype), None
 
 
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(fctx, x, w, b, r=None):
-        c = _ctx(x)
+        c = _context_of(x)
         in_f, out_f = w.shape
         x2 = x.reshape(-1, in_f).contiguous()
         y = torch.empty(x2.shape[0], out_f, dtype=x.dtype, device=x.device)
-        bp = _p(None if b is None else b.contiguous())
+        wc, bc = w.contiguous(), None if b is None else b.contiguous()
         if r is None:
-            N.check(N.lib().hx_linear_fwd(c.handle, _DTYPES[x.dtype], _p(x2), _p(w.contiguous()), bp, _p(y),
-                                          x2.shape[0], in_f, out_f), c.handle)
+            c.call(N.lib().hx_linear_fwd, _DTYPES[x.dtype], x2.data_ptr(), wc.data_ptr(), _p(bc), y.data_ptr(),
+                   x2.shape[0], in_f, out_f)
         else:
             r2 = r.reshape(x2.shape[0], out_f).contiguous()
-            N.check(N.lib().hx_linear_residual_fwd(c.handle, _DTYPES[x.dtype], _p(x2), _p(w.contiguous()), bp,
-                                                   _p(r2), _p(y), x2.shape[0], in_f, out_f), c.handle)
+            c.call(N.lib().hx_linear_residual_fwd, _DTYPES[x.dtype], x2.data_ptr(), wc.data_ptr(), _p(bc),
+                   r2.data_ptr(), y.data_ptr(), x2.shape[0], in_f, out_f)
         fctx.save_for_backward(x2, w)
         fctx.in_shape, fctx.has_bias, fctx.has_res = x.shape, b is not None, r is not None
         return y.view(*x.shape[:-1], out_f)
@@ -100,15 +92,16 @@ class _LinearFn(torch.autograd.Function):
     @staticmethod
     def backward(fctx, dy):
         x2, w = fctx.saved_tensors
-        c = _ctx(x2)
+        c = _context_of(x2)
         in_f, out_f = w.shape
         dy2 = dy.reshape(-1, out_f).contiguous()
         need_x, need_w, need_b = fctx.needs_input_grad[:3]
         dx = torch.empty_like(x2) if need_x else None
         dw = torch.empty_like(w) if need_w else None
         db = torch.empty(out_f, dtype=w.dtype, device=w.device) if (need_b and fctx.has_bias) else None
-        N.check(N.lib().hx_linear_bwd(c.handle, _DTYPES[x2.dtype], _p(x2), _p(w.contiguous()), _p(dy2), _p(dx),
-                                      _p(dw), _p(db), x2.shape[0], in_f, out_f), c.handle)
+        wc = w.contiguous()
+        c.call(N.lib().hx_linear_bwd, _DTYPES[x2.dtype], x2.data_ptr(), wc.data_ptr(), dy2.data_ptr(), _p(dx), _p(dw),
+               _p(db), x2.shape[0], in_f, out_f)
         dr = dy if fctx.has_res else None  # y = r + ...: the residual's gradient is dy itself
         return (None if dx is None else dx.view(fctx.in_shape)), dw, db, dr
 
@@ -116,20 +109,20 @@ class _LinearFn(torch.autograd.Function):
 class _GeluFn(torch.autograd.Function):
     @staticmethod
     def forward(fctx, x):
-        c = _ctx(x)
+        c = _context_of(x)
         x = x.contiguous()
         y = torch.empty_like(x)
-        N.check(N.lib().hx_gelu_fwd(c.handle, _DTYPES[x.dtype], _p(x), _p(y), x.numel()), c.handle)
+        c.call(N.lib().hx_gelu_fwd, _DTYPES[x.dtype], x.data_ptr(), y.data_ptr(), x.numel())
         fctx.save_for_backward(x)
         return y
 
     @staticmethod
     def backward(fctx, dy):
         (x,) = fctx.saved_tensors
-        c = _ctx(x)
+        c = _context_of(x)
         dy = dy.contiguous()
         dx = torch.empty_like(x)
-        N.check(N.lib().hx_gelu_bwd(c.handle, _DTYPES[x.dtype], _p(dy), _p(x), _p(dx), x.numel()), c.handle)
+        c.call(N.lib().hx_gelu_bwd, _DTYPES[x.dtype], dy.data_ptr(), x.data_ptr(), dx.data_ptr(), x.numel())
         return dx
 
 
@@ -142,12 +135,13 @@ def _ids(ids: torch.Tensor) -> torch.Tensor:
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(fctx, ids, table):
-        c = _ctx(table)
+        c = _context_of(table)
         vocab, dim = table.shape
         flat = _ids(ids)
         out = torch.empty(flat.numel(), dim, dtype=table.dtype, device=table.device)
-        N.check(N.lib().hx_embedding_fwd(c.handle, _DTYPES[table.dtype], _p(table.contiguous()), _p(flat), _p(out),
-                                         flat.numel(), vocab, dim), c.handle)
+        rows = table.contiguous()
+        c.call(N.lib().hx_embedding_fwd, _DTYPES[table.dtype], rows.data_ptr(), flat.data_ptr(), out.data_ptr(),
+               flat.numel(), vocab, dim)
         fctx.save_for_backward(flat)
         fctx.vocab, fctx.table_dtype = vocab, table.dtype
         return out.view(*ids.shape, dim)
@@ -155,19 +149,19 @@ class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def backward(fctx, dout):
         (flat,) = fctx.saved_tensors
-        c = _ctx(dout)
+        c = _context_of(dout)
         dim = dout.shape[-1]
         dout = dout.contiguous()
         dtable = torch.zeros(fctx.vocab, dim, dtype=torch.float32, device=dout.device)
-        N.check(N.lib().hx_embedding_bwd(c.handle, _DTYPES[dout.dtype], _p(dout), _p(flat), _p(dtable),
-                                         flat.numel(), fctx.vocab, dim), c.handle)
+        c.call(N.lib().hx_embedding_bwd, _DTYPES[dout.dtype], dout.data_ptr(), flat.data_ptr(), dtable.data_ptr(),
+               flat.numel(), fctx.vocab, dim)
         return None, dtable.to(fctx.table_dtype)
 
 
 class _CrossEntropyFn(torch.autograd.Function):
     @staticmethod
     def forward(fctx, logits, targets):
-        c = _ctx(logits)
+        c = _context_of(logits)
         rows, classes = logits.shape
         logits = logits.contiguous()
         flat = _ids(targets)
@@ -175,8 +169,8 @@ class _CrossEntropyFn(torch.autograd.Function):
             raise ValueError("targets length must match the number of logit rows")
         loss = torch.empty((), dtype=torch.float32, device=logits.device)
         dlogits = torch.empty_like(logits) if fctx.needs_input_grad[0] else None
-        N.check(N.lib().hx_cross_entropy(c.handle, _DTYPES[logits.dtype], _p(logits), _p(flat), _p(loss),
-                                         _p(dlogits), rows, classes), c.handle)
+        c.call(N.lib().hx_cross_entropy, _DTYPES[logits.dtype], logits.data_ptr(), flat.data_ptr(), loss.data_ptr(),
+               _p(dlogits), rows, classes)
         fctx.dlogits = dlogits
         return loss
 
@@ -207,15 +201,8 @@ def _token_logprobs(logits, flat, top_k, with_stats):
     if top_k:
         ids = logits.new_empty((rows, top_k), dtype=torch.int32)
         top = logits.new_empty((rows, top_k), dtype=torch.float32)
-    with c.lock:
-        c.use_stream()
-        st = N.lib().hx_token_logprobs_fwd(c.handle, _DTYPES[logits.dtype], logits.data_ptr(), stride, flat.data_ptr(),
-                                           logprob.data_ptr(), entropy.data_ptr(),
-                                           stats.data_ptr() if with_stats else None, top_k,
-                                           ids.data_ptr() if top_k else None, top.data_ptr() if top_k else None,
-                                           rows, classes)
-        if st:
-            N.check(st, c.handle)
+    c.call(N.lib().hx_token_logprobs_fwd, _DTYPES[logits.dtype], logits.data_ptr(), stride, flat.data_ptr(),
+           logprob.data_ptr(), entropy.data_ptr(), _p(stats), top_k, _p(ids), _p(top), rows, classes)
     return logprob, entropy, ids, top, stats
 
 
@@ -242,13 +229,8 @@ class _TokenLogprobsFn(torch.autograd.Function):
         d = torch.empty_strided((rows, classes), (dstride, 1), dtype=logits.dtype, device=logits.device)
         gl = None if g_logprob is None else g_logprob.contiguous()
         gh = None if g_entropy is None else g_entropy.contiguous()
-        c = _context_of(logits)
-        with c.lock:
-            c.use_stream()
-            N.check(N.lib().hx_token_logprobs_bwd(c.handle, _DTYPES[logits.dtype], logits.data_ptr(), stride,
-                                                  flat.data_ptr(), stats.data_ptr(), None if gl is None else gl.data_ptr(),
-                                                  None if gh is None else gh.data_ptr(), d.data_ptr(), dstride, rows,
-                                                  classes), c.handle)
+        _context_of(logits).call(N.lib().hx_token_logprobs_bwd, _DTYPES[logits.dtype], logits.data_ptr(), stride,
+                                 flat.data_ptr(), stats.data_ptr(), _p(gl), _p(gh), d.data_ptr(), dstride, rows, classes)
         return d, None, None
 
 
@@ -310,10 +292,8 @@ def quantize_w4(weight: torch.Tensor, group: int = 128):
         raise ValueError("group must be a multiple of 32")
     packed = torch.empty(-(-in_f // 8), out_f, dtype=torch.int32, device=w.device)
     scales = torch.empty(-(-in_f // group), out_f, dtype=w.dtype, device=w.device)
-    with c.lock:
-        c.use_stream()
-        N.check(N.lib().hx_quantize_w4(c.handle, _DTYPES[w.dtype], w.data_ptr(), packed.data_ptr(), scales.data_ptr(),
-                                       in_f, out_f, group), c.handle)
+    c.call(N.lib().hx_quantize_w4, _DTYPES[w.dtype], w.data_ptr(), packed.data_ptr(), scales.data_ptr(), in_f, out_f,
+           group)
     return packed, scales
 
 
@@ -357,14 +337,8 @@ def linear_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, group
         rows *= n
     if rows == 0 or out_f == 0:
         return y
-    with c.lock:
-        c.use_stream()
-        st = N.lib().hx_linear_w4_fwd(c.handle, _DTYPES[dt], x.data_ptr(), packed.data_ptr(), scales.data_ptr(),
-                                      None if bias is None else bias.data_ptr(),
-                                      None if residual is None else residual.data_ptr(), y.data_ptr(), rows, in_f, out_f,
-                                      group)
-        if st:
-            N.check(st, c.handle)
+    c.call(N.lib().hx_linear_w4_fwd, _DTYPES[dt], x.data_ptr(), packed.data_ptr(), scales.data_ptr(), _p(bias),
+           _p(residual), y.data_ptr(), rows, in_f, out_f, group)
     return y
 
 

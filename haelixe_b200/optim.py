@@ -62,12 +62,9 @@ class AdamW:
             table.append(t)
         if not table:
             return
-        c = context(dev)
-        c.use_stream()
         arr = (N.AdamWTensor * len(table))(*table)
-        N.check(N.lib().hx_adamw_step(c.handle, ctypes.cast(arr, ctypes.c_void_p), len(table), self.lr,
-                                      self.beta1, self.beta2, self.eps, self.weight_decay, self.step_count),
-                c.handle)
+        context(dev).call(N.lib().hx_adamw_step, ctypes.cast(arr, ctypes.c_void_p), len(table), self.lr, self.beta1,
+                          self.beta2, self.eps, self.weight_decay, self.step_count)
 
     def zero_grad(self) -> None:
         """The reference keeps no gradient buffers (optim.rs:193-199); neither does this."""

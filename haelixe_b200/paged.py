@@ -176,12 +176,7 @@ def paged_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, seq_ids:
         if out_q is not None:
             raise ValueError("paged_append: out_q without q")
         heads, qr, outr = 0, None, None
-    ctx = cache._ctx
-    with ctx.lock:
-        ctx.use_stream()
-        st = N.lib().hx_paged_append(ctx.handle, cache._dt, cache._ref, n, kr, vr, ids, pos, heads, qr, outr, base)
-        if st:
-            N.check(st, ctx.handle)
+    cache._ctx.call(N.lib().hx_paged_append, cache._dt, cache._ref, n, kr, vr, ids, pos, heads, qr, outr, base)
     return out_q
 
 
@@ -214,11 +209,6 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, seq_lens: torch.Tensor
         raise ValueError("paged_attention: lse must be a contiguous f32 [sequences, query heads]")
     # A tensor of the current stream, so that calls on other streams and captured graphs have their own.
     ws = q.new_empty(need, dtype=torch.uint8)
-    ctx = cache._ctx
-    with ctx.lock:
-        ctx.use_stream()
-        st = N.lib().hx_paged_attention(ctx.handle, cache._dt, cache._ref, heads, qr, outr, lse.data_ptr(), lens, scale,
-                                        ws.data_ptr(), need)
-        if st:
-            N.check(st, ctx.handle)
+    cache._ctx.call(N.lib().hx_paged_attention, cache._dt, cache._ref, heads, qr, outr, lse.data_ptr(), lens, scale,
+                    ws.data_ptr(), need)
     return out, lse

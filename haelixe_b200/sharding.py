@@ -131,17 +131,21 @@ class HeadGroup:
         else:
             raise ValueError("the shard must be contiguous as [B, H/N, S, D] or as [B, S, H/N, D]")
         ctx = context(shard.device.index)
-        ctx.use_stream()
-        self._check(N.lib().hx_allgather_heads(
-            self.handle, member, ctx.handle, _DTYPES[shard.dtype], ctypes.c_void_p(shard.data_ptr()),
-            ctypes.c_void_p(merged.data_ptr()) if merged is not None else None, B, Hs, S, D, lay))
+        with ctx.lock:
+            ctx.use_stream()
+            st = N.lib().hx_allgather_heads(
+                self.handle, member, ctx.handle, _DTYPES[shard.dtype], ctypes.c_void_p(shard.data_ptr()),
+                ctypes.c_void_p(merged.data_ptr()) if merged is not None else None, B, Hs, S, D, lay)
+        self._check(st)
         return merged
 
     def wait(self, member: int = 0, device: int | None = None):
         """The current stream waits (on the device) for the member's last gather."""
         ctx = context(self.devices[member] if device is None else device)
-        ctx.use_stream()
-        self._check(N.lib().hx_group_wait(self.handle, member, ctx.handle))
+        with ctx.lock:
+            ctx.use_stream()
+            st = N.lib().hx_group_wait(self.handle, member, ctx.handle)
+        self._check(st)
 
     def sync(self, member: int = 0):
         """Blocks until the member's last gather finished (or the timeout)."""
@@ -179,12 +183,9 @@ def reassemble_heads(gathered: torch.Tensor, out: torch.Tensor, n_shards: int, l
     if n != n_shards:
         raise ValueError("shard count mismatch")
     ctx = context(gathered.device.index)
-    ctx.use_stream()
     lay = {"bhsd": 0, "bshd": 1}[layout]
-    N.check(N.lib().hx_reassemble_heads(ctx.handle, _DTYPES[gathered.dtype],
-                                        ctypes.c_void_p(gathered.data_ptr()),
-                                        ctypes.c_void_p(out.data_ptr()), n, B, Hs, S, D, lay),
-            ctx.handle)
+    ctx.call(N.lib().hx_reassemble_heads, _DTYPES[gathered.dtype], gathered.data_ptr(), out.data_ptr(), n, B, Hs, S, D,
+             lay)
     return out
 
 

@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import haelixe_b200 as hx
+from haelixe_b200 import _native as N
 
 pytestmark = pytest.mark.gpu
 
@@ -149,3 +150,89 @@ def test_refusals():
     with pytest.raises(RuntimeError):  # 4-bit weights have no backward
         stack.quantize_w4(32).loss(torch.zeros(1, 4, dtype=torch.int64, device="cuda"),
                                    torch.zeros(4, dtype=torch.int64, device="cuda"))
+
+
+class _Watched:
+    """The library, with every call that launches work checked for the context's lock."""
+
+    def __init__(self, lib, lock, seen):
+        self._lib, self._lock, self._seen = lib, lock, seen
+
+    def __getattr__(self, name):
+        fn = getattr(self._lib, name)
+        if name in _NO_LAUNCH:
+            return fn
+
+        def call(*args):
+            self._seen[name] = self._seen.get(name, True) and self._lock.locked()
+            return fn(*args)
+        return call
+
+
+_NO_LAUNCH = {"hx_last_error", "hx_status_string", "hx_paged_attention_workspace_size", "hx_sync", "hx_last_path"}
+
+
+def test_every_call_holds_the_context_from_its_stream_to_its_launch(monkeypatch):
+    """Otherwise a call in another thread could change the stream in between."""
+    seen, lib = {}, N.lib()
+    watched = _Watched(lib, hx.context().lock, seen)
+    monkeypatch.setattr(N, "lib", lambda: watched)
+    stack = _stack(BF16)
+    ids = torch.randint(VOCAB, (2, 12), generator=torch.Generator().manual_seed(6)).cuda()
+    stack.loss(ids, ids.reshape(-1)).backward()
+    hx.optim.AdamW(1e-3).step([(p.detach(), p.grad) for p in stack.parameters()])
+    table = torch.arange(4, dtype=torch.int32, device="cuda").view(2, 2)
+    caches = stack.caches(4, 16, table)
+    logits = stack.prefill(ids, caches)
+    at = torch.full((2,), 12, dtype=torch.int32, device="cuda")
+    stack.decode(ids[:, 0], caches, at)
+    stack.quantize_w4(32).decode(ids[:, 0], caches, at)
+    leaf = logits.detach().requires_grad_()
+    hx.nn.token_logprobs(leaf, ids[:, 0]).logprob.sum().backward()
+    x = torch.randn(2, 2, 64, 64, device="cuda", dtype=BF16)
+    q, k = x.clone().requires_grad_(), x.clone()
+    hx.flash_attention(q, k, x, 0.125, True).sum().backward()
+    hx.flash_attention(q.detach().requires_grad_(), k, x, 0.125, True, rope_base=1e4).sum().backward()
+    hx.rope_forward(x, 1e4), hx.rope_backward(x, 1e4), hx.attention.rope_forward_qk(x, k, 1e4)
+    from haelixe_b200 import sharding
+
+    sharding.reassemble_heads(x[None], torch.empty(2, 64, 2, 64, device="cuda", dtype=BF16), 1)
+    assert len(seen) >= 20 and all(seen.values()), [n for n, held in seen.items() if not held]
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_two_threads_decode_on_streams_of_their_own(quantized):
+    """Each with its own stack and caches: the logits of one after the other (cuBLAS may choose
+    other products beside a second stream)."""
+    import threading
+
+    def job(seed, stream, out):
+        (stack, ids, caches, at), logits = out["made"], []
+        with torch.cuda.stream(stream):
+            for i in range(12):
+                logits.append(stack.decode((ids + i) % VOCAB, caches, at + i))
+            stream.synchronize()
+        out["logits"] = torch.stack(logits)
+
+    def make(seed):
+        stack = hx.nn.BlockStack(VOCAB, HIDDEN, HEADS, LAYERS, device="cuda", dtype=BF16, init_std=0.05, seed=seed)
+        prompts = torch.randint(VOCAB, (2, 12), generator=torch.Generator().manual_seed(seed)).cuda()
+        caches = stack.caches(4, 16, torch.arange(4, dtype=torch.int32, device="cuda").view(2, 2))
+        stack.prefill(prompts, caches)
+        if quantized:
+            stack.quantize_w4(32)
+        return stack, prompts[:, 0], caches, torch.full((2,), 12, dtype=torch.int32, device="cuda")
+
+    for turn in range(10):
+        alone, both = [{"made": make(s)} for s in (7, 8)], [{"made": make(s)} for s in (7, 8)]
+        torch.cuda.synchronize()
+        for s in range(2):
+            job(s, torch.cuda.Stream(), alone[s])
+        threads = [threading.Thread(target=job, args=(s, torch.cuda.Stream(), both[s])) for s in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        for a, b in zip(alone, both):
+            _near(b["logits"], a["logits"], BF16)
