@@ -23,6 +23,7 @@
 // join has a fixed order.
 #include <cooperative_groups.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "hx_internal.h"
@@ -526,14 +527,17 @@ cudaError_t launch(cudaStream_t st, int sm_count, Args a) {
     const int skip = ((groups << a.ks_log) - 1) * kUnitK;
     a.skip_rows = skip / a.group, a.skip_rest = skip % a.group;
     const int bytes = Layout(R, CH, 1 << a.wn_log, sizeof(T)).total;
-    static std::atomic<int> allowed[64];  // by device: the shared memory the kernel may have so far
+    auto kernel = linear_w4_kernel<T, NT, CH, L, VEC>;
+    // The kernel may have what its larger form needs, whichever comes first: then it does not matter in which
+    // order threads get here.
+    const int most = std::max(Layout(R, CH, 1, sizeof(T)).total, Layout(R, CH, 2, sizeof(T)).total);
+    static std::atomic<bool> allowed[64];  // by device
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    auto kernel = linear_w4_kernel<T, NT, CH, L, VEC>;
-    if (dev >= 64 || allowed[dev].load(std::memory_order_acquire) < bytes) {
-        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) != cudaSuccess) return e;
-        if (dev < 64) allowed[dev].store(bytes, std::memory_order_release);
+    if (dev >= 64 || !allowed[dev].load(std::memory_order_acquire)) {
+        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most)) != cudaSuccess) return e;
+        if (dev < 64) allowed[dev].store(true, std::memory_order_release);
     }
     if (VEC && (!row_map(&a.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT32, a.packed, (a.in + 7) / 8, a.out, 4, 32, kUnitRows) ||
                 !row_map(&a.x_map, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.x,

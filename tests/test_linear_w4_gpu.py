@@ -223,3 +223,48 @@ def test_forward_mode_is_refused(mode):
             with pytest.raises(RuntimeError):
                 hx.nn.linear_w4(packed=packed, group=32, **{**args, name: dual})
         hx.nn.linear_w4(packed=packed, group=32, **args)  # without a tangent
+
+
+def test_first_calls_of_two_contexts_at_once():
+    """In a process of its own: two threads with a context each make a kernel's first calls, one of a form that needs
+    less shared memory than the other's. Both are launched, then and later."""
+    import subprocess
+    import sys
+
+    code = """
+import threading, torch
+import haelixe_b200 as hx
+from haelixe_b200 import _native as N
+L, bad = N.lib(), []
+ctx = [hx.CudaContext(0), hx.CudaContext(0)]
+stream = torch.cuda.Stream()
+for c in ctx:
+    c.use_stream(stream)
+x = torch.zeros(33, 512, device="cuda")
+y = [torch.zeros(33, 8192, device="cuda") for _ in ctx]
+packed, scales = torch.zeros(64, 8192, dtype=torch.int32, device="cuda"), torch.zeros(16, 8192, device="cuda")
+torch.cuda.synchronize()
+def call(i, dtype, rows, group):
+    out = (8192, 64)[i]
+    st = L.hx_linear_w4_fwd(ctx[i].handle, dtype, x.data_ptr(), packed.data_ptr(), scales.data_ptr(), None, None,
+                            y[i].data_ptr(), rows, 512, out, group)
+    if st:
+        bad.append((out, dtype, rows, group, N.last_error(ctx[i].handle)))
+for dtype in (0, 1):
+    for rows in (8, 16, 33):
+        for group in (32, 64, 128):
+            start = threading.Barrier(2)
+            def go(i):
+                start.wait()
+                call(i, dtype, rows, group)
+            ts = [threading.Thread(target=go, args=(i,)) for i in range(2)]
+            [t.start() for t in ts]
+            [t.join() for t in ts]
+            for i in (0, 1, 0):
+                call(i, dtype, rows, group)
+torch.cuda.synchronize()
+assert not bad, bad
+"""
+    root = __file__.rsplit("/tests/", 1)[0]
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
