@@ -268,3 +268,32 @@ assert not bad, bad
     root = __file__.rsplit("/tests/", 1)[0]
     r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("in_f,out_f,group", [
+    (100, 4612, 32), (136, 8192, 64), (1000, 4612, 96), (2048, 8196, 128), (4104, 4612, 192), (5000, 8192, 32),
+    (8192, 4864, 64), (16384, 4612, 128),
+])
+@pytest.mark.parametrize("rows", [1, 8, 9, 16, 17, 33])
+def test_wide_outputs(dtype, in_f, out_f, group, rows):
+    """Outputs wide enough that two warps share each unit of k, with units that do and do not divide among the
+    groups of warps and the CTAs of a cluster."""
+    x, packed, scales = _make(rows, in_f, out_f, group, dtype, rows + in_f)
+    w = _weight(packed, scales, group, in_f)
+    g = _gen(3)
+    bias, res = (torch.randn(s, generator=g, device="cuda").to(dtype) for s in ((out_f,), (rows, out_f)))
+    y = hx.nn.linear_w4(x, packed, scales, group, bias, res)
+    _check(y, x, w, bias, res)
+    for _ in range(3):
+        assert torch.equal(hx.nn.linear_w4(x, packed, scales, group, bias, res), y)
+
+
+@pytest.mark.parametrize("in_f,group", [(1000, 64), (8200, 128)])
+@pytest.mark.parametrize("rows", [17, 32, 33])
+def test_wide_outputs_of_many_rows(in_f, group, rows):
+    """Over 16 rows in bf16 a CTA is half as wide, so two warps share a unit from half as many columns on."""
+    x, packed, scales = _make(rows, in_f, 2400, group, BF16, rows)
+    y = hx.nn.linear_w4(x, packed, scales, group)
+    _check(y, x, _weight(packed, scales, group, in_f))
+    assert torch.equal(hx.nn.linear_w4(x, packed, scales, group), y)
