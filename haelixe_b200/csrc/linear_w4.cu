@@ -517,16 +517,10 @@ cudaError_t launch(cudaStream_t st, int sm_count, Args a) {
     const int units = (a.in + kUnitK - 1) / kUnitK, R = 8 * NT;
     auto tiles = [&] { return (a.out + (32 * CH << a.wn_log) - 1) / (32 * CH << a.wn_log); };
     // Two warps share a unit, or none where the columns are too few to occupy the SMs (8192 x
-    // 2048 in f32, 5 rows: 7.6 us against 11.0 with two). k is split as long as all CTAs are
-    // resident at once, two an SM, and every group keeps two units (8192 x 8192, 16 rows: 16.8 us
-    // at 128 CTAs, 15.5 at 256, 19.5 at 512).
+    // 2048 in f32, 5 rows: 7.6 us against 11.0 with two).
     a.wn_log = VEC ? 1 : 0;
     if (VEC && 4 * tiles() < sm_count) a.wn_log = 0;
-    const int groups = kWarps >> a.wn_log;
-    while (a.ks_log < 3 && tiles() << a.ks_log <= sm_count && units >= 4 * groups << a.ks_log) ++a.ks_log;
-    const int skip = ((groups << a.ks_log) - 1) * kUnitK;
-    a.skip_rows = skip / a.group, a.skip_rest = skip % a.group;
-    const int bytes = Layout(R, CH, 1 << a.wn_log, sizeof(T)).total;
+    const int groups = kWarps >> a.wn_log, bytes = Layout(R, CH, 1 << a.wn_log, sizeof(T)).total;
     auto kernel = linear_w4_kernel<T, NT, CH, L, VEC>;
     // The kernel may have what its larger form needs, whichever comes first: then it does not matter in which
     // order threads get here.
@@ -539,6 +533,20 @@ cudaError_t launch(cudaStream_t st, int sm_count, Args a) {
         if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most)) != cudaSuccess) return e;
         if (dev < 64) allowed[dev].store(true, std::memory_order_release);
     }
+    // CTAs resident on an SM: one or two, as the form's shared memory allows.
+    static std::atomic<int> known[2];
+    int resident = known[a.wn_log].load(std::memory_order_relaxed);
+    if (resident == 0) {
+        if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, kThreads, bytes)) != cudaSuccess) return e;
+        known[a.wn_log].store(resident, std::memory_order_relaxed);
+    }
+    // k is split as long as all CTAs are resident at once and every group keeps two units (8192 x 8192, 16
+    // rows, two an SM: 16.8 us at 128 CTAs, 15.5 at 256, 19.5 at 512; 16384 x 2048, 16 rows, one an SM: 9.8 us at
+    // 128, 18.6 at 256; 32 rows of 8192 x 2048 8.5 and 11.4; 8192 x 8192 in f32, 16 rows: 29.6 and 33.1).
+    while (a.ks_log < 3 && (int64_t)tiles() << (a.ks_log + 1) <= (int64_t)sm_count * resident && units >= 4 * groups << a.ks_log)
+        ++a.ks_log;
+    const int skip = ((groups << a.ks_log) - 1) * kUnitK;
+    a.skip_rows = skip / a.group, a.skip_rest = skip % a.group;
     if (VEC && (!row_map(&a.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT32, a.packed, (a.in + 7) / 8, a.out, 4, 32, kUnitRows) ||
                 !row_map(&a.x_map, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.x,
                          a.rows, a.in, sizeof(T), 128 / (int)sizeof(T), R)))
