@@ -439,10 +439,15 @@ class MultiHeadAttention:
 
     __call__ = forward
 
+    def _answers(self) -> None:
+        if not self.causal:
+            raise ValueError("answering from a cache needs a causal layer")
+
     def prefill(self, x: torch.Tensor, cache: PagedKVCache, seq_ids: torch.Tensor, positions: torch.Tensor,
                 residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         """forward of prompts [B, S, hidden] from position 0 whose rotated keys and values also enter
-        the cache: token (b, s) at positions[b * S + s] of seq_ids[b * S + s], padding negative."""
+        the cache: token (b, s) at positions[b * S + s] of seq_ids[b * S + s], padding negative. The layer is causal."""
+        self._answers()
         B, S, Hd = x.shape
         H, D = self.num_heads, self.head_dim
         n = self.norm(x)
@@ -455,7 +460,8 @@ class MultiHeadAttention:
     def decode(self, x: torch.Tensor, cache: PagedKVCache, seq_ids: torch.Tensor, positions: torch.Tensor,
                seq_lens: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         """forward of one new token a sequence [sequences, hidden]: its keys and values enter the cache
-        and it attends to the seq_lens positions that are there then."""
+        and it attends to the seq_lens positions that are there then. The layer is causal."""
+        self._answers()
         T, H, D = x.shape[0], self.num_heads, self.head_dim
         n = self.norm(x)
         q, k, v = (p(n).view(T, H, D) for p in (self.q_proj, self.k_proj, self.v_proj))
@@ -577,8 +583,8 @@ class BlockStack:
                 for _ in self.blocks]
 
     def _answers(self, caches) -> None:
-        if not all(b.mha.causal for b in self.blocks):
-            raise ValueError("answering from a cache needs causal blocks")
+        for b in self.blocks:
+            b.mha._answers()
         if len(caches) != len(self.blocks):
             raise ValueError("one cache a block")
 

@@ -236,3 +236,18 @@ def test_two_threads_decode_on_streams_of_their_own(quantized):
         torch.cuda.synchronize()
         for a, b in zip(alone, both):
             _near(b["logits"], a["logits"], BF16)
+
+
+def test_layers_that_are_not_causal_do_not_answer_from_a_cache():
+    """A whole pass of such a layer attends both ways, which neither a causal prompt nor a decode step does."""
+    mha = _stack(BF16, causal=False).blocks[0]
+    cache = _stack(BF16).caches(1, 16, torch.zeros(1, 1, dtype=torch.int32, device="cuda"))[0]
+    x = torch.zeros(1, 4, HIDDEN, device="cuda", dtype=BF16)
+    one = torch.ones(1, dtype=torch.int32, device="cuda")
+    seq, at = torch.zeros(4, dtype=torch.int32, device="cuda"), torch.arange(4, dtype=torch.int32, device="cuda")
+    for layer in (mha, mha.mha):
+        with torch.no_grad(), pytest.raises(ValueError):
+            layer.prefill(x, cache, seq, at)
+        with torch.no_grad(), pytest.raises(ValueError):
+            layer.decode(x[:, 0], cache, one - 1, one - 1, one)
+    assert not cache.k.any() and not cache.v.any()
