@@ -615,7 +615,7 @@ class BlockStack:
         self._answers(caches)
         every = torch.arange(ids.shape[0], dtype=torch.int32, device=ids.device)
         seq_ids = torch.where(positions < 0, -1, every)
-        seq_lens = positions.clamp(min=-1) + 1
+        seq_lens = positions.clamp(-1, 2**31 - 2) + 1  # the last int32 stays outside the table
         x = self.embed(ids)
         for blk, cache in zip(self.blocks, caches):
             x = blk.decode(x, cache, seq_ids, positions, seq_lens)

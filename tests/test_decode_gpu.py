@@ -251,3 +251,11 @@ def test_layers_that_are_not_causal_do_not_answer_from_a_cache():
         with torch.no_grad(), pytest.raises(ValueError):
             layer.decode(x[:, 0], cache, one - 1, one - 1, one)
     assert not cache.k.any() and not cache.v.any()
+
+
+def test_the_last_position_of_an_integer_is_outside_the_table():
+    stack = _stack(BF16)
+    caches = stack.caches(2, 16, torch.arange(2, dtype=torch.int32, device="cuda").view(2, 1))
+    ids = torch.zeros(2, dtype=torch.int64, device="cuda")
+    logits = stack.decode(ids, caches, torch.tensor([0, 2**31 - 1], dtype=torch.int32, device="cuda"))
+    assert torch.isfinite(logits[0]).all() and torch.isnan(logits[1]).all()
