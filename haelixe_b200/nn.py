@@ -590,21 +590,24 @@ class BlockStack:
 
     @torch.no_grad()
     def prefill(self, ids: torch.Tensor, caches: list, lens: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """Prompts [B, S] (row b is sequence b of the caches; its first lens[b] >= 1 ids count, all
-        without lens; the table must hold them) into the caches. Returns the logits [B, vocab] after each prompt's last token."""
+        """Prompts [B, S] (row b is sequence b of the caches; its first lens[b] ids count, all without
+        lens; the table must hold them) into the caches. Returns the logits [B, vocab] after each prompt's
+        last token: NaN for a length outside 1 to S."""
         self._answers(caches)
         B, S = ids.shape
         positions = torch.arange(S, dtype=torch.int32, device=ids.device).repeat(B)
         seq_ids = torch.arange(B, dtype=torch.int32, device=ids.device).repeat_interleave(S)
-        last = torch.full((B,), S - 1, device=ids.device)
+        last, bad = torch.full((B,), S - 1, device=ids.device), None
         if lens is not None:
-            last = lens.to(torch.int64) - 1
+            bad = (lens < 1) | (lens > S)
+            last = (lens.to(torch.int64) - 1).clamp(0, S - 1)
             seq_ids = torch.where(positions < lens.repeat_interleave(S), seq_ids, -1)
         x = self.embed(ids)
         for blk, cache in zip(self.blocks, caches):
             x = blk.prefill(x, cache, seq_ids, positions)
         x = x[torch.arange(B, device=ids.device), last]
-        return self.head(self.norm(x))
+        logits = self.head(self.norm(x))
+        return logits if bad is None else logits.masked_fill_(bad[:, None], float("nan"))
 
     @torch.no_grad()
     def decode(self, ids: torch.Tensor, caches: list, positions: torch.Tensor) -> torch.Tensor:

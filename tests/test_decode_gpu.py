@@ -259,3 +259,17 @@ def test_the_last_position_of_an_integer_is_outside_the_table():
     ids = torch.zeros(2, dtype=torch.int64, device="cuda")
     logits = stack.decode(ids, caches, torch.tensor([0, 2**31 - 1], dtype=torch.int32, device="cuda"))
     assert torch.isfinite(logits[0]).all() and torch.isnan(logits[1]).all()
+
+
+def test_prompt_lengths_outside_the_prompt():
+    """They give NaN logits, and the other prompts what they give alone."""
+    stack = _stack(F32)
+    ids = torch.randint(VOCAB, (6, 9), generator=torch.Generator().manual_seed(9)).cuda()
+    table = torch.arange(6, dtype=torch.int32, device="cuda").view(6, 1)
+    lens = torch.tensor([9, 0, 10, -1, 4, 2**31 - 1], dtype=torch.int32, device="cuda")
+    for n in (lens, lens.long()):
+        logits = stack.prefill(ids, stack.caches(6, 16, table), n)
+        assert torch.isnan(logits[[1, 2, 3, 5]]).all()
+        with torch.no_grad():
+            _near(logits[0], stack(ids[:1])[8], F32)
+            _near(logits[4], stack(ids[4:5])[3], F32)
