@@ -587,6 +587,8 @@ class BlockStack:
             b.mha._answers()
         if len(caches) != len(self.blocks):
             raise ValueError("one cache a block")
+        if any(c.num_seqs != caches[0].num_seqs for c in caches):
+            raise ValueError("the caches must hold the same sequences")
 
     @torch.no_grad()
     def prefill(self, ids: torch.Tensor, caches: list, lens: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -595,6 +597,10 @@ class BlockStack:
         last token: NaN for a length outside 1 to S."""
         self._answers(caches)
         B, S = ids.shape
+        if B > caches[0].num_seqs:
+            raise ValueError(f"{B} prompts for caches of {caches[0].num_seqs} sequences")
+        if lens is None and any(S > c.block_table.shape[1] * c.k.shape[1] for c in caches):
+            raise ValueError(f"the caches' tables do not hold {S} positions")
         positions = torch.arange(S, dtype=torch.int32, device=ids.device).repeat(B)
         seq_ids = torch.arange(B, dtype=torch.int32, device=ids.device).repeat_interleave(S)
         last, bad = torch.full((B,), S - 1, device=ids.device), None
@@ -616,6 +622,8 @@ class BlockStack:
         Returns the logits [B, vocab]: of no use for a sequence that is left out, NaN for a position
         outside the table."""
         self._answers(caches)
+        if ids.shape[0] != caches[0].num_seqs:
+            raise ValueError(f"{ids.shape[0]} ids for caches of {caches[0].num_seqs} sequences")
         every = torch.arange(ids.shape[0], dtype=torch.int32, device=ids.device)
         seq_ids = torch.where(positions < 0, -1, every)
         seq_lens = positions.clamp(-1, 2**31 - 2) + 1  # the last int32 stays outside the table

@@ -273,3 +273,23 @@ def test_prompt_lengths_outside_the_prompt():
         with torch.no_grad():
             _near(logits[0], stack(ids[:1])[8], F32)
             _near(logits[4], stack(ids[4:5])[3], F32)
+
+
+
+def test_more_prompts_or_positions_than_the_table_holds_are_refused():
+    stack = _stack(BF16)
+    caches = stack.caches(4, 16, torch.arange(4, dtype=torch.int32, device="cuda").view(2, 2))
+    stack.prefill(torch.zeros(1, 32, dtype=torch.int64, device="cuda"), caches)
+    before = [c.k.clone() for c in caches]
+    with pytest.raises(ValueError):
+        stack.prefill(torch.zeros(3, 4, dtype=torch.int64, device="cuda"), caches)
+    with pytest.raises(ValueError):
+        stack.prefill(torch.zeros(2, 33, dtype=torch.int64, device="cuda"), caches)
+    for n in (1, 3):
+        with pytest.raises(ValueError):
+            stack.decode(torch.zeros(n, dtype=torch.int64, device="cuda"), caches,
+                         torch.zeros(n, dtype=torch.int32, device="cuda"))
+    assert all(torch.equal(c.k, k) for c, k in zip(caches, before))
+    # A longer padded batch is fine when its lengths fit.
+    lens = torch.tensor([32, 5], dtype=torch.int32, device="cuda")
+    assert torch.isfinite(stack.prefill(torch.zeros(2, 40, dtype=torch.int64, device="cuda"), caches, lens)).all()
