@@ -131,12 +131,14 @@ def _indices(cache: PagedKVCache, who: str, name: str, t: torch.Tensor, n: int) 
     return t.data_ptr()
 
 
-def _no_backward(who: str) -> None:
-    raise RuntimeError(f"{who} has no backward: call it under torch.no_grad()")
-
-
-def _no_forward_mode(who: str) -> None:
-    raise RuntimeError(f"{who} has no forward-mode derivative")
+def _inference(who: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Refuses operands, outputs among them, whose derivative would be lost."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{who} has no backward: call it under torch.no_grad()")
+    if has_tangent(*tensors):
+        raise RuntimeError(f"{who} has no forward-mode derivative")
 
 
 def paged_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, seq_ids: torch.Tensor,
@@ -154,10 +156,7 @@ def paged_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, seq_ids:
     nothing to the cache and NaN to its row of out_q.
     """
     who = "paged_append"
-    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad)):
-        _no_backward(who)
-    if has_tangent(k, v, q):
-        _no_forward_mode(who)
+    _inference(who, cache._k, cache._v, k, v, q, out_q)
     n = k.shape[0]
     kr, vr = _rows(cache, who, "k", k, n, cache.heads), _rows(cache, who, "v", v, n, cache.heads)
     ids, pos = _indices(cache, who, "seq_ids", seq_ids, n), _indices(cache, who, "positions", positions, n)
@@ -192,10 +191,7 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, seq_lens: torch.Tensor
     the cache holds at or past seq_lens is not read.
     """
     who = "paged_attention"
-    if q.requires_grad and torch.is_grad_enabled():
-        _no_backward(who)
-    if has_tangent(q):
-        _no_forward_mode(who)
+    _inference(who, cache._k, cache._v, q, out, lse)
     n, heads = cache.num_seqs, q.shape[1] if q.dim() == 3 else 0
     qr = _rows(cache, who, "q", q, n, heads)
     lens = _indices(cache, who, "seq_lens", seq_lens, n)

@@ -650,3 +650,25 @@ def test_forward_mode_is_refused(mode):
                 bad()
         hx.paged_append(cache, x, x, _lens(0, 1), _lens(0, 0), q=x)  # without a tangent
         hx.paged_attention(cache, x, lens, 1.0)
+
+
+def test_caches_and_outputs_that_need_a_gradient_are_refused():
+    table = torch.zeros(2, 1, dtype=torch.int32, device="cuda")
+    k = torch.zeros(2, 16, 2, 64, device="cuda", dtype=BF16)
+    lens, x = _lens(1, 1), torch.zeros(2, 2, 64, device="cuda", dtype=BF16)
+    leaf = x.clone().requires_grad_()
+    cache = hx.PagedKVCache(k, k.clone(), table)
+    for kv in ((k.clone().requires_grad_(), k.clone()), (k.clone(), k.clone().requires_grad_())):
+        c = hx.PagedKVCache(*kv, table)
+        for call in (lambda: hx.paged_attention(c, x, lens, 1.0), lambda: hx.paged_append(c, x, x, lens, lens)):
+            with pytest.raises(RuntimeError):
+                call()
+            with torch.no_grad():
+                call()
+    for call in (lambda: hx.paged_attention(cache, x, lens, 1.0, out=leaf),
+                 lambda: hx.paged_append(cache, x, x, lens, lens, q=x, out_q=leaf),
+                 lambda: hx.paged_attention(cache, x, lens, 1.0, lse=torch.zeros(2, 2, device="cuda", requires_grad=True))):
+        with pytest.raises(RuntimeError):
+            call()
+        with torch.no_grad():
+            call()
