@@ -7,6 +7,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <functional>
 #include <initializer_list>
 #include <utility>
 
@@ -731,9 +732,40 @@ static bool rows_overlap(int64_t inner, std::initializer_list<std::pair<int64_t,
 static bool operand_overlaps(const hx_rows& r, int rows, int heads, int D) {
     return rows_overlap(D, {{r.stride_row, rows}, {r.stride_head, heads}});
 }
-// Whether two operands that start at the same address are laid out differently.
-static bool clash(const hx_rows& a, const hx_rows& b, int rows, int heads) {
-    return a.data == b.data && ((rows > 1 && a.stride_row != b.stride_row) || (heads > 1 && a.stride_head != b.stride_head));
+// Whether two sets of rows of `width`, one `delta` from the other and both placed by the same strides (largest
+// first, none of them over the one before it; all but the rows of size > 1), have memory in common.
+static bool rows_at_meet(int64_t delta, int64_t width, const std::pair<int64_t, int64_t>* dims, int n) {
+    if (n == 0) return delta > -width && delta < width;
+    const int64_t stride = dims->first, near = -delta / stride;
+    for (int64_t i = near - 1; i <= near + 1; ++i)
+        if (i > -dims->second && i < dims->second && rows_at_meet(delta + i * stride, width, dims + 1, n - 1)) return true;
+    return false;
+}
+static bool rows_meet(const void* a, const void* b, int64_t eb, int64_t width,
+                      std::initializer_list<std::pair<int64_t, int64_t>> strides_sizes) {
+    std::pair<int64_t, int64_t> dims[3];
+    int n = 0;
+    for (const auto& d : strides_sizes)
+        if (d.second > 1) dims[n++] = {d.first * eb, d.second};
+    std::sort(dims, dims + n, std::greater<std::pair<int64_t, int64_t>>());
+    return rows_at_meet((int64_t)((intptr_t)b - (intptr_t)a), width * eb, dims, n);
+}
+// Whether an output of rows that do not overlap has memory in common with an input, unless it is that input. Those
+// of different strides are not looked at row by row: they have it where their extents do.
+static bool clash(const hx_rows& in, const hx_rows& out, int rows, int heads, int D, int64_t eb) {
+    const bool alike = (rows == 1 || in.stride_row == out.stride_row) && (heads == 1 || in.stride_head == out.stride_head);
+    if (alike)
+        return in.data != out.data &&
+               rows_meet(in.data, out.data, eb, D, {{out.stride_row, rows}, {out.stride_head, heads}});
+    intptr_t lo[2], hi[2];
+    const hx_rows* both[2] = {&in, &out};
+    for (int i = 0; i < 2; ++i) {
+        lo[i] = hi[i] = (intptr_t)both[i]->data;
+        const int64_t far[2] = {both[i]->stride_row * (rows - 1) * eb, both[i]->stride_head * (heads - 1) * eb};
+        for (int64_t f : far) (f < 0 ? lo[i] : hi[i]) += f;
+        hi[i] += D * eb;
+    }
+    return lo[0] < hi[1] && lo[1] < hi[0];
 }
 
 static hx::PagedView view_of(const hx_paged_cache& c) {
@@ -773,8 +805,12 @@ int hx_paged_append(hx_ctx* c, hx_dtype dt, const hx_paged_cache* cache, int tok
     if (rows_overlap(cache->D, {{cache->stride_head, cache->H}, {cache->stride_slot, cache->page_size},
                                 {cache->stride_page, cache->num_pages}}))
         return set_error(c, HX_ERR_INVALID, "%s: rows of the cache share memory, so they cannot be written", who);
-    if (Hq > 0 && (operand_overlaps(*q_out, tokens, Hq, cache->D) || clash(*q, *q_out, tokens, Hq)))
-        return set_error(c, HX_ERR_INVALID, "%s: rows of q_out overlap each other, or q at other strides", who);
+    const int64_t eb = dt == HX_F32 ? 4 : 2;
+    if (rows_meet(cache->k, cache->v, eb, cache->D, {{cache->stride_head, cache->H}, {cache->stride_slot, cache->page_size},
+                                                     {cache->stride_page, cache->num_pages}}))
+        return set_error(c, HX_ERR_INVALID, "%s: keys and values of the cache share memory, so they cannot be written", who);
+    if (Hq > 0 && (operand_overlaps(*q_out, tokens, Hq, cache->D) || clash(*q, *q_out, tokens, Hq, cache->D, eb)))
+        return set_error(c, HX_ERR_INVALID, "%s: rows of q_out overlap each other, or q in part", who);
     DeviceGuard g(c->device);
     NvtxRange nv(who);
     LaunchCount lc(c);
@@ -825,8 +861,8 @@ int hx_paged_attention(hx_ctx* c, hx_dtype dt, const hx_paged_cache* cache, int 
     const int64_t eb = dt == HX_F32 ? 4 : 2;
     if (!aligned16(q->data) || (q->stride_row * eb) % 16 || (q->stride_head * eb) % 16)
         return set_error(c, HX_ERR_INVALID, "%s: q and its strides must be 16-byte aligned", who);
-    if (operand_overlaps(*o, cache->num_seqs, Hq, cache->D) || clash(*q, *o, cache->num_seqs, Hq))
-        return set_error(c, HX_ERR_INVALID, "%s: rows of o overlap each other, or q at other strides", who);
+    if (operand_overlaps(*o, cache->num_seqs, Hq, cache->D) || clash(*q, *o, cache->num_seqs, Hq, cache->D, eb))
+        return set_error(c, HX_ERR_INVALID, "%s: rows of o overlap each other, or q in part", who);
     DeviceGuard g(c->device);
     NvtxRange nv(who);
     LaunchCount lc(c);

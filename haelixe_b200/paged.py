@@ -149,7 +149,7 @@ def paged_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, seq_ids:
     Token t is position positions[t] of sequence seq_ids[t] (int32 on the device).
     With rope_base, k is rotated by its position, and so is q [tokens, query
     heads, head_dim], in the same launch; the result is out_q (a new tensor by
-    default; q itself for in place). A negative seq_id marks padding: nothing of
+    default; q itself for in place; memory of its own otherwise). A negative seq_id marks padding: nothing of
     that token is written, its row of out_q included. No two tokens may have the same
     place. A token whose sequence or
     position the table does not hold, or whose entry there is no page, writes
@@ -185,7 +185,7 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, seq_lens: torch.Tensor
 
     q: [sequences, query heads, head_dim], every row on a 16-byte boundary, query
     heads a multiple of the cache's; seq_lens: int32 [sequences] on the device.
-    Returns (o like q, or out, which may be q itself; lse f32 [sequences, query
+    Returns (o like q, or out, which may be q itself or else memory of its own; lse f32 [sequences, query
     heads]). A length of 0 gives zeros and an lse of -inf; a length past the table
     row, or a table entry that is no page, gives NaN. What
     the cache holds at or past seq_lens is not read.

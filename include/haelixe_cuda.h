@@ -257,13 +257,14 @@ typedef struct hx_rows {
  * int32). With rope_base > 0, k is rotated by its position first (the pairs of
  * hx_rope_fwd; the angle is formed in f64, so far positions keep their
  * accuracy), and q ([tokens, Hq, D]; NULL with Hq 0) is rotated into q_out
- * (which may be q itself, at its strides). rope_base 0 writes k, and copies q, as they are.
+ * (which may be q itself, at its strides; refused where it overlaps q otherwise, and
+ * it must not overlap k, v or the cache). rope_base 0 writes k, and copies q, as they are.
  * A token with a negative seq_id is padding: neither the cache nor its q_out
  * row is touched. A token without a slot (sequence or position outside the
  * table, an entry that is no page) writes nothing to the cache and NaN to its
  * q_out row. Two tokens of a call must not have the
  * same slot: it would hold a mixture of both; a cache whose strides give two
- * slots or heads the same memory is refused. */
+ * slots or heads the same memory, or whose keys and values share it, is refused. */
 int hx_paged_append(hx_ctx* ctx, hx_dtype dtype, const hx_paged_cache* cache, int tokens, const hx_rows* k,
                     const hx_rows* v, const int32_t* seq_ids, const int32_t* positions, int Hq, const hx_rows* q,
                     const hx_rows* q_out, float rope_base);
@@ -280,7 +281,8 @@ int hx_paged_attention_workspace_size(hx_dtype dtype, const hx_paged_cache* cach
  * than 2^31 - 256), or that reads an entry that is no page, gives NaN. Positions at or past
  * seq_lens are not read. The result does not depend on what else is in the
  * batch beyond rounding, and equal calls give equal bits. q and its strides
- * (in bytes) are multiples of 16; o needs neither, and may be q itself at q's strides. workspace
+ * (in bytes) are multiples of 16; o needs neither, and may be q itself at q's strides, but
+ * not overlap it otherwise. workspace
  * (256-byte aligned) may be NULL, except during stream capture: the call then
  * takes it from the context's arena. Calls that overlap on the GPU need
  * workspaces of their own. */

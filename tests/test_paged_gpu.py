@@ -623,7 +623,7 @@ def test_values_near_the_largest(dtype, dim, group, lens):
     t = cache.block_table.long()
     for s, n in enumerate(lens):
         j = torch.arange(n, device="cuda")
-        # Of one sign in every second element, of both in the others; keys that score ever higher in sequence 0.
+        # Of one sign in every second element, of both in the others.
         v = (1 + torch.rand(n, 2, dim, generator=_gen(84 + s), device="cuda")) * 2.0 ** 126
         v[..., 1::2] *= torch.sign(torch.randn(n, 2, dim // 2, generator=_gen(94 + s), device="cuda"))
         vs[s] = v.to(dtype)
@@ -672,3 +672,45 @@ def test_caches_and_outputs_that_need_a_gradient_are_refused():
             call()
         with torch.no_grad():
             call()
+
+
+def test_outputs_that_overlap_their_inputs_in_part_are_refused():
+    """An output may be its input; it may not begin inside it."""
+    table = torch.zeros(2, 1, dtype=torch.int32, device="cuda")
+    k = torch.zeros(2, 16, 2, 64, device="cuda", dtype=BF16)
+    cache, lens = hx.PagedKVCache(k, k.clone(), table), _lens(1, 1)
+    buf = torch.zeros(4, 2, 64, device="cuda", dtype=BF16)
+    wide = torch.zeros(2, 4, 64, device="cuda", dtype=BF16)
+    flat = torch.zeros(1024, device="cuda", dtype=BF16)
+    for q, out in ((buf[:2], buf[1:3]), (buf[1:3], buf[:2]), (wide[:, :2], wide[:, 1:3]),
+                   (flat[:256].view(2, 2, 64), flat[64:320].view(2, 2, 64)), (flat[:256].view(2, 2, 64), flat[8:264].view(2, 2, 64)),
+                   (flat[128:384].view(2, 2, 64), flat.as_strided((2, 2, 64), (256, 64, 1)))):
+        with pytest.raises(N.HxError):
+            hx.paged_attention(cache, q, lens, 1.0, out=out)
+        with pytest.raises(N.HxError):
+            hx.paged_append(cache, q, q, lens, lens, q=q, out_q=out)
+    # Heads of one buffer side by side do not overlap.
+    wide.normal_(generator=_gen(1))
+    want = wide[:, :2].clone()
+    hx.paged_append(cache, want, want, _lens(0, 1), _lens(0, 1), q=wide[:, :2], out_q=wide[:, 2:])
+    assert torch.equal(wide[:, 2:], want) and torch.equal(wide[:, :2], want)
+    out = torch.zeros(2, 2, 192, device="cuda", dtype=BF16)
+    hx.paged_attention(cache, out[:, :, :64], lens, 1.0, out=out[:, :, 64:128])
+
+
+def test_keys_and_values_in_the_same_memory_are_for_reading():
+    table = torch.zeros(1, 2, dtype=torch.int32, device="cuda")
+    k = torch.randn(2, 16, 2, 64, generator=_gen(2), device="cuda", dtype=BF16)
+    x, one = torch.zeros(1, 2, 64, device="cuda", dtype=BF16), _lens(0)
+    both = torch.zeros(2, 16, 4, 64, device="cuda", dtype=BF16)
+    pages = torch.zeros(3, 16, 2, 64, device="cuda", dtype=BF16)
+    for kv in ((k, k), (both[:, :, :2], both[:, :, 1:3]), (pages[:2], pages[1:])):
+        cache = hx.PagedKVCache(*kv, table)
+        hx.paged_attention(cache, x, _lens(1), 1.0)
+        with pytest.raises(N.HxError):
+            hx.paged_append(cache, x, x, one, one)
+    for kv in ((both[:, :, :2], both[:, :, 2:]), (pages[:1], pages[1:2]), (pages[:, :, :, :32], pages[:, :, :, 32:])):
+        cache = hx.PagedKVCache(*kv, table)
+        y = torch.ones(1, 2, kv[0].shape[3], device="cuda", dtype=BF16)
+        hx.paged_append(cache, y, 2 * y, one, one)
+        assert (kv[0][0, 0] == 1).all() and (kv[1][0, 0] == 2).all()
