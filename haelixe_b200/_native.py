@@ -173,6 +173,12 @@ def lib():
     return _lib
 
 
+def check_sizes(who: str, *sizes: int) -> None:
+    """Refuses sizes past the C ABI's int, which ctypes would cut to their low 32 bits."""
+    if max(sizes) > 0x7fffffff:
+        raise ValueError(f"{who}: sizes must be below 2^31, got {max(sizes)}")
+
+
 def last_error(ctx) -> str:
     buf = ctypes.create_string_buffer(512)
     lib().hx_last_error(ctx, buf, 512)

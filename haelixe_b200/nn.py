@@ -260,6 +260,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0) 
     [0, classes) gives NaN; so does a row with NaN, +inf or no finite logit."""
     if logits.dim() != 2 or logits.stride(1) != 1 and logits.shape[1] > 1:
         raise ValueError("logits must be [rows, classes] with contiguous rows")
+    N.check_sizes("token_logprobs", *logits.shape)
     if logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]:
         logits = logits.contiguous()
     flat = targets
@@ -285,6 +286,7 @@ def quantize_w4(weight: torch.Tensor, group: int = 128):
     weight is about (q - 8) * scale."""
     if weight.dim() != 2:
         raise ValueError("weight must be [in, out]")
+    N.check_sizes("quantize_w4", *weight.shape, group)
     c = _context_of(weight)
     w = weight.detach().contiguous()
     in_f, out_f = w.shape
@@ -330,11 +332,12 @@ def linear_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, group
         residual = residual.contiguous()
     if scales.dtype is not dt or scales.get_device() != dev or packed.get_device() != dev:
         raise ValueError("packed and scales must be on x's device, scales in its dtype")
-    x = x.contiguous()
-    y = x.new_empty(shape)
     rows = 1
     for n in lead:
         rows *= n
+    N.check_sizes("linear_w4", rows, in_f, out_f, group)
+    x = x.contiguous()
+    y = x.new_empty(shape)
     if rows == 0 or out_f == 0:
         return y
     c.call(N.lib().hx_linear_w4_fwd, _DTYPES[dt], x.data_ptr(), packed.data_ptr(), scales.data_ptr(), _p(bias),

@@ -52,6 +52,7 @@ class PagedKVCache:
         if block_table.shape[1] > 1 and block_table.stride(1) != 1:
             raise ValueError("rows of block_table must be contiguous")
         pages, slots, heads, dim = k.shape
+        N.check_sizes("the paged cache", *k.shape, *block_table.shape)
         # The stride of a dimension of size 1 never moves an address: give it one that is in order.
         sh = k.stride(2) if heads > 1 else dim
         ss = k.stride(1) if slots > 1 else max(dim, heads * sh)
@@ -158,6 +159,7 @@ def paged_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, seq_ids:
     who = "paged_append"
     _inference(who, cache._k, cache._v, k, v, q, out_q)
     n = k.shape[0]
+    N.check_sizes(who, n)
     kr, vr = _rows(cache, who, "k", k, n, cache.heads), _rows(cache, who, "v", v, n, cache.heads)
     ids, pos = _indices(cache, who, "seq_ids", seq_ids, n), _indices(cache, who, "positions", positions, n)
     base = 0.0

@@ -297,3 +297,13 @@ def test_wide_outputs_of_many_rows(in_f, group, rows):
     y = hx.nn.linear_w4(x, packed, scales, group)
     _check(y, x, _weight(packed, scales, group, in_f))
     assert torch.equal(hx.nn.linear_w4(x, packed, scales, group), y)
+
+
+def test_sizes_past_an_int_are_refused():
+    x, packed, scales = _make(1, 64, 32, 32, BF16)
+    with pytest.raises(ValueError):
+        hx.nn.linear_w4(x.expand(2**32 + 1, 64), packed, scales, 32)
+    with pytest.raises(ValueError):
+        hx.nn.linear_w4(x, packed, scales[:1], 2**32 + 64)  # would be a group of 64
+    with pytest.raises(ValueError):
+        hx.nn.quantize_w4(x[:, :1].expand(1, 2**32 + 1))

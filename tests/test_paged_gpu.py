@@ -714,3 +714,15 @@ def test_keys_and_values_in_the_same_memory_are_for_reading():
         y = torch.ones(1, 2, kv[0].shape[3], device="cuda", dtype=BF16)
         hx.paged_append(cache, y, 2 * y, one, one)
         assert (kv[0][0, 0] == 1).all() and (kv[1][0, 0] == 2).all()
+
+
+def test_sizes_past_an_int_are_refused():
+    """2^32 + 1 pages (one, at stride 0) or sequences would otherwise be taken for one."""
+    k = torch.zeros(1, 16, 1, 8, device="cuda", dtype=BF16)
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    for kv, t in ((k.expand(2**32 + 1, 16, 1, 8), table), (k, table.expand(2**32 + 1, 1))):
+        with pytest.raises(ValueError):
+            hx.PagedKVCache(kv, kv, t)
+    cache = hx.PagedKVCache(k, k.clone(), table)
+    with pytest.raises(ValueError):
+        hx.paged_append(cache, k[0, :1].expand(2**32 + 1, 1, 8), k[0, :1].expand(2**32 + 1, 1, 8), _lens(0), _lens(0))

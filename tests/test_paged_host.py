@@ -85,3 +85,14 @@ def test_a_tangent_is_seen():
         assert not dual.requires_grad and not hx.attention.has_tangent(x, None)
         assert hx.attention.has_tangent(None, dual) and hx.attention.has_tangent(dual[1:], x)
     assert not hx.attention.has_tangent(x)
+
+
+def test_sizes_past_an_int_are_refused():
+    """ctypes keeps the low 32 bits of a larger one, so 2^32 + 1 rows would be one."""
+    assert ctypes.c_int(2**32 + 1).value == 1
+    N.check_sizes("x", 0, 1, 2**31 - 1)
+    for n in (2**31, 2**32 + 1):
+        with pytest.raises(ValueError):
+            N.check_sizes("x", 5, n)
+    with pytest.raises(ValueError):
+        hx.nn.token_logprobs(torch.zeros(1, 4).expand(2**32 + 1, 4), torch.zeros(1, dtype=torch.int32).expand(2**32 + 1))
