@@ -207,6 +207,6 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, seq_lens: torch.Tensor
         raise ValueError("paged_attention: lse must be a contiguous f32 [sequences, query heads]")
     # A tensor of the current stream, so that calls on other streams and captured graphs have their own.
     ws = q.new_empty(need, dtype=torch.uint8)
-    cache._ctx.call(N.lib().hx_paged_attention, cache._dt, cache._ref, heads, qr, outr, lse.data_ptr(), lens, scale,
+    cache._ctx.call(N.lib().hx_paged_attention, cache._dt, cache._ref, heads, qr, outr, lse.data_ptr(), lens, float(scale),
                     ws.data_ptr(), need)
     return out, lse

@@ -726,3 +726,14 @@ def test_sizes_past_an_int_are_refused():
     cache = hx.PagedKVCache(k, k.clone(), table)
     with pytest.raises(ValueError):
         hx.paged_append(cache, k[0, :1].expand(2**32 + 1, 1, 8), k[0, :1].expand(2**32 + 1, 1, 8), _lens(0), _lens(0))
+
+
+def test_scales_of_any_number_type():
+    import numpy as np
+
+    cache, ks, vs = _filled(90, BF16, [33], 16, 2, 64)
+    q = torch.randn(1, 2, 64, generator=_gen(91), device="cuda", dtype=BF16)
+    want = hx.paged_attention(cache, q, _lens(33), 0.25)
+    for scale in (np.float32(0.25), np.float64(0.25), torch.tensor(0.25)):
+        got = hx.paged_attention(cache, q, _lens(33), scale)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
