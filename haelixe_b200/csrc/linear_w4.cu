@@ -7,11 +7,13 @@
 // a byte a weight the memory delivers about 90 weights a clock and SM. Two nibbles
 // become two bf16 in two instructions and a half (see Unpack), and the
 // warp's tensor product multiplies them, so that the f32 pipes only see one scale a
-// group. 16 rows of 8192 x 8192 in groups of 64 take 15.4 us, of which reading is 5.6: bound by the
-// instructions that unpack and multiply, and by filling and joining within so short a call.
-// The order of k inside a product is free as long as both operands agree, so the weights go from a 16-byte global load (4 columns of 8 k) to fragments
-// with no shared memory. q - 8 and bf16 x are exact operands; f32 x is cut into
-// three bf16 that sum to it exactly, three products for one.
+// group. 16 rows of 8192 x 8192 in groups of 64 take 15.2 us, of which reading is 5.6. No pipe is full then
+// (issue slots 44 %, ALU 34 %, tensor 28 %): the 3.5 warps of a scheduler issue once in 8 cycles each, so the
+// latency of unpacking and multiplying bounds it, and filling and joining within so short a call.
+// The order of k inside a product is free as long as both operands agree, so one 16-byte read of a stage
+// (4 columns of 8 k) is the weights' fragments of four products, with nothing exchanged between lanes.
+// q - 8 and bf16 x are exact operands; f32 x is cut into three bf16 that sum to it
+// exactly (from 2^-109 up; below, to bf16's smallest step of 2^-133), three products for one.
 //
 // A CTA's 8 warps form k groups of wn warps: a group takes every so many units of 128 k of
 // 64 wn columns (32 wn for over 16 rows), each warp its own columns. A unit's weights and x come
@@ -38,7 +40,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
-constexpr int kStep = 32;  // k of a warp's tensor products, one 16-byte load of weights a lane and 32 columns
+constexpr int kStep = 32;  // k of a warp's tensor products: a lane's one 16-byte read of weights for 32 columns
 
 struct Args {
     CUtensorMap w_map, x_map;

@@ -13,8 +13,8 @@
 // two a worker, and paged_join_kernel joins an item's parts in the order of its
 // keys (no atomics: the same call gives the same bits).
 //
-// Softmax statistics and all sums are f32. A warp keeps a running maximum that
-// only moves when a score passes it by 2^8, so the accumulator is rarely rescaled.
+// Softmax statistics and all sums are f32. A warp keeps a running maximum; in bf16 it
+// only moves when a score passes it by 2^8, so that the accumulator is rarely rescaled.
 // Positions at or past len are never read: their pages may hold anything.
 #include <atomic>
 #include <type_traits>
@@ -22,6 +22,7 @@
 #include "hx_internal.h"
 #include "launch.h"
 #include "mma_bf16.cuh"
+#include "sm100_ptx.cuh"
 
 namespace hx {
 namespace {
@@ -173,12 +174,7 @@ __device__ __forceinline__ float safe_max(float m) { return m == -INFINITY ? 0.f
 // A part in the workspace: o of HB heads, then (max, sum) of each, a multiple of 16 bytes.
 __host__ __device__ constexpr int part_floats(int HB, int D) { return HB * (D + 4); }
 
-// 2^x to 2^-22, flushing denormals: for weights and probabilities.
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
+using ptx::ex2;  // to 2^-22, denormals as 0
 
 // Bits whose upper half is the largest bf16 below p > 0; 0 of 0, NaN of NaN.
 __device__ __forceinline__ uint32_t below(float p) {
