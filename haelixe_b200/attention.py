@@ -34,7 +34,7 @@ _DTYPES = {torch.float32: N.HX_F32, torch.bfloat16: N.HX_BF16}
 
 def has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
     """Whether one of them is a dual tensor of forward-mode differentiation, which requires_grad does not
-    show. (Outside a dual level none is, and one attribute is read.)"""
+    show. (Outside a dual level, at forward_ad._current_level -1, none is.)"""
     return forward_ad._current_level >= 0 and \
         any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
@@ -91,7 +91,8 @@ class CudaContext:
     def call(self, fn, *args) -> None:
         """The library's `fn` with this context first, on the calling thread's current stream: from any thread."""
         with self.lock:
-            self.use_stream()
+            if torch._C._cuda_getCurrentRawStream(self.device) != self._stream:
+                self.use_stream()
             st = fn(self.handle, *args)
             if st:
                 N.check(st, self.handle)

@@ -22,6 +22,7 @@ import math
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 from .attention import _DTYPES, context, flash_attention, has_tangent
@@ -202,7 +203,8 @@ def _token_logprobs(logits, flat, top_k, with_stats):
         ids = logits.new_empty((rows, top_k), dtype=torch.int32)
         top = logits.new_empty((rows, top_k), dtype=torch.float32)
     c.call(N.lib().hx_token_logprobs_fwd, _DTYPES[logits.dtype], logits.data_ptr(), stride, flat.data_ptr(),
-           logprob.data_ptr(), entropy.data_ptr(), _p(stats), top_k, _p(ids), _p(top), rows, classes)
+           logprob.data_ptr(), entropy.data_ptr(), stats.data_ptr() if with_stats else None, top_k,
+           ids.data_ptr() if top_k else None, top.data_ptr() if top_k else None, rows, classes)
     return logprob, entropy, ids, top, stats
 
 
@@ -260,7 +262,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0) 
     [0, classes) gives NaN; so does a row with NaN, +inf or no finite logit."""
     if logits.dim() != 2 or logits.stride(1) != 1 and logits.shape[1] > 1:
         raise ValueError("logits must be [rows, classes] with contiguous rows")
-    N.check_sizes("token_logprobs", *logits.shape)
+    if max(logits.shape) > 0x7fffffff:
+        N.check_sizes("token_logprobs", *logits.shape)
     if logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]:
         logits = logits.contiguous()
     flat = targets
@@ -274,7 +277,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0) 
     if not 0 <= top_k <= min(32, logits.shape[1]):
         raise ValueError("top_k must be 0 to 32 and at most the number of classes")
     # A dual tensor goes there too: autograd refuses it, for there is no forward-mode derivative.
-    if logits.requires_grad and torch.is_grad_enabled() or has_tangent(logits):
+    if logits.requires_grad and torch.is_grad_enabled() or forward_ad._current_level >= 0 and has_tangent(logits):
         return TokenLogprobs(*_TokenLogprobsFn.apply(logits, flat, top_k))
     return TokenLogprobs(*_token_logprobs(logits, flat, top_k, False)[:4])
 
@@ -307,7 +310,7 @@ def linear_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, group
     if torch.is_grad_enabled() and (x.requires_grad or scales.requires_grad or (bias is not None and bias.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
         raise RuntimeError("linear_w4 has no backward: call it under torch.no_grad()")
-    if has_tangent(x, scales, bias, residual):
+    if forward_ad._current_level >= 0 and has_tangent(x, scales, bias, residual):
         raise RuntimeError("linear_w4 has no forward-mode derivative")
     c = _context_of(x)
     lead, in_f, out_f = x.shape[:-1], x.shape[-1], packed.shape[-1]
@@ -335,13 +338,15 @@ def linear_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, group
     rows = 1
     for n in lead:
         rows *= n
-    N.check_sizes("linear_w4", rows, in_f, out_f, group)
+    if max(rows, in_f, out_f, group) > 0x7fffffff:
+        N.check_sizes("linear_w4", rows, in_f, out_f, group)
     x = x.contiguous()
     y = x.new_empty(shape)
     if rows == 0 or out_f == 0:
         return y
-    c.call(N.lib().hx_linear_w4_fwd, _DTYPES[dt], x.data_ptr(), packed.data_ptr(), scales.data_ptr(), _p(bias),
-           _p(residual), y.data_ptr(), rows, in_f, out_f, group)
+    c.call(N.lib().hx_linear_w4_fwd, _DTYPES[dt], x.data_ptr(), packed.data_ptr(), scales.data_ptr(),
+           None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(), y.data_ptr(),
+           rows, in_f, out_f, group)
     return y
 
 

@@ -19,6 +19,7 @@ import struct
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 from .attention import _DTYPES, context, has_tangent
@@ -132,14 +133,9 @@ def _indices(cache: PagedKVCache, who: str, name: str, t: torch.Tensor, n: int) 
     return t.data_ptr()
 
 
-def _inference(who: str, *tensors: Optional[torch.Tensor]) -> None:
-    """Refuses operands, outputs among them, whose derivative would be lost."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{who} has no backward: call it under torch.no_grad()")
-    if has_tangent(*tensors):
-        raise RuntimeError(f"{who} has no forward-mode derivative")
+def _refuse_derivative(who: str, grad: bool) -> None:
+    raise RuntimeError(f"{who} has no backward: call it under torch.no_grad()" if grad else
+                       f"{who} has no forward-mode derivative")
 
 
 def paged_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, seq_ids: torch.Tensor,
@@ -157,9 +153,14 @@ def paged_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, seq_ids:
     nothing to the cache and NaN to its row of out_q.
     """
     who = "paged_append"
-    _inference(who, cache._k, cache._v, k, v, q, out_q)
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or cache._k.requires_grad or cache._v.requires_grad
+                                    or q is not None and q.requires_grad or out_q is not None and out_q.requires_grad):
+        _refuse_derivative(who, True)
+    if forward_ad._current_level >= 0 and has_tangent(cache._k, cache._v, k, v, q, out_q):
+        _refuse_derivative(who, False)
     n = k.shape[0]
-    N.check_sizes(who, n)
+    if n > 0x7fffffff:
+        N.check_sizes(who, n)
     kr, vr = _rows(cache, who, "k", k, n, cache.heads), _rows(cache, who, "v", v, n, cache.heads)
     ids, pos = _indices(cache, who, "seq_ids", seq_ids, n), _indices(cache, who, "positions", positions, n)
     base = 0.0
@@ -193,7 +194,11 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, seq_lens: torch.Tensor
     the cache holds at or past seq_lens is not read.
     """
     who = "paged_attention"
-    _inference(who, cache._k, cache._v, q, out, lse)
+    if torch.is_grad_enabled() and (q.requires_grad or cache._k.requires_grad or cache._v.requires_grad or
+                                    out is not None and out.requires_grad or lse is not None and lse.requires_grad):
+        _refuse_derivative(who, True)
+    if forward_ad._current_level >= 0 and has_tangent(cache._k, cache._v, q, out, lse):
+        _refuse_derivative(who, False)
     n, heads = cache.num_seqs, q.shape[1] if q.dim() == 3 else 0
     qr = _rows(cache, who, "q", q, n, heads)
     lens = _indices(cache, who, "seq_lens", seq_lens, n)
