@@ -39,6 +39,9 @@ constexpr int kLazy = 8;  // log2 growth of the maximum that triggers a rescale
 // and no sum passes the largest value, however large that is; the division by the probabilities' sum takes it
 // back. A power of two, so it changes no bit of a result unless values are under 2^-100 or so.
 __device__ __forceinline__ int shrink_of(int len) { return __clz(len) - 32 - kLazy; }
+// Of normal numbers. (The workers take exp2f, which gives powers of two exactly as well: made of bits, the number is
+// no register's own to the compiler, and 64 sequences of 16 heads of 64 take 27.8 us for 26.4.)
+__device__ __forceinline__ float power_of_two(int n) { return __int_as_float((127 + n) << 23); }
 constexpr float kLn2 = 0.69314718055994530942f;
 
 struct Item {
@@ -211,7 +214,7 @@ __device__ __forceinline__ void finish_item(const PagedAttn& a, const Parts<HB, 
                 T v[4];
             } four;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) four.v[e] = T(o[e] / l * exp2f((float)-shrink_of(len)));
+            for (int e = 0; e < 4; ++e) four.v[e] = T(o[e] / l * power_of_two(-shrink_of(len)));
             if (a.o_vec) {
                 *reinterpret_cast<Four*>(to) = four;
             } else {
@@ -237,7 +240,7 @@ __device__ __forceinline__ void finish_item(const PagedAttn& a, const Parts<HB, 
 // layout to the second's by an 8x8 transpose, as bf16 hi + lo, so that the
 // result carries only its own rounding. hi is the largest bf16 below p, not the nearest, and so lo is
 // more than 0: both products with an infinite value then are that infinity (0 times it, or less than 0,
-// would make NaN of it; it still does for weights under 2^-110 of 1).
+// would make NaN of it; for weights that shrink_of takes under 2^-110 lo is 0 all the same).
 // K of the next step is loaded as soon as the scores are taken, V as soon as P V is,
 // so one of the two is always in flight. (Loading the worker's next item's while one is joined
 // and stored gained nothing: the SM's other workers are in the middle of theirs.)
@@ -818,7 +821,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(PagedAttn a
 #pragma unroll
         for (int w = 0; w < kJoinWarps; ++w)
             if (w < warps) s += f[w] * so[w][d];
-        o[d] = T(s / l * exp2f((float)-shrink_of(a.lens[n])));
+        o[d] = T(s / l * power_of_two(-shrink_of(a.lens[n])));
     }
     if (threadIdx.x == 0 && lse) *lse = (m + log2f(l)) * kLn2;
 }
