@@ -7,7 +7,7 @@
 // a byte a weight the memory delivers about 90 weights a clock and SM. Two nibbles
 // become two bf16 in two instructions and a half (see Unpack), and the
 // warp's tensor product multiplies them, so that the f32 pipes only see one scale a
-// group. 16 rows of 8192 x 8192 in groups of 64 take 15.2 us, of which reading is 5.6. No pipe is full then
+// group. 16 rows of 8192 x 8192 in groups of 64 take 15.0 us, of which reading is 5.6. No pipe is full then
 // (issue slots 44 %, ALU 34 %, tensor 28 %): the 3.5 warps of a scheduler issue once in 8 cycles each, so the
 // latency of unpacking and multiplying bounds it, and filling and joining within so short a call.
 // The order of k inside a product is free as long as both operands agree, so one 16-byte read of a stage
