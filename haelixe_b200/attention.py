@@ -59,9 +59,10 @@ class CudaAllocation:
 class CudaContext:
     """One per device: stream, binning arena, device status word.
 
-    Calls may come from several threads, each on its thread's current stream. Those that take scratch from the
-    arena (backward passes, cross_entropy, f32 attention over whole sequences) have to be ordered by the caller when they are on
-    several streams: a slab goes to the next call when the one before is enqueued, in the order of one stream.
+    Calls may come from several threads, each on its thread's current stream. Those that
+    take scratch from the arena (backward passes, cross_entropy, f32 attention over whole
+    sequences) have to be ordered by the caller when they are on several streams: a slab
+    goes to the next call when the one before is enqueued, in the order of one stream.
     """
 
     def __init__(self, device: int = 0):
